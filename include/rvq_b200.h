@@ -583,6 +583,157 @@ int rvq_kmeans_step(const float* x, int64_t n, const float* centroids, int k, in
  * the bytes are on the device (it waits for its own copies only). */
 int rvq_pack_load(const char* path, uint64_t offset, uint64_t nbytes, void* device_dst, void* stream);
 
+/* ---- Prompt attention --------------------------------------------------------
+ * Attention of whole prompts, grouped heads (head h reads kv head
+ * h / (n_heads / n_kv)), several sequences packed one behind the other:
+ * sequence b has queries cu_q[b] .. cu_q[b+1] - 1 and keys cu_k[b] ..
+ * cu_k[b+1] - 1 (lq and lk of them), and query i sees the keys
+ *   j < min(lk, i + 1 + lk - lq)   (causal: the last query sees every key)
+ *   j < lk                         (not causal).
+ *   s_j = scaling * (q_i . k_j) in fp32; out_i = sum_j softmax(s)_j v_j;
+ *   lse_i = log(sum_j exp(s_j)).
+ * A query that sees no key, or whose every score is -infinity, gets zeros (lse
+ * -infinity).  Rows of out and lse
+ * behind the last sequence (and in front of the first) are left as they were.
+ * Softmax statistics and sums are fp32; the probabilities are rounded to the
+ * operand type for the product with v.  What no query may see (later keys,
+ * other sequences, rows behind the last sequence) may hold anything, NaN and
+ * infinities included.  Replaces the score matrices of the reference's prompt
+ * pass (eager attention, infer_compressed_layerwise_triton.py:64-65, 290-292). */
+typedef struct rvq_prompt_attn_args {
+    const void* q;            /* device [tokens][n_heads][head_dim], strides below */
+    const void* k;            /* device [keys][n_kv][head_dim] */
+    const void* v;
+    void* out;                /* device [tokens][n_heads][head_dim]; overlaps no input */
+    float* lse;               /* device [n_heads][tokens], or NULL */
+    const int32_t* cu_q;      /* device [n_seq + 1], ascending; NULL: one sequence of all tokens and all keys */
+    const int32_t* cu_k;      /* device [n_seq + 1]; NULL: the same as cu_q */
+    int64_t tokens;
+    int64_t keys;
+    int64_t q_stride[2];      /* elements from token to token and from head to head, multiples of 8; */
+    int64_t k_stride[2];      /* the head_dim elements of a head are adjacent */
+    int64_t v_stride[2];
+    int64_t out_stride[2];
+    int32_t n_seq;            /* 1 when cu_q is NULL */
+    int32_t n_heads;
+    int32_t n_kv;             /* n_heads / n_kv <= 64 */
+    int32_t head_dim;         /* a multiple of 8, at most 128 */
+    float scaling;
+    int32_t causal;
+    int32_t kind;             /* RVQ_BF16 or RVQ_F16: q, k, v and out */
+    int32_t reserved;         /* 0 */
+} rvq_prompt_attn_args;
+
+/* Bytes of device workspace that the call needs (0: none).  One call at a time
+ * uses a workspace; its contents need no initialisation. */
+size_t rvq_prompt_attention_workspace_size(const rvq_prompt_attn_args* a);
+int rvq_prompt_attention(const rvq_prompt_attn_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Reads and clears the sticky flag set when a bounded wait of the prompt or
+ * step attention gave up (that launch's result is then invalid).
+ * Synchronises the current device.  Returns 1, 0 or -RVQ_ERR_CUDA. */
+int rvq_take_attention_timeout(void);
+
+/* ---- 4-bit key / value cache ---------------------------------------------------
+ * One record per (sequence, kv head, row), head_dim D = 64 or 128, 5 D / 4 bytes:
+ *   [K codes D/2][V codes D/2][K parameters D/8][V parameters D/8].
+ * A row's D values are D / 32 groups of 32.  A group holds a bf16 zero z =
+ * bf16(min) and a bf16 step s = bf16((max - min) / 15) (in this order in the
+ * parameters, group by group) and 4-bit codes c = clamp(rint((x - z) / s), 0, 15)
+ * (0 when s is 0); its values are z + s c.  Every step of that is one IEEE fp32
+ * operation.  A group with a NaN or an infinity, or whose range overflows
+ * fp32, is held as NaN or infinity.  Code bytes are ordered [w in 0..3][group]
+ * [b in 0..3]: byte b of word (w, group) holds values 8 w + 2 b (low half) and
+ * 8 w + 2 b + 1 (high half) of the group, so that 16 (D = 64: 8) consecutive
+ * bytes hold 8 values of every group. */
+typedef struct rvq_cache4 {
+    void* data;               /* device [n_seq][n_kv][max_len][5 head_dim / 4] bytes, 16-byte aligned */
+    int32_t n_seq;
+    int32_t n_kv;
+    int32_t max_len;
+    int32_t head_dim;
+} rvq_cache4;
+
+/* Bytes of one record, or 0 for a head_dim that is not supported. */
+int rvq_cache4_record_bytes(int head_dim);
+
+/* Packed tokens to or from the cache: token i of sequence b (cu[b] <= i <
+ * cu[b+1]) is row start[b] + i - cu[b].  write quantises k and v into the
+ * records; read writes the held values to k and v (rounded to their type).
+ * Rows outside [0, max_len) are not written, and read as zeros; tokens behind
+ * the last sequence are left alone. */
+typedef struct rvq_cache4_rows_args {
+    rvq_cache4 cache;
+    void* k;                  /* device [tokens][n_kv][head_dim], 16-byte aligned; only read by write */
+    void* v;
+    const int32_t* cu;        /* device [n_seq + 1], ascending; NULL (n_seq 1): all tokens */
+    const int64_t* start;     /* device [n_seq]; NULL: row 0 */
+    int64_t tokens;
+    int64_t k_stride[2];      /* elements from token to token and head to head, multiples of 8 */
+    int64_t v_stride[2];
+    int32_t kind;             /* RVQ_BF16 or RVQ_F16 */
+    int32_t reserved;         /* 0 */
+} rvq_cache4_rows_args;
+
+int rvq_cache4_write(const rvq_cache4_rows_args* a, void* stream);
+int rvq_cache4_read(const rvq_cache4_rows_args* a, void* stream);
+
+/* Attention of one new token of each sequence over its cache: the token's k and
+ * v are quantised and appended at row rows[b], then every query head attends to
+ * the held values of rows 0 .. rows[b] (scores, softmax and sums in fp32).
+ * With k.ptr and v.ptr NULL nothing is appended and rows 0 .. rows[b] - 1 are
+ * attended to.  rows itself is not changed.  Optionally q and k are first
+ * normalised (q_norm, k_norm) and rotated (cos, sin, pos) as in
+ * rvq_step_attention, with its roundings to bf16.
+ * weights[b][g][j] += sum over kv head g's query heads of the softmax weight of
+ * row j; the appended row's is set.
+ * A sequence with rows[b] < 0 is skipped (nothing of it is read or written).
+ * No room (rows[b] >= max_len with a token to append, rows[b] > max_len
+ * without), no row to attend to, or pos[b] outside [0, table_len): zeros in
+ * out, the cache and the weights left alone. */
+typedef struct rvq_cache4_attn_args {
+    rvq_vec q;                /* [n_seq][n_heads][head_dim]: bf16 or fp16, or fp32 partials (rounded to bf16) */
+    rvq_vec k, v;             /* [n_seq][n_kv][head_dim], of q's kind */
+    const void* q_norm;       /* device bf16 [head_dim]; q_norm and k_norm set or both NULL */
+    const void* k_norm;
+    const void* cos;          /* device bf16 [table_len][head_dim]; cos, sin and pos set or all NULL */
+    const void* sin;
+    const int64_t* pos;       /* device [n_seq] */
+    rvq_cache4 cache;
+    const int64_t* rows;      /* device [n_seq] */
+    void* out;                /* device [n_seq][n_heads][head_dim], fp16 for fp16 q, else bf16 */
+    float* weights;           /* device [n_seq][n_kv][max_len], or NULL */
+    float* scores;            /* device [n_seq][n_heads][max_len] of workspace; needed with weights */
+    int32_t n_heads;          /* n_heads / n_kv <= 64 */
+    int32_t table_len;
+    float eps;
+    float scaling;
+} rvq_cache4_attn_args;
+
+int rvq_cache4_attention(const rvq_cache4_attn_args* a, void* stream);
+
+/* Eviction by accumulated attention weight, for every (sequence, kv head): of
+ * n = rows[b] live rows the last `recent` stay, and of the n - recent rows
+ * before them the keep - recent with the largest weight (equal weights: the
+ * lowest row; a NaN counts as the largest).  The kept records and weights move, in row order, to
+ * rows 0 .. keep - 1 of out and out_weights (the same buffers: in place), their
+ * old rows go to kept (-1 behind the last), min(n, keep) to new_rows[b].  n <= keep: every
+ * row stays.  n < 0: the sequence is left alone (kept -1, new_rows n).  n above max_len counts as
+ * max_len.  Rows behind the kept ones are left as they were. */
+typedef struct rvq_cache4_evict_args {
+    rvq_cache4 cache;
+    rvq_cache4 out;           /* equal to cache, or a buffer apart with out.max_len >= keep */
+    const float* weights;     /* device [n_seq][n_kv][cache.max_len] */
+    float* out_weights;       /* device [n_seq][n_kv][out.max_len]: equal to weights, or apart */
+    const int64_t* rows;      /* device [n_seq] */
+    int64_t* new_rows;        /* device [n_seq], apart from rows; or NULL */
+    int32_t* kept;            /* device [n_seq][n_kv][keep] */
+    int32_t keep;             /* 1 .. cache.max_len */
+    int32_t recent;           /* 0 .. keep */
+} rvq_cache4_evict_args;
+
+int rvq_cache4_evict(const rvq_cache4_evict_args* a, void* stream);
+
 /* Last CUDA error code seen by this library on the calling thread (0 = none). */
 int rvq_last_cuda_error(void);
 

@@ -1,0 +1,37 @@
+// The 4-bit cache record (layout in include/rvq_b200.h) and its arithmetic.
+#pragma once
+
+#include "rvq_common.cuh"
+
+namespace rvq {
+namespace cache4 {
+
+constexpr int kGroup = 32;                   // values that share a zero and a step
+
+__host__ __device__ constexpr int record_bytes(int hd) { return hd * 5 / 4; }
+
+// (zero, step) of a group as one word: bf16 zero in the low half, bf16 step in the high half.
+__device__ __forceinline__ float zero_of(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float step_of(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// The parameters of a group with the given extremes.  fminf and fmaxf drop a
+// NaN, so the caller passes NaN extremes for a group that holds one.
+__device__ __forceinline__ uint32_t params_of(float lo, float hi) {
+    const float step = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+    return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(lo)) |
+           (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(step)) << 16;
+}
+
+// clamp(rint((x - z) / s), 0, 15); 0 for s = 0 and for a quotient that is NaN.
+__device__ __forceinline__ uint32_t code_of(float x, float zero, float step) {
+    const float q = rintf(__fdiv_rn(__fsub_rn(x, zero), step));
+    return step > 0.f && q > 0.f ? (uint32_t)fminf(q, 15.0f) : 0u;
+}
+
+// z + s c (s c is exact: 8 by 4 bits)
+__device__ __forceinline__ float value_of(uint32_t c, float zero, float step) {
+    return __fadd_rn(zero, __fmul_rn(step, (float)c));
+}
+
+}  // namespace cache4
+}  // namespace rvq

@@ -181,10 +181,18 @@ class _Op:
             raise ValueError("every tensor must be on the same device")
         self.device = dev
 
-    def _call(self, where: str, fn, *args) -> None:
-        with torch.cuda.device(self.device):
-            rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream))
+    def _bind(self, where: str, *args) -> None:
+        """The C entry point and its arguments but the stream, resolved once."""
+        self._where, self._fn, self._args = where, getattr(_lib(), where), args
+
+    def launch(self) -> None:
+        if torch.cuda.current_device() == self.device.index:
+            rc = self._fn(*self._args, torch._C._cuda_getCurrentRawStream(self.device.index))
+        else:
+            with torch.cuda.device(self.device):
+                rc = self._fn(*self._args, torch.cuda.current_stream().cuda_stream)
         if rc:
+            where = self._where
             if rc == _native.RVQ_ERR_UNSUPPORTED:
                 raise NotImplementedError(f"{where}: {_native.status_string(rc)}")
             if rc == _native.RVQ_ERR_INVALID:
@@ -247,13 +255,7 @@ class PromptAttentionOp(_Op):
         with torch.cuda.device(self.device):
             n = _lib().rvq_prompt_attention_workspace_size(ctypes.byref(self.args))
         self._ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-        self._ws_bytes = n
-
-    def launch(self) -> None:
-        if self.args.tokens == 0:
-            return
-        self._call("rvq_prompt_attention", _lib().rvq_prompt_attention, ctypes.byref(self.args), _ptr(self._ws),
-                   self._ws_bytes)
+        self._bind("rvq_prompt_attention", ctypes.byref(self.args), _ptr(self._ws), n)
 
 
 class Cache4:
@@ -304,11 +306,7 @@ class _Cache4RowsOp(_Op):
         self._on(k, v, cache.data, cu, start)
         self.args = RvqCache4RowsArgs(cache.struct(), _ptr(k), _ptr(v), _ptr(cu), _ptr(start), k.shape[0], _strides(k),
                                       _strides(v), _native.kind_of(k), 0)
-
-    def launch(self) -> None:
-        if self.args.tokens == 0:
-            return
-        self._call(self.name, getattr(_lib(), self.name), ctypes.byref(self.args))
+        self._bind(self.name, ctypes.byref(self.args))
 
 
 class Cache4WriteOp(_Cache4RowsOp):
@@ -404,9 +402,7 @@ class Cache4AttentionOp(_Op):
         self.args = RvqCache4AttnArgs(qv, kv_, vv, _ptr(q_norm), _ptr(k_norm), _ptr(cos), _ptr(sin), _ptr(pos),
                                       cache.struct(), _ptr(rows), _ptr(out), _ptr(weights), _ptr(self._scores), n_heads,
                                       table, float(eps), float(scaling))
-
-    def launch(self) -> None:
-        self._call("rvq_cache4_attention", _lib().rvq_cache4_attention, ctypes.byref(self.args))
+        self._bind("rvq_cache4_attention", ctypes.byref(self.args))
 
 
 class Cache4EvictOp(_Op):
@@ -443,6 +439,4 @@ class Cache4EvictOp(_Op):
         self.kept = torch.empty(n, nkv, keep, dtype=torch.int32, device=self.device) if kept is None else kept
         self.args = RvqCache4EvictArgs(cache.struct(), out.struct(), _ptr(weights), _ptr(out_weights), _ptr(rows),
                                        _ptr(new_rows), _ptr(self.kept), int(keep), int(recent))
-
-    def launch(self) -> None:
-        self._call("rvq_cache4_evict", _lib().rvq_cache4_evict, ctypes.byref(self.args))
+        self._bind("rvq_cache4_evict", ctypes.byref(self.args))

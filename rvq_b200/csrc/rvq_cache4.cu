@@ -245,11 +245,6 @@ int check_rows(const rvq_cache4_rows_args* a) {
     return RVQ_OK;
 }
 
-int status(cudaError_t e) {
-    if (e != cudaSuccess) last_cuda_error_slot() = (int)e;
-    return e == cudaSuccess ? RVQ_OK : RVQ_ERR_CUDA;
-}
-
 template <bool kWrite>
 int run_rows(const rvq_cache4_rows_args* a, void* stream) {
     const int rc = check_rows(a);

@@ -33,5 +33,10 @@ __device__ __forceinline__ float value_of(uint32_t c, float zero, float step) {
     return __fadd_rn(zero, __fmul_rn(step, (float)c));
 }
 
+inline int status(cudaError_t e) {
+    if (e != cudaSuccess) last_cuda_error_slot() = (int)e;
+    return e == cudaSuccess ? RVQ_OK : RVQ_ERR_CUDA;
+}
+
 }  // namespace cache4
 }  // namespace rvq

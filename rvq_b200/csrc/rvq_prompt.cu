@@ -5,6 +5,9 @@
 #include "rvq_common.cuh"
 
 namespace rvq {
+
+int take_step_timeout();                     // the step attention's flag (rvq_cache4_attn.cu)
+
 namespace prompt {
 
 __device__ int g_attention_timeout;          // sticky: a bounded wait gave up
@@ -112,5 +115,6 @@ extern "C" int rvq_take_attention_timeout(void) {
         last_cuda_error_slot() = (int)e;
         return -RVQ_ERR_CUDA;
     }
-    return v;
+    const int step = take_step_timeout();
+    return step < 0 ? step : v | step;
 }

@@ -1,8 +1,13 @@
 // Attention of whole prompts (rvq_prompt_attention, include/rvq_b200.h).
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <string.h>
 
+#include <mutex>
+
 #include "rvq_common.cuh"
+#include "rvq_sm100.cuh"
 
 namespace rvq {
 
@@ -10,61 +15,471 @@ int take_step_timeout();                     // the step attention's flag (rvq_c
 
 namespace prompt {
 
+using namespace sm100;
+
 __device__ int g_attention_timeout;          // sticky: a bounded wait gave up
 
-// One warp per (token, query head): the keys one after the other, running
-// maximum and sum of the softmax.  Lane l holds elements l, l + 32, ...
-__global__ void __launch_bounds__(128) prompt_simple_kernel(rvq_prompt_attn_args a) {
-    pdl_launch_dependents();
-    pdl_wait();
+// ---------------------------------------------------------------------------
+// A CTA takes 2 tiles of 128 operand rows of one kv head and walks the keys in
+// tiles of 128.  A row is (token, query head of the kv head): a tile holds
+// 128 / rep tokens with all their rep heads, so grouped heads share every K and
+// V tile and short sequences fill the rows.  Roles by warp: 0-3 and 4-7 the
+// softmax of the two tiles (a thread per row), 8 the TMA loads, 9 the MMAs.
+//
+//   S = Q K^T       tcgen05.mma, both operands in shared memory, S in TMEM
+//   P = 2^(c S - m) a row per thread, fp32; rounded to the operand type and
+//                   written over S in TMEM
+//   O += P V        tcgen05.mma, P from TMEM, V as it lies in shared memory
+//
+// While one tile's softmax runs, the tensor cores work for the other one.  The
+// maximum that is subtracted only follows the true one when that has grown by
+// 2^8: O is then rescaled by the row's own thread, which is rare after the first
+// tiles; p stays below 2^8, exact in fp32 sums and with unchanged relative rounding.
+// Keys of other tokens that a tile brings along (behind the sequence, later
+// than the query) get p = 0; values behind the sequence are zeroed in shared
+// memory, and a row that came out non-finite is looked at again (repair), so
+// that no hidden NaN or infinity reaches it through 0 * NaN.
+// ---------------------------------------------------------------------------
+constexpr int kRows = 128;                   // operand rows of a tile (MMA M)
+constexpr int kKeys = 128;                   // keys of a tile
+constexpr int kThreads = 320;
+constexpr int kHalf = kRows * 128;           // bytes of 64 columns of a tile
+constexpr long long kWaitPolls = 1ll << 22;
+constexpr float kGrow = 8.f;                 // the maximum may be passed by 2^kGrow
+
+struct Params {
+    CUtensorMap q, k, v;
+    rvq_prompt_attn_args a;
+    int32_t rep;
+    int32_t tile_tokens;                     // 128 / rep
+    int32_t pairs;                           // upper bound of the pairs of tiles of all sequences
+};
+
+template <int HD>
+struct Smem {
+    static constexpr int kTileBytes = HD / 64 * kHalf;
+    uint8_t q[2][kTileBytes];
+    uint8_t k[2][kTileBytes];
+    uint8_t v[2][kTileBytes];
+    uint64_t q_full, drain, k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean, s_full[2], p_full[2], o_full[2];
+    uint32_t tmem;
+    int32_t seq, pair;                       // this CTA's sequence (-1: none) and pair of tiles in it
+    int32_t dead;                            // a bounded wait gave up
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];\n" ::"r"(dst),
+        "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+
+// N-major operand (rows of 64 N-elements, one row per k) with 128-byte swizzle:
+// 8-row atoms of 1024 bytes along k (stride offset), `next` bytes from one block
+// of 64 columns to the next (leading offset).
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t next) {
+    return (sw128_desc(saddr) & ~(0x3fffull << 16)) | (uint64_t)(next >> 4) << 16;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// Bounded wait of a whole warp; once one wait of the CTA has given up, the others end at once.
+template <int HD>
+__device__ __forceinline__ bool wait(Smem<HD>& S, uint64_t& bar, uint32_t parity) {
+    const uint32_t b = smem_addr(&bar);
+    bool done = false;
+    for (long long i = 0; i < kWaitPolls && !done; ++i) {
+        done = mbar_try_wait(b, parity);
+        if (!done && (i & 63) == 63 && *(volatile int32_t*)&S.dead) break;
+    }
+    if (__all_sync(0xffffffffu, done)) return true;
+    atomicExch(&g_attention_timeout, 1);
+    *(volatile int32_t*)&S.dead = 1;
+    return false;
+}
+
+// The sequence of pair number `want` (pairs counted over the sequences in order) by one warp: -1 if there is none.
+__device__ __forceinline__ void find_pair(const rvq_prompt_attn_args& a, int per_pair, int want, int32_t* seq, int32_t* pair) {
     const int lane = threadIdx.x & 31;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (unit >= a.tokens * a.n_heads) return;
-    const int64_t tok = unit / a.n_heads;
-    const int h = (int)(unit - tok * a.n_heads), g = h / (a.n_heads / a.n_kv);
-    int64_t q0 = 0, q1 = a.tokens, k0 = 0, k1 = a.keys;
-    if (a.cu_q != nullptr) {
-        int lo = 0, hi = a.n_seq;                 // the last sequence that starts at or before tok
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (a.cu_q[mid] <= tok) lo = mid;
-            else hi = mid;
+    int64_t before = 0;
+    *seq = -1;
+    for (int base = 0; base < a.n_seq; base += 32) {
+        const int b = base + lane;
+        int64_t q0 = 0, q1 = 0;
+        if (b < a.n_seq) {
+            q0 = a.cu_q != nullptr ? max(0, __ldg(a.cu_q + b)) : 0;
+            q1 = a.cu_q != nullptr ? min(a.tokens, (int64_t)__ldg(a.cu_q + b + 1)) : a.tokens;
         }
-        q0 = max(0, a.cu_q[lo]), q1 = min(a.tokens, (int64_t)a.cu_q[lo + 1]);
-        const int32_t* cu_k = a.cu_k != nullptr ? a.cu_k : a.cu_q;
-        k0 = max((int64_t)0, (int64_t)cu_k[lo]), k1 = min(a.keys, (int64_t)cu_k[lo + 1]);
-        if (tok < q0 || tok >= q1) return;
+        const int64_t mine = q1 > q0 ? (q1 - q0 + per_pair - 1) / per_pair : 0;
+        int64_t upto = mine;                                 // inclusive prefix sum over the lanes
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+        if (want < before + total) {
+            const uint32_t has = __ballot_sync(0xffffffffu, want < before + upto);
+            const int l = __ffs(has) - 1;
+            *seq = base + l;
+            *pair = (int32_t)(want - before - __shfl_sync(0xffffffffu, upto - mine, l));
+            return;
+        }
+        before += total;
     }
-    const int64_t lk = max((int64_t)0, k1 - k0);
-    const int64_t n = a.causal ? min(lk, tok - q0 + 1 + lk - (q1 - q0)) : lk;
-    const int hd = a.head_dim;
-    float qv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+}
+
+// Output row of a query whose hidden values (keys [n, hidden_end) of the last tiles) may have leaked in, by a whole warp:
+// where one of them is not finite and no seen value in the last tile is NaN, the columns concerned are summed again over
+// the n keys that the query sees, one by one.
+__device__ __noinline__ void repair(const rvq_prompt_attn_args& a, int64_t tok, int h, int64_t k0, int64_t n,
+                                    int64_t hidden_end, float c, float m, float inv) {
+    const int lane = threadIdx.x & 31, g = h / (a.n_heads / a.n_kv), hd = a.head_dim;
+    const int64_t vr = g * a.v_stride[1], kr = g * a.k_stride[1];
+    bool leak[4];
+    bool any = false;
     for (int j = 0; j < 4; ++j) {
         const int d = lane + 32 * j;
-        qv[j] = d < hd ? load_as_f32(a.q, tok * a.q_stride[0] + h * a.q_stride[1] + d, a.kind) : 0.f;
+        leak[j] = false;
+        if (d >= hd) continue;
+        for (int64_t i = n; i < hidden_end; ++i) {
+            const float v = load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + d, a.kind);
+            leak[j] |= !(fabsf(v) <= 3.4e38f);
+        }
+        for (int64_t i = max((int64_t)0, hidden_end - kKeys); leak[j] && i < n; ++i) {
+            const float v = load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + d, a.kind);
+            leak[j] = v == v;
+        }
+        any |= leak[j];
     }
-    float m = -INFINITY, sum = 0.f;
+    if (!__any_sync(0xffffffffu, any)) return;
+    float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 4; ++j)
+        q[j] = lane + 32 * j < hd ? load_as_f32(a.q, tok * a.q_stride[0] + h * a.q_stride[1] + lane + 32 * j, a.kind) : 0.f;
     for (int64_t i = 0; i < n; ++i) {
-        const int64_t kr = (k0 + i) * a.k_stride[0] + g * a.k_stride[1];
-        const int64_t vr = (k0 + i) * a.v_stride[0] + g * a.v_stride[1];
-        float s = 0.f;
+        float x = 0.f;
         for (int j = 0; j < 4; ++j)
-            if (lane + 32 * j < hd) s = fmaf(qv[j], load_as_f32(a.k, kr + lane + 32 * j, a.kind), s);
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= a.scaling;
-        const float mn = fmaxf(m, s);
-        const float old = mn == -INFINITY ? 1.f : expf(m - mn), p = mn == -INFINITY ? expf(s) : expf(s - mn);
-        sum = sum * old + p;
+            if (lane + 32 * j < hd) x = fmaf(q[j], load_as_f32(a.k, (k0 + i) * a.k_stride[0] + kr + lane + 32 * j, a.kind), x);
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        const float p = exp2_approx(fmaf(x, c, -m));
         for (int j = 0; j < 4; ++j)
-            if (lane + 32 * j < hd) acc[j] = acc[j] * old + p * load_as_f32(a.v, vr + lane + 32 * j, a.kind);
-        m = mn;
+            if (leak[j]) acc[j] += p * load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + lane + 32 * j, a.kind);
     }
-    for (int j = 0; j < 4; ++j) {
-        const int d = lane + 32 * j;
-        if (d < hd)
-            store_from_f32(a.out, tok * a.out_stride[0] + h * a.out_stride[1] + d, a.kind, sum != 0.f ? acc[j] / sum : 0.f);
+    for (int j = 0; j < 4; ++j)
+        if (leak[j])
+            store_from_f32(a.out, tok * a.out_stride[0] + h * a.out_stride[1] + lane + 32 * j, a.kind, acc[j] * inv);
+}
+
+template <int HD, bool kHalfType>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    Smem<HD>& S = *reinterpret_cast<Smem<HD>*>(smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023));
+    const rvq_prompt_attn_args& a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kv = blockIdx.x % a.n_kv;
+    const int T = p.tile_tokens;
+    pdl_launch_dependents();
+    if (tid == 0) {
+        mbar_init(smem_addr(&S.q_full), 1);
+        mbar_init(smem_addr(&S.v_clean), 1);
+        mbar_init(smem_addr(&S.drain), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_addr(&S.k_full[i]), 1);
+            mbar_init(smem_addr(&S.k_empty[i]), 1);
+            mbar_init(smem_addr(&S.v_full[i]), 1);
+            mbar_init(smem_addr(&S.v_empty[i]), 1);
+            mbar_init(smem_addr(&S.s_full[i]), 1);
+            mbar_init(smem_addr(&S.p_full[i]), 4);
+            mbar_init(smem_addr(&S.o_full[i]), 1);
+        }
+        S.dead = 0;
+        mbar_init_fence();
     }
-    if (a.lse != nullptr && lane == 0) a.lse[(int64_t)h * a.tokens + tok] = m + logf(sum);
+    if (warp == 9) tmem_alloc(smem_addr(&S.tmem), 512);
+    pdl_wait();
+    if (warp == 8) {
+        // the last pairs of a causal sequence see the most keys: they start first
+        int32_t seq, pair = 0;
+        find_pair(a, 2 * T, p.pairs - 1 - (int)(blockIdx.x / a.n_kv), &seq, &pair);
+        if (lane == 0) S.seq = seq, S.pair = pair;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = S.tmem;
+    const int seq = S.seq;
+    if (seq >= 0) {
+        int64_t q0 = 0, q1 = a.tokens, k0 = 0, k1 = a.keys;
+        if (a.cu_q != nullptr) {
+            const int32_t* cu_k = a.cu_k != nullptr ? a.cu_k : a.cu_q;
+            q0 = max(0, __ldg(a.cu_q + seq)), q1 = min(a.tokens, (int64_t)__ldg(a.cu_q + seq + 1));
+            k0 = max(0, __ldg(cu_k + seq)), k1 = min(a.keys, (int64_t)__ldg(cu_k + seq + 1));
+        }
+        const int lq = (int)(q1 - q0), lk = (int)max((int64_t)0, k1 - k0);
+        const int tok0 = S.pair * 2 * T;                     // first token of tile 0 in its sequence
+        // keys that tile i's last token sees, in tiles
+        int n[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int last = min(lq, tok0 + (i + 1) * T) - 1;
+            const int see = last < tok0 + i * T ? 0 : a.causal ? min(lk, max(0, last + 1 + lk - lq)) : lk;
+            n[i] = (see + kKeys - 1) / kKeys;
+        }
+        const int total = max(n[0], n[1]);
+        const bool clean = lk % kKeys != 0 && total * kKeys > lk && k0 + lk < a.keys;   // values of others in the last tile
+
+        if (warp == 8) {
+            if (lane == 0 && total > 0) {
+                mbar_expect_tx(smem_addr(&S.q_full), (n[1] > 0 ? 2 : 1) * HD / 64 * (uint32_t)(T * p.rep * 128));
+                for (int i = 0; i < (n[1] > 0 ? 2 : 1); ++i)
+                    for (int h = 0; h < HD / 64; ++h)
+                        tma_load_3d(smem_addr(S.q[i] + h * kHalf), &p.q, 64 * h, kv * p.rep, (int)q0 + tok0 + i * T,
+                                    smem_addr(&S.q_full));
+            }
+            int loaded_k = 0, loaded_v = 0;
+            for (int j = 0; j < total; ++j) {
+                const int st = j & 1, row = (int)k0 + j * kKeys;
+                if (j >= 2 && !wait(S, S.k_empty[st], (j / 2 - 1) & 1)) break;
+                if (lane == 0) {
+                    mbar_expect_tx(smem_addr(&S.k_full[st]), Smem<HD>::kTileBytes);
+                    for (int h = 0; h < HD / 64; ++h)
+                        tma_load_3d(smem_addr(S.k[st] + h * kHalf), &p.k, 64 * h, kv, row, smem_addr(&S.k_full[st]));
+                }
+                loaded_k = j + 1;
+                if (j >= 2 && !wait(S, S.v_empty[st], (j / 2 - 1) & 1)) break;
+                if (lane == 0) {
+                    mbar_expect_tx(smem_addr(&S.v_full[st]), Smem<HD>::kTileBytes);
+                    for (int h = 0; h < HD / 64; ++h)
+                        tma_load_3d(smem_addr(S.v[st] + h * kHalf), &p.v, 64 * h, kv, row, smem_addr(&S.v_full[st]));
+                }
+                loaded_v = j + 1;
+            }
+            if (clean && loaded_v == total && wait(S, S.v_full[(total - 1) & 1], ((total - 1) / 2) & 1)) {
+                uint8_t* v = S.v[(total - 1) & 1];
+                const int r0 = lk - (total - 1) * kKeys;     // rows r0 .. 127 belong to others (a swizzled row stays a row)
+                for (int h = 0; h < HD / 64; ++h)
+                    for (int i = r0 * 8 + lane; i < kRows * 8; i += 32)
+                        reinterpret_cast<uint4*>(v + h * kHalf)[i] = make_uint4(0, 0, 0, 0);
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&S.v_clean));
+            }
+            if (*(volatile int32_t*)&S.dead) {               // copies in flight end before this CTA's shared memory is given up
+                for (int i = 0; i < 2; ++i) {
+                    if (loaded_k > i) mbar_wait(smem_addr(&S.k_full[(loaded_k - 1 - i) & 1]), ((loaded_k - 1 - i) / 2) & 1,
+                                                kWaitPolls, &g_attention_timeout);
+                    if (loaded_v > i) mbar_wait(smem_addr(&S.v_full[(loaded_v - 1 - i) & 1]), ((loaded_v - 1 - i) / 2) & 1,
+                                                kWaitPolls, &g_attention_timeout);
+                }
+                if (total > 0) mbar_wait(smem_addr(&S.q_full), 0, kWaitPolls, &g_attention_timeout);
+            }
+        } else if (warp == 9) {
+            constexpr uint32_t kTypes = kHalfType ? 0u : (1u << 7) | (1u << 10);
+            constexpr uint32_t kS = (1u << 4) | kTypes | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+            constexpr uint32_t kO = (1u << 4) | kTypes | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+            auto scores = [&](int i, int j) {                // S_i = Q_i K_j^T
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k)
+                        mma_bf16(tmem + i * kKeys, sw128_desc(smem_addr(S.q[i]) + (k / 4) * kHalf + (k % 4) * 32),
+                                 sw128_desc(smem_addr(S.k[j & 1]) + (k / 4) * kHalf + (k % 4) * 32), kS, k > 0);
+                    mma_commit(smem_addr(&S.s_full[i]));
+                }
+                __syncwarp();
+            };
+            bool ok = total == 0 || wait(S, S.q_full, 0);
+            if (ok && total > 0) ok = wait(S, S.k_full[0], 0);
+            if (ok && total > 0) {
+                for (int i = 0; i < 2; ++i)
+                    if (n[i] > 0) scores(i, 0);
+                if (lane == 0) mma_commit(smem_addr(&S.k_empty[0]));
+                __syncwarp();
+            }
+            for (int j = 0; ok && j < total; ++j) {
+                ok = wait(S, S.v_full[j & 1], (j / 2) & 1);
+                if (ok && clean && j == total - 1) ok = wait(S, S.v_clean, 0);
+                if (ok && j + 1 < total) ok = wait(S, S.k_full[(j + 1) & 1], ((j + 1) / 2) & 1);
+                for (int i = 0; ok && i < 2; ++i) {
+                    if (j >= n[i]) continue;
+                    ok = wait(S, S.p_full[i], j & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k)
+                            mma_bf16_ts(tmem + 2 * kKeys + i * HD, tmem + i * kKeys + 8 * k,
+                                        sw128_desc_mn(smem_addr(S.v[j & 1]) + k * 2048, kHalf), kO, j > 0 || k > 0);
+                        if (j + 1 == n[i]) mma_commit(smem_addr(&S.o_full[i]));
+                    }
+                    __syncwarp();
+                    if (j + 1 < n[i]) scores(i, j + 1);
+                }
+                if (ok && lane == 0) {
+                    mma_commit(smem_addr(&S.v_empty[j & 1]));
+                    if (j + 1 < total) mma_commit(smem_addr(&S.k_empty[(j + 1) & 1]));
+                }
+                __syncwarp();
+            }
+            if (!ok) {                                       // products in flight end before TMEM is given up
+                if (lane == 0) mma_commit(smem_addr(&S.drain));
+                __syncwarp();
+                mbar_wait(smem_addr(&S.drain), 0, kWaitPolls, &g_attention_timeout);
+            }
+        } else {
+            const int i = warp >> 2, row = tid & 127;
+            const int in = row / p.rep, h = kv * p.rep + row % p.rep;
+            const int tok = tok0 + i * T + in;               // in the sequence
+            const bool valid = in < T && tok < lq;
+            const int limit = !valid ? 0 : a.causal ? min(lk, max(0, tok + 1 + lk - lq)) : lk;
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 2 * kKeys + i * HD;
+            const bool negative = a.scaling < 0.f;
+            const float c = fabsf(a.scaling) * 1.4426950408889634f;
+            float m = -INFINITY, sum = 0.f;                  // m: of the scores times c
+            bool ok = true;
+            for (int j = 0; j < n[i]; ++j) {
+                ok = wait(S, S.s_full[i], j & 1);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t r[4][32];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) tmem_ld32(ts + 32 * x, r[x]);
+                tmem_ld_wait();
+                float (&s)[4][32] = reinterpret_cast<float (&)[4][32]>(r);
+                if (negative) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[x][e] = -s[x][e];
+                }
+                const int seen = limit - j * kKeys;          // columns of this tile that the row sees
+                const bool masked = __any_sync(0xffffffffu, seen < kKeys);
+                if (masked) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (32 * x + e >= seen) s[x][e] = -INFINITY;
+                }
+                float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 32; e += 2)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) t[x] = fmaxf(fmaxf(t[x], s[x][e]), s[x][e + 1]);
+                const float raw = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                const float top = raw == -INFINITY ? -INFINITY : raw * c;
+                const bool grow = j == 0 ? top > m : top > m + kGrow;
+                if (j == 0) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, grow)) {
+                    // S is full: the products before it, which summed into O, are complete
+                    const float f = grow ? exp2_approx(m - top) : 1.f;
+                    if (grow) m = top;
+                    sum *= f;
+#pragma unroll 1
+                    for (int x = 0; x < HD / 32; ++x) {
+                        uint32_t o[32];
+                        tmem_ld32(to + 32 * x, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(to + 32 * x, o);
+                    }
+                    tmem_st_wait();
+                }
+                const float sub = m == -INFINITY ? 0.f : m;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < 4; x += 2) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float p0 = exp2_approx(fmaf(s[x + y][e], c, -sub));
+                            float p1 = exp2_approx(fmaf(s[x + y][e + 1], c, -sub));
+                            if (masked) {                    // c may be 0
+                                if (32 * (x + y) + e >= seen) p0 = 0.f;
+                                if (32 * (x + y) + e + 1 >= seen) p1 = 0.f;
+                            }
+                            part[2 * y] += p0;
+                            part[2 * y + 1] += p1;
+                            w[16 * y + e / 2] = pack2(p0, p1, kHalfType ? RVQ_F16 : RVQ_BF16);
+                        }
+                    tmem_st32(ts + 16 * x, w);
+                }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&S.p_full[i]));
+            }
+            if (ok && n[i] > 0) ok = wait(S, S.o_full[i], 0);
+            tc_fence_after();
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int64_t at = (q0 + tok) * a.out_stride[0] + h * a.out_stride[1];
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at;
+            bool bad = false;
+#pragma unroll 1
+            for (int x = 0; x < HD / 32; ++x) {
+                uint32_t o[32];
+                if (ok && n[i] > 0) {
+                    tmem_ld32(to + 32 * x, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                }
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float v0 = __uint_as_float(o[e]), v1 = __uint_as_float(o[e + 1]);
+                    bad |= !(fabsf(v0) + fabsf(v1) <= 3.4e38f);
+                    v0 = limit == 0 || inv == 0.f ? 0.f : v0 * inv;
+                    v1 = limit == 0 || inv == 0.f ? 0.f : v1 * inv;
+                    w[e / 2] = pack2(v0, v1, kHalfType ? RVQ_F16 : RVQ_BF16);
+                }
+                if (valid) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (32 * x + 8 * e < a.head_dim)
+                            *reinterpret_cast<uint4*>(out + 32 * x + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                }
+            }
+            if (valid && a.lse != nullptr)
+                a.lse[(int64_t)h * a.tokens + q0 + tok] = limit == 0 || sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+            // values between this row's last key and the end of its last tile may have leaked in
+            const int hidden_end = min(lk, n[i] * kKeys);
+            uint32_t again = __ballot_sync(0xffffffffu, ok && valid && bad && limit > 0 && limit < hidden_end && fabsf(sum) <= 3.4e38f);
+            while (again) {
+                const int l = __ffs(again) - 1;
+                again &= again - 1;
+                __syncwarp();
+                repair(a, q0 + __shfl_sync(0xffffffffu, tok, l), __shfl_sync(0xffffffffu, h, l), k0, __shfl_sync(0xffffffffu, limit, l),
+                       hidden_end, negative ? -c : c, __shfl_sync(0xffffffffu, m, l), __shfl_sync(0xffffffffu, inv, l));
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
 int check(const rvq_prompt_attn_args* a) {
@@ -85,6 +500,47 @@ int check(const rvq_prompt_attn_args* a) {
     return RVQ_OK;
 }
 
+std::mutex g_mu;
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+
+int prepare() {
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (g_encode != nullptr) return RVQ_OK;
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+        last_cuda_error_slot() = (int)e;
+        return RVQ_ERR_UNAVAILABLE;
+    }
+    g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    return RVQ_OK;
+}
+
+// [rows][heads][head_dim] by boxes of 64 columns, `heads` heads and `rows` rows.
+bool encode(CUtensorMap* map, const void* ptr, const rvq_prompt_attn_args& a, int64_t n_rows, int64_t n_heads,
+            const int64_t* stride, int box_heads, int box_rows) {
+    const cuuint64_t dims[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)n_heads, (cuuint64_t)n_rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)stride[1] * 2, (cuuint64_t)stride[0] * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return g_encode(map, a.kind == RVQ_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                    const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD, bool kHalfType>
+int run(const Params& p, cudaStream_t s) {
+    auto* kernel = prompt_kernel<HD, kHalfType>;
+    const int smem = (int)sizeof(Smem<HD>) + 1024;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+        e = launch_pdl(kernel, dim3((unsigned)p.pairs * (unsigned)p.a.n_kv), dim3(kThreads), (size_t)smem, s, p);
+    if (e != cudaSuccess) last_cuda_error_slot() = (int)e;
+    return e == cudaSuccess ? RVQ_OK : RVQ_ERR_CUDA;
+}
+
 }  // namespace prompt
 }  // namespace rvq
 
@@ -96,13 +552,29 @@ extern "C" size_t rvq_prompt_attention_workspace_size(const rvq_prompt_attn_args
 }
 
 extern "C" int rvq_prompt_attention(const rvq_prompt_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-    const int rc = check(a);
+    int rc = check(a);
     if (rc != RVQ_OK || a->tokens == 0) return rc;
-    const int64_t blocks = (a->tokens * a->n_heads + 3) / 4;
-    if (blocks >= (1ll << 31)) return RVQ_ERR_TOO_LARGE;
-    const cudaError_t e = launch_pdl(prompt_simple_kernel, dim3((unsigned)blocks), dim3(128), 0, (cudaStream_t)stream, *a);
-    if (e != cudaSuccess) last_cuda_error_slot() = (int)e;
-    return e == cudaSuccess ? RVQ_OK : RVQ_ERR_CUDA;
+    rc = prepare();
+    if (rc != RVQ_OK) return rc;
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.a = *a;
+    p.rep = a->n_heads / a->n_kv;
+    p.tile_tokens = kRows / p.rep;
+    // each sequence has at most one pair of tiles that is not full
+    const int64_t pairs = a->n_seq == 1 ? (a->tokens + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens)
+                                        : a->tokens / (2 * p.tile_tokens) + a->n_seq;
+    if (pairs * a->n_kv >= (1ll << 31)) return RVQ_ERR_TOO_LARGE;
+    p.pairs = (int32_t)pairs;
+    // without keys nothing is loaded: any valid map will do
+    const bool none = a->keys == 0;
+    if (!encode(&p.q, a->q, *a, a->tokens, a->n_heads, a->q_stride, p.rep, p.tile_tokens) ||
+        !encode(&p.k, none ? a->q : a->k, *a, none ? 1 : a->keys, none ? 1 : a->n_kv, a->k_stride, 1, kKeys) ||
+        !encode(&p.v, none ? a->q : a->v, *a, none ? 1 : a->keys, none ? 1 : a->n_kv, a->v_stride, 1, kKeys))
+        return RVQ_ERR_INVALID;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (a->kind == RVQ_F16) return a->head_dim > 64 ? run<128, true>(p, s) : run<64, true>(p, s);
+    return a->head_dim > 64 ? run<128, false>(p, s) : run<64, false>(p, s);
 }
 
 extern "C" int rvq_take_attention_timeout(void) {

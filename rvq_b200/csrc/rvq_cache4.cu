@@ -21,8 +21,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return d;
 }
 
-// Record of packed token `tok` and its kv head, or NULL where the token is in
-// no sequence; *row_ok: the row lies in the cache.
+// Record of packed token `tok` and kv head g, or NULL where the token is in no sequence; *row_ok: the row lies in the cache.
 __device__ __forceinline__ uint8_t* record_of(const rvq_cache4_rows_args& a, int64_t tok, int g, int rec, bool* row_ok) {
     int b = 0;
     int64_t i = tok;
@@ -42,71 +41,88 @@ __device__ __forceinline__ uint8_t* record_of(const rvq_cache4_rows_args& a, int
            (((int64_t)b * a.cache.n_kv + g) * a.cache.max_len + (*row_ok ? row : 0)) * rec;
 }
 
-// HD / 4 adjacent threads per (token, kv head): half of them K, half V; four
-// adjacent ones hold a group, 8 values (one 16-byte load or store) each, which
-// are one code word.  A warp's code words fill whole 32-byte sectors.
+// HD / 4 adjacent threads per token of the block's kv head: half of them K, half V; four adjacent ones hold a group, 8
+// values (one 16-byte load or store) each, which are one code word.  A block's tokens are neighbouring records, so code
+// words and parameters fill whole sectors; kTokens tokens a thread keep enough bytes in flight.
+constexpr int kTokens = 2;
+
 template <int HD, bool kWrite>
 __global__ void __launch_bounds__(kRowsThreads) cache4_rows_kernel(rvq_cache4_rows_args a) {
-    constexpr int T = HD / 4, G = HD / kGroup;
+    constexpr int T = HD / 4, G = HD / kGroup, B = kRowsThreads / T;
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t idx = (int64_t)blockIdx.x * kRowsThreads + threadIdx.x;
-    const int64_t unit = idx / T;
-    const bool live = unit < a.tokens * a.cache.n_kv;
-    const int in = (int)(idx % T), which = in / (T / 2), grp = in % (T / 2) / 4, w = in & 3;
-    const int64_t tok = live ? unit / a.cache.n_kv : 0;
-    const int g = live ? (int)(unit - tok * a.cache.n_kv) : 0;
-    bool row_ok = false;
-    uint8_t* rec = live ? record_of(a, tok, g, record_bytes(HD), &row_ok) : nullptr;
+    const int in = threadIdx.x % T, which = in / (T / 2), grp = in % (T / 2) / 4, w = in & 3;
+    const int g = blockIdx.y;
     const int64_t* st = which ? a.v_stride : a.k_stride;
-    uint4* x = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(which ? a.v : a.k) + tok * st[0] + g * st[1] +
-                                        grp * kGroup + 8 * w);
-    uint32_t* codes = reinterpret_cast<uint32_t*>(rec + which * (HD / 2)) + w * G + grp;
-    uint32_t* params = reinterpret_cast<uint32_t*>(rec + HD + which * (HD / 8)) + grp;
-    if constexpr (kWrite) {
-        const uint4 raw = rec != nullptr ? *x : make_uint4(0, 0, 0, 0);
-        const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
-        float v[8];
+    uint16_t* base = reinterpret_cast<uint16_t*>(which ? a.v : a.k) + g * st[1] + grp * kGroup + 8 * w;
+    uint8_t* rec[kTokens];
+    bool row_ok[kTokens];
+    uint4* x[kTokens];
+    uint4 raw[kTokens];
+    uint32_t word[kTokens], par[kTokens];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint16_t u = (uint16_t)(r[i / 2] >> (16 * (i & 1)));
-            v[i] = a.kind == RVQ_F16 ? __half2float(__ushort_as_half(u)) : __bfloat162float(__ushort_as_bfloat16(u));
+    for (int u = 0; u < kTokens; ++u) {
+        const int64_t tok = ((int64_t)blockIdx.x * kTokens + u) * B + threadIdx.x / T;
+        row_ok[u] = false;
+        rec[u] = tok < a.tokens ? record_of(a, tok, g, record_bytes(HD), &row_ok[u]) : nullptr;
+        x[u] = reinterpret_cast<uint4*>(base + tok * st[0]);
+        raw[u] = make_uint4(0, 0, 0, 0);
+        word[u] = par[u] = 0;
+        if (rec[u] == nullptr) continue;
+        if constexpr (kWrite) {
+            raw[u] = *x[u];
+        } else if (row_ok[u]) {
+            word[u] = *(reinterpret_cast<uint32_t*>(rec[u] + which * (HD / 2)) + w * G + grp);
+            par[u] = *(reinterpret_cast<uint32_t*>(rec[u] + HD + which * (HD / 8)) + grp);
         }
-        float lo = v[0], hi = v[0];
+    }
 #pragma unroll
-        for (int i = 1; i < 8; ++i) lo = min_nan(lo, v[i]), hi = max_nan(hi, v[i]);
+    for (int u = 0; u < kTokens; ++u) {
+        if constexpr (kWrite) {
+            const uint32_t r[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            float v[8];
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            for (int i = 0; i < 8; ++i) {
+                const uint16_t h = (uint16_t)(r[i / 2] >> (16 * (i & 1)));
+                v[i] = a.kind == RVQ_F16 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
+            }
+            float lo = v[0], hi = v[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) lo = min_nan(lo, v[i]), hi = max_nan(hi, v[i]);
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            const uint32_t p = params_of(lo, hi);
+            const float zero = zero_of(p), step = step_of(p), inv = 1.0f / step;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) word[u] |= code_of(v[i], zero, step, inv) << (4 * i);
+            if (rec[u] != nullptr && row_ok[u]) {
+                *(reinterpret_cast<uint32_t*>(rec[u] + which * (HD / 2)) + w * G + grp) = word[u];
+                if (w == 0) *(reinterpret_cast<uint32_t*>(rec[u] + HD + which * (HD / 8)) + grp) = p;
+            }
+        } else if (rec[u] != nullptr) {
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[i] = pack2(value_of(word[u] >> (8 * i) & 15, zero_of(par[u]), step_of(par[u])),
+                             value_of(word[u] >> (8 * i + 4) & 15, zero_of(par[u]), step_of(par[u])), a.kind);
+            *x[u] = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        const uint32_t p = params_of(lo, hi);
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) word |= code_of(v[i], zero_of(p), step_of(p)) << (4 * i);
-        if (rec != nullptr && row_ok) {
-            *codes = word;
-            if (w == 0) *params = p;
-        }
-    } else if (rec != nullptr) {
-        const uint32_t word = row_ok ? *codes : 0, p = row_ok ? *params : 0;
-        uint32_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            o[i] = pack2(value_of(word >> (8 * i) & 15, zero_of(p), step_of(p)),
-                         value_of(word >> (8 * i + 4) & 15, zero_of(p), step_of(p)), a.kind);
-        *x = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
 // ---------------------------------------------------------------------------
 // Eviction.  select: a CTA per (sequence, kv head) finds the (keep - recent)-th
-// largest weight of the older rows bit by bit, then walks the rows in order and
-// writes the kept ones' indices and weights.  move: the records follow.  Rows
-// only move down, so a chunk that is loaded whole before it is stored never
-// overwrites a row that is still to be read: the same walk serves in place.
+// largest weight of the older rows, 8 bits of it a pass by a histogram in shared
+// memory, then writes the kept rows' indices in order (each warp a contiguous
+// part of the rows, whose counts are added up first) and gathers the weights.
+// move: the records follow.  Rows only move down, so rows that are loaded before
+// any row behind them is stored over serve in place too.
 // ---------------------------------------------------------------------------
 constexpr int kEvictThreads = 1024;
+constexpr int kEvictWarps = kEvictThreads / 32;
 
 // Weights ordered as unsigned integers: -0 as 0, NaN above everything.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -121,105 +137,170 @@ __device__ __forceinline__ int64_t live_rows(const rvq_cache4_evict_args& a, int
 }
 
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(rvq_cache4_evict_args a) {
-    __shared__ int red[kEvictThreads / 32];
+    __shared__ int hist[256];
+    __shared__ int above[kEvictWarps], equal[kEvictWarps];
+    __shared__ uint32_t sh_bar;
+    __shared__ int sh_want;
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.x / a.cache.n_kv;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t n = live_rows(a, b);
+    const int64_t live = live_rows(a, b);
+    const int n = (int)(live < 0 ? 0 : live);
     const float* w = a.weights + (int64_t)blockIdx.x * a.cache.max_len;
     float* wo = a.out_weights + (int64_t)blockIdx.x * a.out.max_len;
     int32_t* kept = a.kept + (int64_t)blockIdx.x * a.keep;
-    if (a.new_rows != nullptr && blockIdx.x % a.cache.n_kv == 0 && tid == 0)
-        a.new_rows[b] = n < a.keep ? n : a.keep;
-    const int64_t old = n > a.keep ? n - a.recent : 0;      // rows [0, old) compete for want places
-    const int want = a.keep - a.recent;
-    uint32_t bar = 0;
-    int ties = 0;
-    if (n > a.keep && want > 0) {
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t cand = bar | 1u << bit;
-            int c = 0;
-            for (int64_t i = tid; i < old; i += kEvictThreads) c += order_key(w[i]) >= cand;
-            for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-            __syncthreads();
-            if (lane == 0) red[warp] = c;
-            __syncthreads();
-            int t = 0;
-            for (int i = 0; i < kEvictThreads / 32; ++i) t += red[i];
-            if (t >= want) bar = cand;
+    if (a.new_rows != nullptr && blockIdx.x % a.cache.n_kv == 0 && tid == 0) a.new_rows[b] = live < a.keep ? live : a.keep;
+    if (n <= a.keep) {                                      // every row stays
+        for (int i = tid; i < a.keep; i += kEvictThreads) {
+            kept[i] = i < n ? i : -1;
+            if (i < n && wo != w) wo[i] = w[i];
         }
-        int c = 0;
-        for (int64_t i = tid; i < old; i += kEvictThreads) c += order_key(w[i]) > bar;
-        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-        __syncthreads();
-        if (lane == 0) red[warp] = c;
-        __syncthreads();
-        ties = want;
-        for (int i = 0; i < kEvictThreads / 32; ++i) ties -= red[i];
+        return;
     }
-    int64_t at = 0;                                         // rows written so far
-    int tied = 0;                                           // equal rows seen so far
-    for (int64_t base = 0; base < n; base += kEvictThreads) {
-        const int64_t i = base + tid;
-        const float v = i < n ? w[i] : 0.f;
-        const uint32_t key = order_key(v);
-        const bool older = i < old;
-        const bool tie = older && want > 0 && key == bar;
+    const int old = n - a.recent;                           // rows [0, old) compete for want places
+    uint32_t bar = 0, mask = 0;                             // the bits of the want-th largest key found so far
+    int want = a.keep - a.recent;                           // among the keys with those bits
+    const bool select = want > 0;
+    if (select) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            if (tid < 256) hist[tid] = 0;
+            __syncthreads();
+            for (int base = 0; base < old; base += kEvictThreads) {
+                const int i = base + tid;
+                const uint32_t key = i < old ? order_key(w[i]) : 0;
+                const bool in = i < old && (key & mask) == bar;
+                // keys share their high bits: one addition for the lanes of a bin
+                const uint32_t act = __ballot_sync(0xffffffffu, in);
+                if (in) {
+                    const uint32_t bin = key >> shift & 255;
+                    const uint32_t same = __match_any_sync(act, bin);
+                    if (lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+                }
+            }
+            __syncthreads();
+            if (warp == 0) {
+                // the bin where the count from the top reaches want; lane l: bins 255 - 8 l .. 248 - 8 l
+                int c[8], sum = 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) c[k] = hist[255 - 8 * lane - k], sum += c[k];
+                int upto = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                int before = upto - sum;
+                if (before < want && want <= upto) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if (before < want && want <= before + c[k]) {
+                            sh_bar = bar | (uint32_t)(255 - 8 * lane - k) << shift;
+                            sh_want = want - before;
+                        }
+                        before += c[k];
+                    }
+                }
+            }
+            __syncthreads();
+            bar = sh_bar;
+            want = sh_want;
+            mask |= 255u << shift;
+        }
+    }
+    // rows above bar, and the first `want` of those at it; each warp its part of the rows
+    const int part = (n + kEvictThreads - 1) / kEvictThreads * 32;
+    const int r0 = min(n, warp * part), r1 = min(n, r0 + part);
+    int na = 0, ne = 0;
+    for (int base = r0; base < r1; base += 32) {
+        const int i = base + lane;
+        const uint32_t key = i < r1 && i < old ? order_key(w[i]) : 0;
+        na += __popc(__ballot_sync(0xffffffffu, i < r1 && (i >= old || (select && key > bar))));
+        ne += __popc(__ballot_sync(0xffffffffu, i < r1 && i < old && select && key == bar));
+    }
+    if (lane == 0) above[warp] = na, equal[warp] = ne;
+    __syncthreads();
+    int pos = 0, tied = 0;                                  // rows kept, and rows at bar, before this warp's
+    for (int k = 0; k < warp; ++k) {
+        pos += above[k];
+        tied += equal[k];
+    }
+    pos += min(tied, want);
+    for (int base = r0; base < r1; base += 32) {
+        const int i = base + lane;
+        const uint32_t key = i < r1 && i < old ? order_key(w[i]) : 0;
+        const bool tie = i < r1 && i < old && select && key == bar;
         const uint32_t tb = __ballot_sync(0xffffffffu, tie);
-        __syncthreads();
-        if (lane == 0) red[warp] = __popc(tb);
-        __syncthreads();
-        int rank = tied + __popc(tb & ((1u << lane) - 1));
-        for (int k = 0; k < kEvictThreads / 32; ++k) {
-            if (k < warp) rank += red[k];
-            tied += red[k];
-        }
-        const bool keep = i < n && (!older || (want > 0 && (key > bar || (tie && rank < ties))));
+        const uint32_t below = (1u << lane) - 1;
+        const bool keep = i < r1 && (i >= old || (select && key > bar) || (tie && tied + __popc(tb & below) < want));
         const uint32_t kb = __ballot_sync(0xffffffffu, keep);
-        __syncthreads();                                    // the chunk's weights are read, and red
-        if (lane == 0) red[warp] = __popc(kb);
-        __syncthreads();
-        int64_t pos = at + __popc(kb & ((1u << lane) - 1));
-        for (int k = 0; k < kEvictThreads / 32; ++k) {
-            if (k < warp) pos += red[k];
-            at += red[k];
+        if (keep) kept[pos + __popc(kb & below)] = i;
+        pos += __popc(kb);
+        tied += __popc(tb);
+    }
+    __syncthreads();                                        // kept is complete, and the old weights are read
+    constexpr int U = 8;
+    for (int base = 0; base < a.keep; base += kEvictThreads * U) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = base + u * kEvictThreads + tid;
+            if (i < a.keep) v[u] = w[kept[i]];
         }
-        if (keep) {
-            kept[pos] = (int32_t)i;
-            wo[pos] = v;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = base + u * kEvictThreads + tid;
+            if (i < a.keep) wo[i] = v[u];
         }
     }
-    for (int64_t i = (at > 0 ? at : 0) + tid; i < a.keep; i += kEvictThreads) kept[i] = -1;
 }
 
 constexpr int kMoveThreads = 512;
+constexpr int kMoveLoads = 8;
 
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(rvq_cache4_evict_args a, int vecs) {
+// blockIdx.y: apart, a part of the rows; in place, a fifth of every record (its rows depend on one another, its columns do
+// not): 32 or 16 bytes wide, whole sectors of a head_dim 128 record.
+template <int VECS>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(rvq_cache4_evict_args a) {
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t n = live_rows(a, blockIdx.x / a.cache.n_kv);
+    const int64_t live = live_rows(a, blockIdx.x / a.cache.n_kv);
     const bool in_place = a.out.data == a.cache.data;
-    if (n <= 0 || (in_place && n <= a.keep)) return;
-    const int count = (int)(n < a.keep ? n : a.keep);
-    const uint4* src = reinterpret_cast<const uint4*>(a.cache.data) + (int64_t)blockIdx.x * a.cache.max_len * vecs;
-    uint4* dst = reinterpret_cast<uint4*>(a.out.data) + (int64_t)blockIdx.x * a.out.max_len * vecs;
+    if (live <= 0 || (in_place && live <= a.keep)) return;
+    const int count = (int)(live < a.keep ? live : a.keep);
+    const uint4* src = reinterpret_cast<const uint4*>(a.cache.data) + (int64_t)blockIdx.x * a.cache.max_len * VECS;
+    uint4* dst = reinterpret_cast<uint4*>(a.out.data) + (int64_t)blockIdx.x * a.out.max_len * VECS;
     const int32_t* kept = a.kept + (int64_t)blockIdx.x * a.keep;
-    constexpr int U = 4;
-    const int64_t total = (int64_t)count * vecs;
-    for (int64_t base = 0; base < total; base += kMoveThreads * U) {
+    constexpr int U = kMoveLoads, W = VECS / 5;
+    if (!in_place) {
+        const int64_t total = (int64_t)count * VECS;
+        for (int64_t base = (int64_t)blockIdx.y * kMoveThreads * U; base < total; base += (int64_t)gridDim.y * kMoveThreads * U) {
+            uint4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t i = base + u * kMoveThreads + threadIdx.x;
+                const int row = (int)(i / VECS);
+                if (i < total) v[u] = src[(int64_t)__ldg(kept + row) * VECS + (i - (int64_t)row * VECS)];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t i = base + u * kMoveThreads + threadIdx.x;
+                if (i < total) dst[i] = v[u];
+            }
+        }
+        return;
+    }
+    const int rows = kMoveThreads / W, col = blockIdx.y * W + threadIdx.x % W, r = threadIdx.x / W;
+    for (int base = 0; base < count; base += rows * U) {
         uint4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t i = base + u * kMoveThreads + threadIdx.x;
-            if (i < total) v[u] = src[(int64_t)kept[i / vecs] * vecs + i % vecs];
-        }
-        if (in_place) __syncthreads();
+        for (int u = 0; u < U; ++u)
+            if (base + u * rows + r < count) v[u] = src[(int64_t)__ldg(kept + base + u * rows + r) * VECS + col];
+        __syncthreads();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t i = base + u * kMoveThreads + threadIdx.x;
-            if (i < total) dst[i] = v[u];
-        }
+        for (int u = 0; u < U; ++u)
+            if (base + u * rows + r < count) dst[(int64_t)(base + u * rows + r) * VECS + col] = v[u];
     }
 }
 
@@ -249,10 +330,11 @@ template <bool kWrite>
 int run_rows(const rvq_cache4_rows_args* a, void* stream) {
     const int rc = check_rows(a);
     if (rc != RVQ_OK || a->tokens == 0) return rc;
-    const int64_t blocks = (a->tokens * a->cache.n_kv * (a->cache.head_dim / 4) + kRowsThreads - 1) / kRowsThreads;
-    if (blocks >= (1ll << 31)) return RVQ_ERR_TOO_LARGE;
+    const int per_block = kTokens * kRowsThreads / (a->cache.head_dim / 4);
+    const int64_t blocks = (a->tokens + per_block - 1) / per_block;
+    if (a->cache.n_kv > 65535) return RVQ_ERR_TOO_LARGE;
     auto* kernel = a->cache.head_dim == 128 ? cache4_rows_kernel<128, kWrite> : cache4_rows_kernel<64, kWrite>;
-    return status(launch_pdl(kernel, dim3((unsigned)blocks), dim3(kRowsThreads), 0, (cudaStream_t)stream, *a));
+    return status(launch_pdl(kernel, dim3((unsigned)blocks, a->cache.n_kv), dim3(kRowsThreads), 0, (cudaStream_t)stream, *a));
 }
 
 // Whether two byte ranges share a byte.
@@ -299,6 +381,10 @@ extern "C" int rvq_cache4_evict(const rvq_cache4_evict_args* a, void* stream) {
     if (a->new_rows != nullptr && overlap(a->rows, 8ll * c.n_seq, a->new_rows, 8ll * c.n_seq)) return RVQ_ERR_INVALID;
     rc = status(launch_pdl(evict_select_kernel, dim3((unsigned)heads), dim3(kEvictThreads), 0, (cudaStream_t)stream, *a));
     if (rc != RVQ_OK) return rc;
-    return status(launch_pdl(evict_move_kernel, dim3((unsigned)heads), dim3(kMoveThreads), 0, (cudaStream_t)stream, *a,
-                             record_bytes(c.head_dim) / 16));
+    // apart: blocks of 8 loads a thread, a few thousand of them at most; in place: the five columns
+    const int vecs = record_bytes(c.head_dim) / 16;
+    const int64_t chunks = ((int64_t)a->keep * vecs + kMoveThreads * kMoveLoads - 1) / (kMoveThreads * kMoveLoads);
+    const unsigned parts = o.data == c.data ? 5 : (unsigned)(chunks < 64 ? chunks : 64);
+    auto* move = c.head_dim == 128 ? evict_move_kernel<10> : evict_move_kernel<5>;
+    return status(launch_pdl(move, dim3((unsigned)heads, parts), dim3(kMoveThreads), 0, (cudaStream_t)stream, *a));
 }

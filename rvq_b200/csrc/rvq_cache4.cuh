@@ -22,10 +22,19 @@ __device__ __forceinline__ uint32_t params_of(float lo, float hi) {
            (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(step)) << 16;
 }
 
-// clamp(rint((x - z) / s), 0, 15); 0 for s = 0 and for a quotient that is NaN.
+// clamp(rint((x - z) / s), 0, 15) with an IEEE quotient; 0 for s = 0 and for a quotient that is NaN.
 __device__ __forceinline__ uint32_t code_of(float x, float zero, float step) {
     const float q = rintf(__fdiv_rn(__fsub_rn(x, zero), step));
     return step > 0.f && q > 0.f ? (uint32_t)fminf(q, 15.0f) : 0u;
+}
+
+// The same with inv = 1 / step (approximate): where the product is clearly nearer to one integer than to the next, that
+// integer is the quotient's too (|d - k s| < 0.4999 s leaves 2^-13 for the roundings of d inv, of d - k s and of the
+// quotient, 2^-22 each); only the others divide.
+__device__ __forceinline__ uint32_t code_of(float x, float zero, float step, float inv) {
+    const float d = __fsub_rn(x, zero), k = rintf(__fmul_rn(d, inv));
+    if (fabsf(fmaf(-k, step, d)) < 0.4999f * step && k < 64.f) return k > 0.f ? (uint32_t)fminf(k, 15.0f) : 0u;
+    return code_of(x, zero, step);
 }
 
 // z + s c (s c is exact: 8 by 4 bits)

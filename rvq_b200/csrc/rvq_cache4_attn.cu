@@ -14,9 +14,7 @@ namespace rvq {
 namespace cache4 {
 
 using namespace stepops;
-using namespace sm100;
-
-__device__ int g_step_timeout;               // sticky: a bounded wait gave up
+using sm100::smem_addr;
 
 // ---------------------------------------------------------------------------
 // A cluster of C CTAs per (kv head, group of at most 8 query heads, sequence)
@@ -40,11 +38,11 @@ __device__ int g_step_timeout;               // sticky: a bounded wait gave up
 // ---------------------------------------------------------------------------
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = 32;                    // rows of a ring stage
-constexpr int kStages = 3;
-constexpr int kHeads = 8;                    // query heads of a pass
+constexpr int kTile = 16;                    // rows of a ring stage
+constexpr int kStages = 4;
+constexpr int kHeads = kWarps;               // query heads of a pass (a warp each where heads are worked on)
 constexpr int kMaxRep = 64;
-constexpr long long kWaitPolls = 1ll << 22;  // a try_wait sleeps in hardware: seconds
+constexpr float kGrow = 8.f;
 
 template <int HD>
 struct Smem {
@@ -58,23 +56,40 @@ struct Smem {
     float wm[kWarps][kHeads], wl[kWarps][kHeads];
     float m[kHeads], l[kHeads];              // this CTA's maximum and sum
     float fm[kHeads], fr[kHeads];            // the final maximum and 1 / sum
-    alignas(8) uint64_t bar[kWarps][kStages];
 };
 
-// 1 + c / 16 for the codes in bits 4 i .. 4 i + 3 and 4 i + 16 .. of a word
+// c / 64 for the codes c in bits 4 I .. and 4 I + 16 .. (I = 0 or 1) of a word, as a bf16 pair.  A code in a bf16
+// number's lowest bits is the (sub)normal number c 2^-133 (c 2^-129 in bits 4 to 7: the step from the mantissa into the
+// exponent is linear there), which one multiplication makes c / 64: exact, and on the FMA pipe, of which there is more.
 template <int I>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-    const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3 > 0 ? 4 * I - 3 : 0);
     uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(0x00780078u), "r"(0x3f803f80u));   // (x & m) | o
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w & (I ? 0x00f000f0u : 0x000f000fu)), "r"(I ? 0x7d007d00u : 0x7f007f00u));
     return r;
 }
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+// Numbers of a parameter word: the shift as a multiplication (`shift` holds 65536 where the compiler cannot see it), which
+// runs on the FMA pipe; the masks and shifts of this kernel's integer pipe are what bounds it.
+__device__ __forceinline__ float zero_by(uint32_t p, uint32_t shift) {
+    uint32_t r;
+    asm("mul.lo.u32 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(shift));
+    return __uint_as_float(r);
+}
+
+// D += A B, and D = A B
+__device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_set(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -83,9 +98,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 
 // hi + lo = x to 16 bits
-__device__ __forceinline__ void split_bf16(float x, float y, uint32_t* hi, uint32_t* lo) {
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t* hi, uint32_t* lo, uint32_t shift) {
     *hi = pack_bf16(x, y);
-    *lo = pack_bf16(x - __uint_as_float(*hi << 16), y - __uint_as_float(*hi & 0xffff0000u));
+    *lo = pack_bf16(x - zero_by(*hi, shift), y - step_of(*hi));
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -94,138 +109,134 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
+// 16 bytes to shared memory, or 16 zero bytes.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-// What a warp carries over its tiles.  Lane 4 g + t: head g's maximum, the parts of its sums over this lane's rows,
-// and output values of head g (bf16 parts, then remainders).
+// What a warp carries over its tiles.  Lane 4 g + t: head g's maximum and this lane's part of its sum; of the sums of
+// p zero and p step, those of group t for head g (and the parts from p's remainder); and of the output, transposed: heads
+// 2 t and 2 t + 1, value 4 g + i of group G in o[G][i / 2][2 (i & 1) + (0, 1)].
 template <int HD>
 struct State {
     static constexpr int G = HD / kGroup;
     float m, l;
-    float zero[G];                           // sum of p (zero - 16 step)
-    float o[G][4][4];
+    float zero[4];
+    float o[G][2][4];
 };
 
-// One tile of `valid` rows (the records behind them hold zeros if valid < kTile).
+template <int G>
+__device__ __forceinline__ void load_words(uint32_t (&w)[G], uint32_t addr) {
+    if constexpr (G == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+    else
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+}
+
+// A tile of 16 rows, `valid` of them live (the records behind those hold zeros).
 template <int HD, bool kSplitQ>
-__device__ __forceinline__ void tile_step(const uint8_t* rec, int valid, const uint32_t (&qa)[HD / 16][kSplitQ ? 4 : 2],
-                                          const float (&qs)[HD / kGroup], float scale16, State<HD>& st, float* scores) {
-    constexpr int G = HD / kGroup, REC = record_bytes(HD);
+__device__ __forceinline__ void tile_step(uint32_t base, int valid, const uint32_t (&qa)[HD / 16][kSplitQ ? 4 : 2],
+                                          const uint32_t (&qz)[3], float scale64, uint32_t shift, State<HD>& st,
+                                          float* scores) {
+    constexpr int G = HD / kGroup, REC = record_bytes(HD), kLo = kSplitQ ? 2 : 0;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll 1
-    for (int half = 0; half < kTile / 16; ++half) {
-        if (half * 16 >= valid) break;
-        const uint8_t* base = rec + half * 16 * REC;
-        // columns n of a score tile hold row (n with its two low bits swapped): a quarter warp's 16-byte loads of two
-        // rows then fall into different banks, and this lane's columns 2 t and 2 t + 1 are rows ra and ra + 2
-        const int rn = (g & 4) | (g & 1) << 1 | (g >> 1 & 1);
-        const int ra = (t >> 1) * 4 + (t & 1);
-        float s[4];
+    // columns n of a score tile hold row (n with its two low bits swapped): a quarter warp's 16-byte loads of two
+    // rows then fall into different banks, and this lane's columns 2 t and 2 t + 1 are rows ra and ra + 2
+    const int rn = (g & 4) | (g & 1) << 1 | (g >> 1 & 1);
+    const int ra = (t >> 1) * 4 + (t & 1);
+    float s[4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const uint8_t* r0 = base + (8 * n + ra) * REC + HD;
-            uint32_t kc[G], pa[G], pb[G];
-            if constexpr (HD == 128) {
-                *reinterpret_cast<uint4*>(kc) = *reinterpret_cast<const uint4*>(base + (8 * n + rn) * REC + 16 * t);
-                *reinterpret_cast<uint4*>(pa) = *reinterpret_cast<const uint4*>(r0);
-                *reinterpret_cast<uint4*>(pb) = *reinterpret_cast<const uint4*>(r0 + 2 * REC);
-            } else {
-                *reinterpret_cast<uint2*>(kc) = *reinterpret_cast<const uint2*>(base + (8 * n + rn) * REC + 8 * t);
-                *reinterpret_cast<uint2*>(pa) = *reinterpret_cast<const uint2*>(r0);
-                *reinterpret_cast<uint2*>(pb) = *reinterpret_cast<const uint2*>(r0 + 2 * REC);
-            }
-            float sa = 0.f, sb = 0.f;
+    for (int n = 0; n < 2; ++n) {
+        const uint32_t rk = base + (8 * n + rn) * REC, r0 = base + (8 * n + ra) * REC + HD;
+        uint32_t kc[G], pa[G], pb[G], pz;
+        load_words<G>(kc, rk + 4 * G * t);
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pz) : "r"(rk + HD + 4 * (t & (G - 1))));
+        load_words<G>(pa, r0);
+        load_words<G>(pb, r0 + 2 * REC);
+        float z[4], c[G][4];                                 // zero . (q . 1) / 64; q . c / 64 of every group
+        mma_set(z, qz[0], qz[2], qz[1], 0u, pz, pz);
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                float c[4] = {-qs[i], -qs[i], 0.f, 0.f};
+        for (int i = 0; i < G; ++i)
+            mma_set(c[i], qa[2 * i][0], kSplitQ ? qa[2 * i][kLo] : 0u, qa[2 * i][1], kSplitQ ? qa[2 * i][kLo + 1] : 0u,
+                    code_pair<0>(kc[i]), code_pair<1>(kc[i]));
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    uint32_t a[4] = {qa[2 * i + k][0], 0u, qa[2 * i + k][1], 0u};
-                    if constexpr (kSplitQ) a[1] = qa[2 * i + k][2], a[3] = qa[2 * i + k][3];
-                    mma16816(c, a, k ? code_pair<2>(kc[i]) : code_pair<0>(kc[i]), k ? code_pair<3>(kc[i]) : code_pair<1>(kc[i]));
-                }
-                if constexpr (kSplitQ) c[0] += c[2], c[1] += c[3];
-                // in units of 16: step (q . c) / 16 + zero (q . 1) / 16
-                sa = fmaf(step_of(pa[i]), c[0], fmaf(zero_of(pa[i]), qs[i] * 0.0625f, sa));
-                sb = fmaf(step_of(pb[i]), c[1], fmaf(zero_of(pb[i]), qs[i] * 0.0625f, sb));
-            }
-            s[2 * n] = sa * scale16;
-            s[2 * n + 1] = sb * scale16;
-        }
-        if (half * 16 + 16 > valid) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (half * 16 + 8 * (i >> 1) + ra + 2 * (i & 1) >= valid) s[i] = -INFINITY;
-        }
-        if (scores != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = half * 16 + 8 * (i >> 1) + ra + 2 * (i & 1);
-                if (row < valid) scores[row] = s[i];
-            }
-        }
-        float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const bool grows = top > st.m;
-        if (__any_sync(0xffffffffu, grows)) {
-            const float m = fmaxf(st.m, top);
-            const float f = st.m == m ? 1.f : exp2_approx(st.m - m);
-            st.m = m;
-            st.l *= f;
-#pragma unroll
-            for (int i = 0; i < G; ++i) {
-                st.zero[i] *= f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) st.o[i][j][c] *= f;
-            }
-        }
-        // nothing but -infinities so far: p = exp(-infinity) = 0, not exp(-infinity + infinity)
-        const float sub = st.m == -INFINITY ? 0.f : st.m;
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            p[i] = exp2_approx(s[i] - sub);
-            st.l += p[i];
-        }
-        uint32_t vc[4][G], vp[4][G];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint8_t* r = base + (8 * (i >> 1) + ra + 2 * (i & 1)) * REC;
-            if constexpr (HD == 128) {
-                *reinterpret_cast<uint4*>(vc[i]) = *reinterpret_cast<const uint4*>(r + HD / 2 + 16 * (g >> 1));
-                *reinterpret_cast<uint4*>(vp[i]) = *reinterpret_cast<const uint4*>(r + HD + HD / 8);
-            } else {
-                *reinterpret_cast<uint2*>(vc[i]) = *reinterpret_cast<const uint2*>(r + HD / 2 + 8 * (g >> 1));
-                *reinterpret_cast<uint2*>(vp[i]) = *reinterpret_cast<const uint2*>(r + HD + HD / 8);
-            }
-        }
-        const uint32_t half_sel = g & 1 ? 0x7632u : 0x5410u;      // this lane's 4 values are half a code word
+        for (int i = 0; i < G; ++i)
+            mma_add(c[i], qa[2 * i + 1][0], kSplitQ ? qa[2 * i + 1][kLo] : 0u, qa[2 * i + 1][1],
+                    kSplitQ ? qa[2 * i + 1][kLo + 1] : 0u, code_pair<0>(kc[i] >> 8), code_pair<1>(kc[i] >> 8));
+        float sa = z[0] + z[2], sb = z[1] + z[3];
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            float ps[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float step = step_of(vp[k][i]);
-                ps[k] = p[k] * step;
-                st.zero[i] = fmaf(p[k], fmaf(-16.f, step, zero_of(vp[k][i])), st.zero[i]);
-            }
-            uint32_t a[4];
-            split_bf16(ps[0], ps[1], &a[0], &a[1]);
-            split_bf16(ps[2], ps[3], &a[2], &a[3]);
-            const uint32_t w0 = __byte_perm(vc[0][i], vc[1][i], half_sel);
-            const uint32_t w1 = __byte_perm(vc[2][i], vc[3][i], half_sel);
-            mma16816(st.o[i][0], a, code_pair<0>(w0), code_pair<0>(w1));
-            mma16816(st.o[i][1], a, code_pair<1>(w0), code_pair<1>(w1));
-            mma16816(st.o[i][2], a, code_pair<2>(w0), code_pair<2>(w1));
-            mma16816(st.o[i][3], a, code_pair<3>(w0), code_pair<3>(w1));
+            if constexpr (kSplitQ) c[i][0] += c[i][2], c[i][1] += c[i][3];
+            sa = fmaf(step_of(pa[i]), c[i][0], sa);
+            sb = fmaf(step_of(pb[i]), c[i][1], sb);
         }
+        s[2 * n] = sa * scale64;
+        s[2 * n + 1] = sb * scale64;
+    }
+    if (valid < 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (8 * (i >> 1) + ra + 2 * (i & 1) >= valid) s[i] = -INFINITY;
+    }
+    if (scores != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 8 * (i >> 1) + ra + 2 * (i & 1);
+            if (row < valid) scores[row] = s[i];
+        }
+    }
+    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    // the maximum that is subtracted follows the true one only when that has grown by 2^8 (p stays below 2^8): of 32
+    // rows and heads some has a new maximum in most tiles, and following it at once costs a fifth of the loop
+    if (__any_sync(0xffffffffu, top > st.m + kGrow)) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m = fmaxf(st.m, top);
+        const float f = st.m == m ? 1.f : exp2_approx(st.m - m);
+        st.m = m;
+        st.l *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.zero[i] *= f;
+        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                st.o[i][j][0] *= f0, st.o[i][j][2] *= f0;
+                st.o[i][j][1] *= f1, st.o[i][j][3] *= f1;
+            }
+    }
+    // nothing but -infinities so far: p = exp(-infinity) = 0, not exp(-infinity + infinity)
+    const float sub = st.m == -INFINITY ? 0.f : st.m;
+    float p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = exp2_approx(s[i] - sub);
+    st.l += (p[0] + p[1]) + (p[2] + p[3]);
+    uint32_t vc[4][G], vp[4][G], h[4], zs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t r = base + (8 * (i >> 1) + ra + 2 * (i & 1)) * REC + HD / 2;
+        load_words<G>(vc[i], r + 4 * G * (g >> 1));
+        load_words<G>(vp[i], r + HD / 2 + HD / 8);
+        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(zs[i]) : "r"(r + HD / 2 + HD / 8 + 2 * (g & (2 * G - 1))));
+    }
+    // sums of p zero (columns 2 group) and p step (2 group + 1)
+    split_bf16(p[0], p[1], &h[0], &h[1], shift);
+    split_bf16(p[2], p[3], &h[2], &h[3], shift);
+    mma_add(st.zero, h[0], h[1], h[2], h[3], __byte_perm(zs[0], zs[1], 0x5410u), __byte_perm(zs[2], zs[3], 0x5410u));
+    const uint32_t half_sel = g & 1 ? 0x7632u : 0x5410u;     // this lane's 4 values are half a code word
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        split_bf16(p[0] * step_of(vp[0][i]), p[1] * step_of(vp[1][i]), &h[0], &h[1], shift);
+        split_bf16(p[2] * step_of(vp[2][i]), p[3] * step_of(vp[3][i]), &h[2], &h[3], shift);
+        const uint32_t w0 = __byte_perm(vc[0][i], vc[1][i], half_sel), w1 = __byte_perm(vc[2][i], vc[3][i], half_sel);
+        const uint32_t v0 = code_pair<0>(w0), v1 = code_pair<1>(w0), v2 = code_pair<0>(w1), v3 = code_pair<1>(w1);
+        const uint32_t x0 = code_pair<0>(w0 >> 8), x1 = code_pair<1>(w0 >> 8);
+        const uint32_t x2 = code_pair<0>(w1 >> 8), x3 = code_pair<1>(w1 >> 8);
+        mma_add(st.o[i][0], v0, v1, v2, v3, h[0], h[2]);
+        mma_add(st.o[i][1], x0, x1, x2, x3, h[0], h[2]);
+        mma_add(st.o[i][0], v0, v1, v2, v3, h[1], h[3]);
+        mma_add(st.o[i][1], x0, x1, x2, x3, h[1], h[3]);
     }
 }
 
@@ -284,7 +295,7 @@ __device__ __forceinline__ void encode(const float* x, uint8_t* codes, uint32_t*
 }
 
 template <int HD, bool kSplitQ>
-__global__ void __launch_bounds__(kThreads, 1) cache4_attn_kernel(rvq_cache4_attn_args a, int passes) {
+__global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_attn_args a, int passes) {
     constexpr int G = HD / kGroup, REC = record_bytes(HD);
     extern __shared__ __align__(128) uint8_t smem_raw[];
     Smem<HD>& S = *reinterpret_cast<Smem<HD>*>(smem_raw);
@@ -294,11 +305,6 @@ __global__ void __launch_bounds__(kThreads, 1) cache4_attn_kernel(rvq_cache4_att
     const int nkv = a.cache.n_kv, rep = a.n_heads / nkv;
     const int kv = blockIdx.y % nkv, b = blockIdx.z;
     pdl_launch_dependents();
-    if (lane == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(smem_addr(&S.bar[warp][i]), 1);
-        mbar_init_fence();
-        fence_async_shared();
-    }
     pdl_wait();
     const int64_t rows = a.rows[b];
     if (rows < 0) return;                                    // the same in every CTA of the cluster
@@ -322,23 +328,28 @@ __global__ void __launch_bounds__(kThreads, 1) cache4_attn_kernel(rvq_cache4_att
     const int t0 = (int)((int64_t)tiles * rank / C), t1 = (int)((int64_t)tiles * (rank + 1) / C);
     const bool owner = append && rank == 0;                  // this CTA attends to the new row
 
-    int issued = 0, used = 0;                                // ring stages filled and read by this warp
-    bool dead = false;                                       // a copy did not arrive: the result is invalid, flagged
-    auto issue = [&](int tile) {                             // lane 0
-        const int valid = (int)min((int64_t)kTile, rows - (int64_t)tile * kTile);
-        const uint32_t bar = smem_addr(&S.bar[warp][issued % kStages]);
-        mbar_expect_tx(bar, (uint32_t)(valid * REC));
-        bulk_load(smem_addr(S.ring[warp][issued % kStages]), cache + (int64_t)tile * kTile * REC, (uint32_t)(valid * REC), bar);
-        ++issued;
+    uint32_t shift;
+    asm volatile("mov.u32 %0, 65536;" : "=r"(shift));
+    const int live = (int)rows;
+    // this lane's 16-byte pieces of tile number `tile`, into a stage of the warp's ring; a group for every stage, so that
+    // the number of groups behind a tile is known
+    const uint32_t ring = smem_addr(S.ring[warp][0]) + 16 * lane;
+    auto fetch = [&](int tile, int stage) {
+        if (tile < t1) {
+            const uint8_t* src = cache + (int64_t)tile * (kTile * REC) + 16 * lane;
+            const int bytes = (live - tile * kTile) * REC - 16 * lane;
+#pragma unroll
+            for (int i = 0; i < (kTile * REC + 511) / 512; ++i)
+                if ((i + 1) * 512 <= kTile * REC || lane < kTile * REC % 512 / 16)
+                    copy16(ring + stage * (kTile * REC) + 512 * i, bytes > 512 * i ? src + 512 * i : cache, bytes > 512 * i);
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
 
     for (int pass = 0; pass < passes; ++pass) {
         const int h0 = (first + pass) * per, heads = min(per, rep - h0);
         const int64_t q_at = ((int64_t)b * a.n_heads + kv * rep + h0) * HD;
-        int next = t0 + warp;                                // this warp's next tile to fetch
-        if (lane == 0)
-            for (; !dead && issued - used < kStages && next < t1; next += kWarps) issue(next);
-        next = __shfl_sync(0xffffffffu, next, 0);
+        for (int i = 0; i < kStages - 1; ++i) fetch(t0 + warp + i * kWarps, i);
 
         // the heads' q, and the new record
         if (pass == 0 && (a.q_norm != nullptr || a.cos != nullptr)) {
@@ -368,24 +379,27 @@ __global__ void __launch_bounds__(kThreads, 1) cache4_attn_kernel(rvq_cache4_att
                 if (lane == 0) S.qsum[warp][i] = v[i];
             }
         }
-        if (owner && pass == 0 && warp < 2) {
+        if (owner && pass == 0 && warp < 2)                  // the warp that rotated the key, and another
             encode<HD>(S.kv[warp], S.fresh + warp * (HD / 2), reinterpret_cast<uint32_t*>(S.fresh + HD + warp * (HD / 8)));
-        }
         __syncthreads();
         if (owner && pass == 0 && first == 0 && tid < REC / 16)
             reinterpret_cast<uint4*>(cache + rows * REC)[tid] = reinterpret_cast<const uint4*>(S.fresh)[tid];
 
         // operand rows 0..7: q (its bf16 part), rows 8..15: the remainder; column pairs in the code words' order
         uint32_t qa[HD / 16][kSplitQ ? 4 : 2];
-        float qs[G];
-#pragma unroll
-        for (int i = 0; i < G; ++i) qs[i] = S.qsum[g][i];
+        // (q . 1) / 64 of group t against the pairs (zero, step), in three bf16 parts: 24 bits
+        uint32_t qz[3] = {0u, 0u, 0u};
+        if (t < G) {
+            const float x = S.qsum[g][t] * 0.015625f;
+            const float hi = bf16r(x), lo = bf16r(x - hi);
+            qz[0] = pack_bf16(hi, 0.f), qz[1] = pack_bf16(lo, 0.f), qz[2] = pack_bf16(x - hi - lo, 0.f);
+        }
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
             const float* q = &S.q[g][i / 2 * kGroup + 8 * t + 2 * (i & 1)];
             if constexpr (kSplitQ) {
-                split_bf16(q[0], q[4], &qa[i][0], &qa[i][2]);
-                split_bf16(q[1], q[5], &qa[i][1], &qa[i][3]);
+                split_bf16(q[0], q[4], &qa[i][0], &qa[i][2], 65536u);
+                split_bf16(q[1], q[5], &qa[i][1], &qa[i][3], 65536u);
             } else {
                 qa[i][0] = pack_bf16(q[0], q[4]);
                 qa[i][1] = pack_bf16(q[1], q[5]);
@@ -394,64 +408,54 @@ __global__ void __launch_bounds__(kThreads, 1) cache4_attn_kernel(rvq_cache4_att
         State<HD> st;
         st.m = -INFINITY, st.l = 0.f;
 #pragma unroll
-        for (int i = 0; i < G; ++i) {
-            st.zero[i] = 0.f;
+        for (int i = 0; i < 4; ++i) st.zero[i] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < G; ++i) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) st.o[i][j][c] = 0.f;
         }
-        const float scale16 = a.scaling * 16.f * 1.4426950408889634f;      // scores in powers of two
+        const float scale64 = a.scaling * 64.f * 1.4426950408889634f;      // scores in powers of two
         float* sc = a.weights != nullptr && g < heads
                         ? a.scores + ((int64_t)b * a.n_heads + kv * rep + h0 + g) * a.cache.max_len : nullptr;
-        if (owner && warp == kWarps - 1) tile_step<HD, kSplitQ>(S.fresh, 1, qa, qs, scale16, st, sc ? sc + rows : sc);
-        for (int tile = t0 + warp; tile < t1 && !dead; tile += kWarps) {
-            const int slot = used % kStages;
-            const bool here = mbar_wait(smem_addr(&S.bar[warp][slot]), used / kStages & 1, kWaitPolls, &g_step_timeout);
-            if (__any_sync(0xffffffffu, !here)) {
-                dead = true;
-                break;
+        // the last warp begins with the appended record
+        bool extra = owner && warp == kWarps - 1;
+        for (int tile = t0 + warp, stage = 0; tile < t1 || extra;) {
+            uint32_t rec = smem_addr(S.fresh);
+            int row = live, valid = 1;
+            if (!extra) {
+                asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
+                __syncwarp();                                // every lane's pieces are here, and the stage before this one is read
+                fetch(tile + (kStages - 1) * kWarps, stage == 0 ? kStages - 1 : stage - 1);
+                rec = smem_addr(S.ring[warp][stage]);
+                row = tile * kTile;
+                valid = min(kTile, live - row);
+                tile += kWarps;
+                stage = stage + 1 == kStages ? 0 : stage + 1;
             }
-            const int valid = (int)min((int64_t)kTile, rows - (int64_t)tile * kTile);
-            uint8_t* rec = S.ring[warp][slot];
-            if (valid < kTile) {                             // only the last tile: no copy follows into this stage in this pass
-                for (int i = valid * REC / 16 + lane; i < kTile * REC / 16; i += 32)
-                    reinterpret_cast<uint4*>(rec)[i] = make_uint4(0, 0, 0, 0);
-                fence_async_shared();
-                __syncwarp();
-            }
-            tile_step<HD, kSplitQ>(rec, valid, qa, qs, scale16, st, sc ? sc + (int64_t)tile * kTile : sc);
-            __syncwarp();                                    // every lane has read the stage
-            ++used;
-            if (next < t1) {
-                if (lane == 0) issue(next);
-                next += kWarps;
-            }
+            extra = false;
+            tile_step<HD, kSplitQ>(rec, valid, qa, qz, scale64, shift, st, sc ? sc + row : sc);
         }
-        if (dead && lane == 0)                               // once more for the copies in flight, before their stages are reused
-            for (; used < issued; ++used)
-                mbar_wait(smem_addr(&S.bar[warp][used % kStages]), used / kStages & 1, kWaitPolls, &g_step_timeout);
-        __syncwarp();
         // lanes 4 g .. 4 g + 3 hold parts of head g's sums
         float l = st.l;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-            st.zero[i] += __shfl_xor_sync(0xffffffffu, st.zero[i], 1);
-            st.zero[i] += __shfl_xor_sync(0xffffffffu, st.zero[i], 2);
-        }
+        const float zero = st.zero[0] + st.zero[2];          // head g, group t
         __syncthreads();                                     // the rings are read: they take the warps' outputs
         float* wo = reinterpret_cast<float*>(S.ring);        // [kWarps][kHeads][HD], then the CTA's [kHeads][HD]
         float* co = wo + kWarps * kHeads * HD;
 #pragma unroll
-        for (int i = 0; i < G; ++i)
+        for (int i = 0; i < G; ++i) {
+            // the zeros' sums of heads 2 t and 2 t + 1
+            const float z0 = __shfl_sync(0xffffffffu, zero, 8 * t + i), z1 = __shfl_sync(0xffffffffu, zero, 8 * t + 4 + i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float* d = wo + (warp * kHeads + g) * HD + kGroup * i + 8 * t + j;
-                d[0] = fmaf(16.f, st.o[i][j][0] + st.o[i][j][2], st.zero[i]);
-                d[4] = fmaf(16.f, st.o[i][j][1] + st.o[i][j][3], st.zero[i]);
+                float* d = wo + (warp * kHeads + 2 * t) * HD + kGroup * i + 4 * g + j;
+                d[0] = fmaf(64.f, st.o[i][j >> 1][2 * (j & 1)], z0);
+                d[HD] = fmaf(64.f, st.o[i][j >> 1][2 * (j & 1) + 1], z1);
             }
+        }
         if (t == 0) S.wm[warp][g] = st.m, S.wl[warp][g] = l;
         __syncthreads();
         {
@@ -459,19 +463,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache4_attn_kernel(rvq_cache4_att
             float m = S.wm[0][warp];
 #pragma unroll
             for (int w = 1; w < kWarps; ++w) m = fmaxf(m, S.wm[w][warp]);
-            float f[kWarps], total = 0.f;
+            float total = 0.f, o[HD / 32];
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                f[w] = S.wm[w][warp] == m ? 1.f : exp2_approx(S.wm[w][warp] - m);
-                total = fmaf(f[w], S.wl[w][warp], total);
+                const float f = S.wm[w][warp] == m ? 1.f : exp2_approx(S.wm[w][warp] - m);
+                total = fmaf(f, S.wl[w][warp], total);
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d) o[d] = fmaf(f, wo[(w * kHeads + warp) * HD + 32 * d + lane], o[d]);
             }
 #pragma unroll
-            for (int d = lane; d < HD; d += 32) {
-                float o = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) o = fmaf(f[w], wo[(w * kHeads + warp) * HD + d], o);
-                co[warp * HD + d] = o;
-            }
+            for (int d = 0; d < HD / 32; ++d) co[warp * HD + 32 * d + lane] = o[d];
             if (lane == 0) S.m[warp] = m, S.l[warp] = total;
         }
         cluster.sync();
@@ -508,8 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache4_attn_kernel(rvq_cache4_att
             for (int64_t row = (int64_t)t0 * kTile + tid; row < r1; row += kThreads) add(row, w[row]);
             if (owner && tid == 0) add(rows, pass == 0 ? 0.f : w[rows]);
         }
-        fence_async_shared();                                // copies may fill the rings again
-        cluster.sync();                                      // once the others have read this CTA's parts
+        cluster.sync();                                      // the others have read this CTA's parts: the rings may be filled again
     }
 }
 
@@ -556,7 +558,7 @@ int run(const rvq_cache4_attn_args& a, cudaStream_t s) {
     const int passes = a.weights != nullptr ? groups : 1;
     const int64_t units = (int64_t)a.cache.n_seq * a.cache.n_kv * (groups / passes);
     int c = 1;
-    while (c < 16 && units * c * 2 <= sms && (int64_t)c * kWarps * kTile < a.cache.max_len) c *= 2;
+    while (c < 16 && units * c * 2 <= 2 * sms && (int64_t)c * kWarps * kTile < a.cache.max_len) c *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c, a.cache.n_kv * (groups / passes), a.cache.n_seq);
     cfg.blockDim = dim3(kThreads);
@@ -574,15 +576,6 @@ int run(const rvq_cache4_attn_args& a, cudaStream_t s) {
 }
 
 }  // namespace cache4
-
-// 1 if the sticky flag was set (it is cleared), 0 if not, a negative status on an error.
-int take_step_timeout() {
-    int v = 0;
-    const int zero = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&v, cache4::g_step_timeout, sizeof(int));
-    if (e == cudaSuccess) e = cudaMemcpyToSymbol(cache4::g_step_timeout, &zero, sizeof(int));
-    return e == cudaSuccess ? v : -cache4::status(e);
-}
 
 }  // namespace rvq
 

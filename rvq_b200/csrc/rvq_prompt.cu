@@ -10,9 +10,6 @@
 #include "rvq_sm100.cuh"
 
 namespace rvq {
-
-int take_step_timeout();                     // the step attention's flag (rvq_cache4_attn.cu)
-
 namespace prompt {
 
 using namespace sm100;
@@ -587,6 +584,5 @@ extern "C" int rvq_take_attention_timeout(void) {
         last_cuda_error_slot() = (int)e;
         return -RVQ_ERR_CUDA;
     }
-    const int step = take_step_timeout();
-    return step < 0 ? step : v | step;
+    return v;
 }

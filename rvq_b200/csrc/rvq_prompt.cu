@@ -111,6 +111,67 @@ __device__ __forceinline__ bool wait(Smem<HD>& S, uint64_t& bar, uint32_t parity
     return false;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// x b + c and y b + c in one instruction, each rounded as by itself
+__device__ __forceinline__ void fma2(float& x, float& y, float b, float c) {
+    asm("{\n .reg .b64 X, B, C;\n mov.b64 X, {%0, %1};\n mov.b64 B, {%2, %2};\n mov.b64 C, {%3, %3};\n"
+        " fma.rn.f32x2 X, X, B, C;\n mov.b64 {%0, %1}, X;\n}\n"
+        : "+f"(x), "+f"(y)
+        : "f"(b), "f"(c));
+}
+
+// A row's scores of a tile in r (a thread's TMEM lane): its columns from `seen` on are hidden.
+template <bool kMasked>
+__device__ __forceinline__ float row_max(float (&s)[4][32], int seen) {
+    if constexpr (kMasked) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (32 * x + e >= seen) s[x][e] = -INFINITY;
+    }
+    float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < 32; e += 2)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) t[x] = max3(t[x], s[x][e], s[x][e + 1]);
+    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+}
+
+// p = 2^(c s - sub) over the scores in TMEM, in the operand type; returns their sum.
+template <bool kMasked, bool kHalfType>
+__device__ __forceinline__ float row_exp(float (&s)[4][32], int seen, float c, float sub, uint32_t ts) {
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; x += 2) {
+        uint32_t w[32];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+                float& p0 = s[x + y][e];
+                float& p1 = s[x + y][e + 1];
+                fma2(p0, p1, c, -sub);
+                p0 = exp2_approx(p0);
+                p1 = exp2_approx(p1);
+                if constexpr (kMasked) {                     // c may be 0
+                    if (32 * (x + y) + e >= seen) p0 = 0.f;
+                    if (32 * (x + y) + e + 1 >= seen) p1 = 0.f;
+                }
+                part[2 * y] += p0;
+                part[2 * y + 1] += p1;
+                w[16 * y + e / 2] = pack2(p0, p1, kHalfType ? RVQ_F16 : RVQ_BF16);
+            }
+        tmem_st32(ts + 16 * x, w);
+    }
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
 // The sequence of pair number `want` (pairs counted over the sequences in order) by one warp: -1 if there is none.
 __device__ __forceinline__ void find_pair(const rvq_prompt_attn_args& a, int per_pair, int want, int32_t* seq, int32_t* pair) {
     const int lane = threadIdx.x & 31;
@@ -290,12 +351,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             constexpr uint32_t kTypes = kHalfType ? 0u : (1u << 7) | (1u << 10);
             constexpr uint32_t kS = (1u << 4) | kTypes | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
             constexpr uint32_t kO = (1u << 4) | kTypes | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+            // c is |scaling|: a negative one negates Q on its way (so that the largest score stays the largest)
+            const uint32_t types_s = kS | (a.scaling < 0.f ? 1u << 13 : 0u);
             auto scores = [&](int i, int j) {                // S_i = Q_i K_j^T
                 if (lane == 0) {
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k)
                         mma_bf16(tmem + i * kKeys, sw128_desc(smem_addr(S.q[i]) + (k / 4) * kHalf + (k % 4) * 32),
-                                 sw128_desc(smem_addr(S.k[j & 1]) + (k / 4) * kHalf + (k % 4) * 32), kS, k > 0);
+                                 sw128_desc(smem_addr(S.k[j & 1]) + (k / 4) * kHalf + (k % 4) * 32), types_s, k > 0);
                     mma_commit(smem_addr(&S.s_full[i]));
                 }
                 __syncwarp();
@@ -346,7 +409,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const int limit = !valid ? 0 : a.causal ? min(lk, max(0, tok + 1 + lk - lq)) : lk;
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 2 * kKeys + i * HD;
-            const bool negative = a.scaling < 0.f;
             const float c = fabsf(a.scaling) * 1.4426950408889634f;
             float m = -INFINITY, sum = 0.f;                  // m: of the scores times c
             bool ok = true;
@@ -359,27 +421,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 for (int x = 0; x < 4; ++x) tmem_ld32(ts + 32 * x, r[x]);
                 tmem_ld_wait();
                 float (&s)[4][32] = reinterpret_cast<float (&)[4][32]>(r);
-                if (negative) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) s[x][e] = -s[x][e];
-                }
                 const int seen = limit - j * kKeys;          // columns of this tile that the row sees
                 const bool masked = __any_sync(0xffffffffu, seen < kKeys);
-                if (masked) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (32 * x + e >= seen) s[x][e] = -INFINITY;
-                }
-                float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int e = 0; e < 32; e += 2)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) t[x] = fmaxf(fmaxf(t[x], s[x][e]), s[x][e + 1]);
-                const float raw = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                const float raw = masked ? row_max<true>(s, seen) : row_max<false>(s, seen);
                 const float top = raw == -INFINITY ? -INFINITY : raw * c;
                 const bool grow = j == 0 ? top > m : top > m + kGrow;
                 if (j == 0) {
@@ -401,27 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     tmem_st_wait();
                 }
                 const float sub = m == -INFINITY ? 0.f : m;
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int x = 0; x < 4; x += 2) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float p0 = exp2_approx(fmaf(s[x + y][e], c, -sub));
-                            float p1 = exp2_approx(fmaf(s[x + y][e + 1], c, -sub));
-                            if (masked) {                    // c may be 0
-                                if (32 * (x + y) + e >= seen) p0 = 0.f;
-                                if (32 * (x + y) + e + 1 >= seen) p1 = 0.f;
-                            }
-                            part[2 * y] += p0;
-                            part[2 * y + 1] += p1;
-                            w[16 * y + e / 2] = pack2(p0, p1, kHalfType ? RVQ_F16 : RVQ_BF16);
-                        }
-                    tmem_st32(ts + 16 * x, w);
-                }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                sum += masked ? row_exp<true, kHalfType>(s, seen, c, sub, ts) : row_exp<false, kHalfType>(s, seen, c, sub, ts);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -469,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 again &= again - 1;
                 __syncwarp();
                 repair(a, q0 + __shfl_sync(0xffffffffu, tok, l), __shfl_sync(0xffffffffu, h, l), k0, __shfl_sync(0xffffffffu, limit, l),
-                       hidden_end, negative ? -c : c, __shfl_sync(0xffffffffu, m, l), __shfl_sync(0xffffffffu, inv, l));
+                       hidden_end, a.scaling < 0.f ? -c : c, __shfl_sync(0xffffffffu, m, l), __shfl_sync(0xffffffffu, inv, l));
             }
         }
     }

@@ -39,9 +39,10 @@ __device__ int g_attention_timeout;          // sticky: a bounded wait gave up
 // ---------------------------------------------------------------------------
 constexpr int kRows = 128;                   // operand rows of a tile (MMA M)
 constexpr int kKeys = 128;                   // keys of a tile
-constexpr int kThreads = 320;
+constexpr int kSoftmaxWarps = 16;            // 8 a tile
+constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
 constexpr int kHalf = kRows * 128;           // bytes of 64 columns of a tile
-constexpr long long kWaitPolls = 1ll << 22;
+constexpr int kWaitPolls = 1 << 22;
 constexpr float kGrow = 8.f;                 // the maximum may be passed by 2^kGrow
 
 struct Params {
@@ -58,7 +59,10 @@ struct Smem {
     uint8_t q[2][kTileBytes];
     uint8_t k[2][kTileBytes];
     uint8_t v[2][kTileBytes];
-    uint64_t q_full, drain, k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean, s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, drain, v_clean, s_full[2], p_full[2], o_full[2];
+    uint64_t first_full, first_empty;        // K of tile 0
+    uint64_t kv_full[2], kv_empty[2];        // V of tile j and K of tile j + 1, at j & 1
+    float top[2][2][kRows];                  // a row's maximum (at the end: sum) over either half of the columns
     uint32_t tmem;
     int32_t seq, pair;                       // this CTA's sequence (-1: none) and pair of tiles in it
     int32_t dead;                            // a bounded wait gave up
@@ -96,19 +100,32 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         : "memory");
 }
 
-// Bounded wait of a whole warp; once one wait of the CTA has given up, the others end at once.
+// 8 consecutive 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
+// Bounded wait of a thread; once one wait of the CTA has given up, the others end at once.
 template <int HD>
-__device__ __forceinline__ bool wait(Smem<HD>& S, uint64_t& bar, uint32_t parity) {
-    const uint32_t b = smem_addr(&bar);
-    bool done = false;
-    for (long long i = 0; i < kWaitPolls && !done; ++i) {
-        done = mbar_try_wait(b, parity);
-        if (!done && (i & 63) == 63 && *(volatile int32_t*)&S.dead) break;
+__device__ __forceinline__ bool wait1(Smem<HD>& S, uint32_t bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    for (int i = 0; i < kWaitPolls; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63) == 63 && *(volatile int32_t*)&S.dead) return false;
     }
-    if (__all_sync(0xffffffffu, done)) return true;
     atomicExch(&g_attention_timeout, 1);
     *(volatile int32_t*)&S.dead = 1;
     return false;
+}
+
+// The same of a whole warp.
+template <int HD>
+__device__ __forceinline__ bool wait(Smem<HD>& S, uint64_t& bar, uint32_t parity) {
+    const bool ok = wait1(S, smem_addr(&bar), parity);
+    return __all_sync(0xffffffffu, ok);
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -125,49 +142,51 @@ __device__ __forceinline__ void fma2(float& x, float& y, float b, float c) {
         : "f"(b), "f"(c));
 }
 
-// A row's scores of a tile in r (a thread's TMEM lane): its columns from `seen` on are hidden.
+// Half of a row's scores of a tile (64 columns of a thread's TMEM lane): its columns from `seen` on are hidden.
 template <bool kMasked>
-__device__ __forceinline__ float row_max(float (&s)[4][32], int seen) {
+__device__ __forceinline__ float row_max(float (&s)[2][32], int seen) {
     if constexpr (kMasked) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
                 if (32 * x + e >= seen) s[x][e] = -INFINITY;
     }
     float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int e = 0; e < 32; e += 2)
+    for (int e = 0; e < 32; e += 4)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) t[x] = max3(t[x], s[x][e], s[x][e + 1]);
-    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        for (int x = 0; x < 2; ++x) {
+            t[2 * x] = max3(t[2 * x], s[x][e], s[x][e + 1]);
+            t[2 * x + 1] = max3(t[2 * x + 1], s[x][e + 2], s[x][e + 3]);
+        }
+    return fmaxf(max3(t[0], t[1], t[2]), t[3]);
 }
 
 // p = 2^(c s - sub) over the scores in TMEM, in the operand type; returns their sum.
 template <bool kMasked, bool kHalfType>
-__device__ __forceinline__ float row_exp(float (&s)[4][32], int seen, float c, float sub, uint32_t ts) {
+__device__ __forceinline__ float row_exp(float (&s)[2][32], int seen, float c, float sub, uint32_t ts) {
     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < 4; x += 2) {
-        uint32_t w[32];
+    for (int x = 0; x < 2; ++x) {
+        uint4 q[4];
+        uint32_t* w = reinterpret_cast<uint32_t*>(q);
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                float& p0 = s[x + y][e];
-                float& p1 = s[x + y][e + 1];
-                fma2(p0, p1, c, -sub);
-                p0 = exp2_approx(p0);
-                p1 = exp2_approx(p1);
-                if constexpr (kMasked) {                     // c may be 0
-                    if (32 * (x + y) + e >= seen) p0 = 0.f;
-                    if (32 * (x + y) + e + 1 >= seen) p1 = 0.f;
-                }
-                part[2 * y] += p0;
-                part[2 * y + 1] += p1;
-                w[16 * y + e / 2] = pack2(p0, p1, kHalfType ? RVQ_F16 : RVQ_BF16);
+        for (int e = 0; e < 32; e += 2) {
+            float& p0 = s[x][e];
+            float& p1 = s[x][e + 1];
+            fma2(p0, p1, c, -sub);
+            p0 = exp2_approx(p0);
+            p1 = exp2_approx(p1);
+            if constexpr (kMasked) {                         // c may be 0
+                if (32 * x + e >= seen) p0 = 0.f;
+                if (32 * x + e + 1 >= seen) p1 = 0.f;
             }
-        tmem_st32(ts + 16 * x, w);
+            part[2 * x] += p0;
+            part[2 * x + 1] += p1;
+            w[e / 2] = pack2(p0, p1, kHalfType ? RVQ_F16 : RVQ_BF16);
+        }
+        tmem_st16(ts + 16 * x, q);
     }
     return (part[0] + part[1]) + (part[2] + part[3]);
 }
@@ -257,21 +276,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         mbar_init(smem_addr(&S.q_full), 1);
         mbar_init(smem_addr(&S.v_clean), 1);
         mbar_init(smem_addr(&S.drain), 1);
+        mbar_init(smem_addr(&S.first_full), 1);
+        mbar_init(smem_addr(&S.first_empty), 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_addr(&S.k_full[i]), 1);
-            mbar_init(smem_addr(&S.k_empty[i]), 1);
-            mbar_init(smem_addr(&S.v_full[i]), 1);
-            mbar_init(smem_addr(&S.v_empty[i]), 1);
+            mbar_init(smem_addr(&S.kv_full[i]), 1);
+            mbar_init(smem_addr(&S.kv_empty[i]), 1);
             mbar_init(smem_addr(&S.s_full[i]), 1);
-            mbar_init(smem_addr(&S.p_full[i]), 4);
+            mbar_init(smem_addr(&S.p_full[i]), kSoftmaxWarps / 2);
             mbar_init(smem_addr(&S.o_full[i]), 1);
         }
         S.dead = 0;
         mbar_init_fence();
     }
-    if (warp == 9) tmem_alloc(smem_addr(&S.tmem), 512);
+    if (warp == kSoftmaxWarps + 1) tmem_alloc(smem_addr(&S.tmem), 512);
     pdl_wait();
-    if (warp == 8) {
+    if (warp == kSoftmaxWarps) {
         // the last pairs of a causal sequence see the most keys: they start first
         int32_t seq, pair = 0;
         find_pair(a, 2 * T, p.pairs - 1 - (int)(blockIdx.x / a.n_kv), &seq, &pair);
@@ -302,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const int total = max(n[0], n[1]);
         const bool clean = lk % kKeys != 0 && total * kKeys > lk && k0 + lk < a.keys;   // values of others in the last tile
 
-        if (warp == 8) {
+        if (warp == kSoftmaxWarps) {
             if (lane == 0 && total > 0) {
                 mbar_expect_tx(smem_addr(&S.q_full), (n[1] > 0 ? 2 : 1) * HD / 64 * (uint32_t)(T * p.rep * 128));
                 for (int i = 0; i < (n[1] > 0 ? 2 : 1); ++i)
@@ -310,25 +329,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         tma_load_3d(smem_addr(S.q[i] + h * kHalf), &p.q, 64 * h, kv * p.rep, (int)q0 + tok0 + i * T,
                                     smem_addr(&S.q_full));
             }
-            int loaded_k = 0, loaded_v = 0;
-            for (int j = 0; j < total; ++j) {
-                const int st = j & 1, row = (int)k0 + j * kKeys;
-                if (j >= 2 && !wait(S, S.k_empty[st], (j / 2 - 1) & 1)) break;
-                if (lane == 0) {
-                    mbar_expect_tx(smem_addr(&S.k_full[st]), Smem<HD>::kTileBytes);
-                    for (int h = 0; h < HD / 64; ++h)
-                        tma_load_3d(smem_addr(S.k[st] + h * kHalf), &p.k, 64 * h, kv, row, smem_addr(&S.k_full[st]));
-                }
-                loaded_k = j + 1;
-                if (j >= 2 && !wait(S, S.v_empty[st], (j / 2 - 1) & 1)) break;
-                if (lane == 0) {
-                    mbar_expect_tx(smem_addr(&S.v_full[st]), Smem<HD>::kTileBytes);
-                    for (int h = 0; h < HD / 64; ++h)
-                        tma_load_3d(smem_addr(S.v[st] + h * kHalf), &p.v, 64 * h, kv, row, smem_addr(&S.v_full[st]));
-                }
-                loaded_v = j + 1;
+            auto load = [&](const CUtensorMap& map, uint8_t* dst, int j, uint64_t& bar) {
+                for (int h = 0; h < HD / 64; ++h)
+                    tma_load_3d(smem_addr(dst + h * kHalf), &map, 64 * h, kv, (int)k0 + j * kKeys, smem_addr(&bar));
+            };
+            if (lane == 0 && total > 0) {
+                mbar_expect_tx(smem_addr(&S.first_full), Smem<HD>::kTileBytes);
+                load(p.k, S.k[0], 0, S.first_full);
             }
-            if (clean && loaded_v == total && wait(S, S.v_full[(total - 1) & 1], ((total - 1) / 2) & 1)) {
+            int loaded = 0;
+            for (int j = 0; j < total; ++j) {
+                const int st = j & 1;
+                if (j >= 2 && !wait(S, S.kv_empty[st], (j / 2 - 1) & 1)) break;
+                if (j == 1 && !wait(S, S.first_empty, 0)) break;            // K of tile 2 replaces that of tile 0
+                if (lane == 0) {
+                    mbar_expect_tx(smem_addr(&S.kv_full[st]), (j + 1 < total ? 2 : 1) * Smem<HD>::kTileBytes);
+                    load(p.v, S.v[st], j, S.kv_full[st]);
+                    if (j + 1 < total) load(p.k, S.k[st ^ 1], j + 1, S.kv_full[st]);
+                }
+                loaded = j + 1;
+            }
+            if (clean && loaded == total && wait(S, S.kv_full[(total - 1) & 1], ((total - 1) / 2) & 1)) {
                 uint8_t* v = S.v[(total - 1) & 1];
                 const int r0 = lk - (total - 1) * kKeys;     // rows r0 .. 127 belong to others (a swizzled row stays a row)
                 for (int h = 0; h < HD / 64; ++h)
@@ -338,92 +359,95 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&S.v_clean));
             }
-            if (*(volatile int32_t*)&S.dead) {               // copies in flight end before this CTA's shared memory is given up
-                for (int i = 0; i < 2; ++i) {
-                    if (loaded_k > i) mbar_wait(smem_addr(&S.k_full[(loaded_k - 1 - i) & 1]), ((loaded_k - 1 - i) / 2) & 1,
-                                                kWaitPolls, &g_attention_timeout);
-                    if (loaded_v > i) mbar_wait(smem_addr(&S.v_full[(loaded_v - 1 - i) & 1]), ((loaded_v - 1 - i) / 2) & 1,
-                                                kWaitPolls, &g_attention_timeout);
-                }
-                if (total > 0) mbar_wait(smem_addr(&S.q_full), 0, kWaitPolls, &g_attention_timeout);
+            if (*(volatile int32_t*)&S.dead && total > 0) {  // copies in flight end before this CTA's shared memory is given up
+                for (int j = max(0, loaded - 2); j < loaded; ++j)
+                    mbar_wait(smem_addr(&S.kv_full[j & 1]), (j / 2) & 1, kWaitPolls, &g_attention_timeout);
+                mbar_wait(smem_addr(&S.first_full), 0, kWaitPolls, &g_attention_timeout);
+                mbar_wait(smem_addr(&S.q_full), 0, kWaitPolls, &g_attention_timeout);
             }
-        } else if (warp == 9) {
+        } else if (warp == kSoftmaxWarps + 1) {
+            // One thread from here to the end: what it does between two products, the tensor cores wait for.
             constexpr uint32_t kTypes = kHalfType ? 0u : (1u << 7) | (1u << 10);
             constexpr uint32_t kS = (1u << 4) | kTypes | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
             constexpr uint32_t kO = (1u << 4) | kTypes | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-            // c is |scaling|: a negative one negates Q on its way (so that the largest score stays the largest)
-            const uint32_t types_s = kS | (a.scaling < 0.f ? 1u << 13 : 0u);
-            auto scores = [&](int i, int j) {                // S_i = Q_i K_j^T
-                if (lane == 0) {
+            if (lane == 0 && total > 0) {
+                // c is |scaling|: a negative one negates Q on its way (so that the largest score stays the largest)
+                const uint32_t types_s = kS | (a.scaling < 0.f ? 1u << 13 : 0u);
+                const uint64_t dq = sw128_desc(smem_addr(S.q[0])), dk = sw128_desc(smem_addr(S.k[0]));
+                const uint64_t dv = sw128_desc_mn(smem_addr(S.v[0]), kHalf);
+                constexpr uint32_t kTile = Smem<HD>::kTileBytes >> 4;      // descriptors count 16 bytes
+                auto scores = [&](int i, int j) {            // S_i = Q_i K_j^T
+                    const uint64_t q = dq + i * kTile, k = dk + (j & 1) * kTile;
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k)
-                        mma_bf16(tmem + i * kKeys, sw128_desc(smem_addr(S.q[i]) + (k / 4) * kHalf + (k % 4) * 32),
-                                 sw128_desc(smem_addr(S.k[j & 1]) + (k / 4) * kHalf + (k % 4) * 32), types_s, k > 0);
+                    for (int x = 0; x < HD / 16; ++x)
+                        mma_bf16(tmem + i * kKeys, q + (x / 4) * (kHalf >> 4) + (x % 4) * 2, k + (x / 4) * (kHalf >> 4) + (x % 4) * 2,
+                                 types_s, x > 0);
                     mma_commit(smem_addr(&S.s_full[i]));
+                };
+                bool ok = wait1(S, smem_addr(&S.q_full), 0) && wait1(S, smem_addr(&S.first_full), 0);
+                if (ok) {
+                    for (int i = 0; i < 2; ++i)
+                        if (n[i] > 0) scores(i, 0);
+                    mma_commit(smem_addr(&S.first_empty));
                 }
-                __syncwarp();
-            };
-            bool ok = total == 0 || wait(S, S.q_full, 0);
-            if (ok && total > 0) ok = wait(S, S.k_full[0], 0);
-            if (ok && total > 0) {
-                for (int i = 0; i < 2; ++i)
-                    if (n[i] > 0) scores(i, 0);
-                if (lane == 0) mma_commit(smem_addr(&S.k_empty[0]));
-                __syncwarp();
-            }
-            for (int j = 0; ok && j < total; ++j) {
-                ok = wait(S, S.v_full[j & 1], (j / 2) & 1);
-                if (ok && clean && j == total - 1) ok = wait(S, S.v_clean, 0);
-                if (ok && j + 1 < total) ok = wait(S, S.k_full[(j + 1) & 1], ((j + 1) / 2) & 1);
-                for (int i = 0; ok && i < 2; ++i) {
-                    if (j >= n[i]) continue;
-                    ok = wait(S, S.p_full[i], j & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (lane == 0) {
+                for (int j = 0; ok && j < total; ++j) {
+                    ok = wait1(S, smem_addr(&S.kv_full[j & 1]), (j / 2) & 1);
+                    if (ok && clean && j == total - 1) ok = wait1(S, smem_addr(&S.v_clean), 0);
+                    const uint64_t v = dv + (j & 1) * kTile;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (!ok || j >= n[i]) continue;
+                        ok = wait1(S, smem_addr(&S.p_full[i]), j & 1);
+                        if (!ok) continue;
+                        tc_fence_after();
 #pragma unroll
                         for (int k = 0; k < kKeys / 16; ++k)
-                            mma_bf16_ts(tmem + 2 * kKeys + i * HD, tmem + i * kKeys + 8 * k,
-                                        sw128_desc_mn(smem_addr(S.v[j & 1]) + k * 2048, kHalf), kO, j > 0 || k > 0);
-                        if (j + 1 == n[i]) mma_commit(smem_addr(&S.o_full[i]));
+                            mma_bf16_ts(tmem + 2 * kKeys + i * HD, tmem + i * kKeys + 8 * k, v + k * (2048 >> 4), kO, j > 0 || k > 0);
+                        if (j + 1 < n[i]) scores(i, j + 1);
+                        else mma_commit(smem_addr(&S.o_full[i]));
                     }
-                    __syncwarp();
-                    if (j + 1 < n[i]) scores(i, j + 1);
+                    if (ok) mma_commit(smem_addr(&S.kv_empty[j & 1]));
                 }
-                if (ok && lane == 0) {
-                    mma_commit(smem_addr(&S.v_empty[j & 1]));
-                    if (j + 1 < total) mma_commit(smem_addr(&S.k_empty[(j + 1) & 1]));
+                if (!ok) {                                   // products in flight end before TMEM is given up
+                    mma_commit(smem_addr(&S.drain));
+                    mbar_wait(smem_addr(&S.drain), 0, kWaitPolls, &g_attention_timeout);
                 }
-                __syncwarp();
             }
-            if (!ok) {                                       // products in flight end before TMEM is given up
-                if (lane == 0) mma_commit(smem_addr(&S.drain));
-                __syncwarp();
-                mbar_wait(smem_addr(&S.drain), 0, kWaitPolls, &g_attention_timeout);
-            }
+            __syncwarp();
         } else {
-            const int i = warp >> 2, row = tid & 127;
+            // two threads a row, 64 columns of S and half of O's each
+            const int i = warp >> 3, half = warp >> 2 & 1, row = tid & 127;
             const int in = row / p.rep, h = kv * p.rep + row % p.rep;
             const int tok = tok0 + i * T + in;               // in the sequence
             const bool valid = in < T && tok < lq;
             const int limit = !valid ? 0 : a.causal ? min(lk, max(0, tok + 1 + lk - lq)) : lk;
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 2 * kKeys + i * HD;
+            const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 2 * kKeys + i * HD + half * (HD / 2);
+            const int pair_bar = 1 + i * 4 + (warp & 3);     // named barrier of the two warps of these rows
             const float c = fabsf(a.scaling) * 1.4426950408889634f;
             float m = -INFINITY, sum = 0.f;                  // m: of the scores times c
             bool ok = true;
             for (int j = 0; j < n[i]; ++j) {
-                ok = wait(S, S.s_full[i], j & 1);
-                if (!ok) break;
+                ok = ok && wait(S, S.s_full[i], j & 1);
+                if (!ok) {                                   // the partner may still come to its barriers
+                    named_sync(pair_bar, 64);
+                    continue;
+                }
                 tc_fence_after();
-                uint32_t r[4][32];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) tmem_ld32(ts + 32 * x, r[x]);
+                uint32_t r[2][32];
+                tmem_ld32(ts + half * 64, r[0]);
+                tmem_ld32(ts + half * 64 + 32, r[1]);
                 tmem_ld_wait();
-                float (&s)[4][32] = reinterpret_cast<float (&)[4][32]>(r);
-                const int seen = limit - j * kKeys;          // columns of this tile that the row sees
-                const bool masked = __any_sync(0xffffffffu, seen < kKeys);
-                const float raw = masked ? row_max<true>(s, seen) : row_max<false>(s, seen);
+                float (&s)[2][32] = reinterpret_cast<float (&)[2][32]>(r);
+                const int seen = limit - j * kKeys - half * 64;             // of this half's columns the row sees these
+                const bool masked = __any_sync(0xffffffffu, seen < kKeys / 2);
+                float raw = masked ? row_max<true>(s, seen) : row_max<false>(s, seen);
+                // both halves are in registers when the barrier opens: P may overwrite either
+                S.top[i][half][row] = raw;
+                tc_fence_before();
+                named_sync(pair_bar, 64);
+                tc_fence_after();
+                raw = fmaxf(raw, S.top[i][half ^ 1][row]);
                 const float top = raw == -INFINITY ? -INFINITY : raw * c;
                 const bool grow = j == 0 ? top > m : top > m + kGrow;
                 if (j == 0) {
@@ -434,18 +458,18 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     if (grow) m = top;
                     sum *= f;
 #pragma unroll 1
-                    for (int x = 0; x < HD / 32; ++x) {
-                        uint32_t o[32];
-                        tmem_ld32(to + 32 * x, o);
+                    for (int x = 0; x < HD / 16; ++x) {      // few columns at a time: the scores stay in registers
+                        uint32_t o[8];
+                        tmem_ld8(to + 8 * x, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st32(to + 32 * x, o);
+                        for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st8(to + 8 * x, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
                     }
                     tmem_st_wait();
                 }
                 const float sub = m == -INFINITY ? 0.f : m;
-                sum += masked ? row_exp<true, kHalfType>(s, seen, c, sub, ts) : row_exp<false, kHalfType>(s, seen, c, sub, ts);
+                sum += masked ? row_exp<true, kHalfType>(s, seen, c, sub, ts + half * 32) : row_exp<false, kHalfType>(s, seen, c, sub, ts + half * 32);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -453,12 +477,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
             if (ok && n[i] > 0) ok = wait(S, S.o_full[i], 0);
             tc_fence_after();
+            named_sync(pair_bar, 64);                        // the partner has read this half's last maximum
+            S.top[i][half][row] = sum;
+            named_sync(pair_bar, 64);
+            sum = S.top[i][0][row] + S.top[i][1][row];
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const int64_t at = (q0 + tok) * a.out_stride[0] + h * a.out_stride[1];
-            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at;
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at + half * (HD / 2);
             bool bad = false;
 #pragma unroll 1
-            for (int x = 0; x < HD / 32; ++x) {
+            for (int x = 0; x < HD / 64; ++x) {
                 uint32_t o[32];
                 if (ok && n[i] > 0) {
                     tmem_ld32(to + 32 * x, o);
@@ -479,11 +507,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 if (valid) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (32 * x + 8 * e < a.head_dim)
+                        if (half * (HD / 2) + 32 * x + 8 * e < a.head_dim)
                             *reinterpret_cast<uint4*>(out + 32 * x + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
                 }
             }
-            if (valid && a.lse != nullptr)
+            if (valid && half == 0 && a.lse != nullptr)
                 a.lse[(int64_t)h * a.tokens + q0 + tok] = limit == 0 || sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
             // values between this row's last key and the end of its last tile may have leaked in
             const int hidden_end = min(lk, n[i] * kKeys);
@@ -500,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 9) tmem_dealloc(tmem, 512);
+    if (warp == kSoftmaxWarps + 1) tmem_dealloc(tmem, 512);
 }
 
 int check(const rvq_prompt_attn_args* a) {

@@ -51,6 +51,9 @@ struct Params {
     int32_t rep;
     int32_t tile_tokens;                     // 128 / rep
     int32_t pairs;                           // upper bound of the pairs of tiles of all sequences
+    int32_t splits;                          // parts of the keys, each with CTAs of its own
+    float* part_o;                           // splits > 1: [splits][tokens][n_heads][head_dim], not yet divided by the sum
+    float2* part_ml;                         // [splits][tokens][n_heads]: maximum (times c) and sum
 };
 
 template <int HD>
@@ -224,9 +227,9 @@ __device__ __forceinline__ void find_pair(const rvq_prompt_attn_args& a, int per
 
 // Output row of a query whose hidden values (keys [n, hidden_end) of the last tiles) may have leaked in, by a whole warp:
 // where one of them is not finite and no seen value in the last tile is NaN, the columns concerned are summed again over
-// the n keys that the query sees, one by one.
-__device__ __noinline__ void repair(const rvq_prompt_attn_args& a, int64_t tok, int h, int64_t k0, int64_t n,
-                                    int64_t hidden_end, float c, float m, float inv) {
+// the keys [begin, n) that the query sees, one by one; into out (times inv), or into part.
+__device__ __noinline__ void repair(const rvq_prompt_attn_args& a, int64_t tok, int h, int64_t k0, int64_t begin, int64_t n,
+                                    int64_t hidden_end, float c, float m, float inv, float* part) {
     const int lane = threadIdx.x & 31, g = h / (a.n_heads / a.n_kv), hd = a.head_dim;
     const int64_t vr = g * a.v_stride[1], kr = g * a.k_stride[1];
     bool leak[4];
@@ -239,7 +242,7 @@ __device__ __noinline__ void repair(const rvq_prompt_attn_args& a, int64_t tok, 
             const float v = load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + d, a.kind);
             leak[j] |= !(fabsf(v) <= 3.4e38f);
         }
-        for (int64_t i = max((int64_t)0, hidden_end - kKeys); leak[j] && i < n; ++i) {
+        for (int64_t i = max(begin, hidden_end - kKeys); leak[j] && i < n; ++i) {
             const float v = load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + d, a.kind);
             leak[j] = v == v;
         }
@@ -249,7 +252,7 @@ __device__ __noinline__ void repair(const rvq_prompt_attn_args& a, int64_t tok, 
     float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < 4; ++j)
         q[j] = lane + 32 * j < hd ? load_as_f32(a.q, tok * a.q_stride[0] + h * a.q_stride[1] + lane + 32 * j, a.kind) : 0.f;
-    for (int64_t i = 0; i < n; ++i) {
+    for (int64_t i = begin; i < n; ++i) {
         float x = 0.f;
         for (int j = 0; j < 4; ++j)
             if (lane + 32 * j < hd) x = fmaf(q[j], load_as_f32(a.k, (k0 + i) * a.k_stride[0] + kr + lane + 32 * j, a.kind), x);
@@ -259,7 +262,9 @@ __device__ __noinline__ void repair(const rvq_prompt_attn_args& a, int64_t tok, 
             if (leak[j]) acc[j] += p * load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + lane + 32 * j, a.kind);
     }
     for (int j = 0; j < 4; ++j)
-        if (leak[j])
+        if (leak[j] && part != nullptr)
+            part[lane + 32 * j] = acc[j];
+        else if (leak[j])
             store_from_f32(a.out, tok * a.out_stride[0] + h * a.out_stride[1] + lane + 32 * j, a.kind, acc[j] * inv);
 }
 
@@ -269,7 +274,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     Smem<HD>& S = *reinterpret_cast<Smem<HD>*>(smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023));
     const rvq_prompt_attn_args& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kv = blockIdx.x % a.n_kv;
+    const int split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
+    const int kv = unit % a.n_kv;
     const int T = p.tile_tokens;
     pdl_launch_dependents();
     if (tid == 0) {
@@ -293,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     if (warp == kSoftmaxWarps) {
         // the last pairs of a causal sequence see the most keys: they start first
         int32_t seq, pair = 0;
-        find_pair(a, 2 * T, p.pairs - 1 - (int)(blockIdx.x / a.n_kv), &seq, &pair);
+        find_pair(a, 2 * T, p.pairs - 1 - unit / a.n_kv, &seq, &pair);
         if (lane == 0) S.seq = seq, S.pair = pair;
     }
     tc_fence_before();
@@ -318,8 +324,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const int see = last < tok0 + i * T ? 0 : a.causal ? min(lk, max(0, last + 1 + lk - lq)) : lk;
             n[i] = (see + kKeys - 1) / kKeys;
         }
+        // this CTA's part of them: tiles j0 .. of the keys (from here on counted from j0)
+        const int j0 = (int)((int64_t)max(n[0], n[1]) * split / p.splits);
+        const int j1 = (int)((int64_t)max(n[0], n[1]) * (split + 1) / p.splits);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) n[i] = max(0, min(n[i], j1) - j0);
         const int total = max(n[0], n[1]);
-        const bool clean = lk % kKeys != 0 && total * kKeys > lk && k0 + lk < a.keys;   // values of others in the last tile
+        // values of others in the last tile
+        const bool clean = lk % kKeys != 0 && (j0 + total) * kKeys > lk && total > 0 && k0 + lk < a.keys;
 
         if (warp == kSoftmaxWarps) {
             if (lane == 0 && total > 0) {
@@ -331,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
             auto load = [&](const CUtensorMap& map, uint8_t* dst, int j, uint64_t& bar) {
                 for (int h = 0; h < HD / 64; ++h)
-                    tma_load_3d(smem_addr(dst + h * kHalf), &map, 64 * h, kv, (int)k0 + j * kKeys, smem_addr(&bar));
+                    tma_load_3d(smem_addr(dst + h * kHalf), &map, 64 * h, kv, (int)k0 + (j0 + j) * kKeys, smem_addr(&bar));
             };
             if (lane == 0 && total > 0) {
                 mbar_expect_tx(smem_addr(&S.first_full), Smem<HD>::kTileBytes);
@@ -351,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
             if (clean && loaded == total && wait(S, S.kv_full[(total - 1) & 1], ((total - 1) / 2) & 1)) {
                 uint8_t* v = S.v[(total - 1) & 1];
-                const int r0 = lk - (total - 1) * kKeys;     // rows r0 .. 127 belong to others (a swizzled row stays a row)
+                const int r0 = lk - (j0 + total - 1) * kKeys;     // rows r0 .. 127 belong to others (a swizzled row stays a row)
                 for (int h = 0; h < HD / 64; ++h)
                     for (int i = r0 * 8 + lane; i < kRows * 8; i += 32)
                         reinterpret_cast<uint4*>(v + h * kHalf)[i] = make_uint4(0, 0, 0, 0);
@@ -439,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 tmem_ld32(ts + half * 64 + 32, r[1]);
                 tmem_ld_wait();
                 float (&s)[2][32] = reinterpret_cast<float (&)[2][32]>(r);
-                const int seen = limit - j * kKeys - half * 64;             // of this half's columns the row sees these
+                const int seen = limit - (j0 + j) * kKeys - half * 64;             // of this half's columns the row sees these
                 const bool masked = __any_sync(0xffffffffu, seen < kKeys / 2);
                 float raw = masked ? row_max<true>(s, seen) : row_max<false>(s, seen);
                 // both halves are in registers when the barrier opens: P may overwrite either
@@ -482,46 +494,60 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             named_sync(pair_bar, 64);
             sum = S.top[i][0][row] + S.top[i][1][row];
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const bool whole = p.splits == 1, none = limit == 0 || (whole && inv == 0.f);
             const int64_t at = (q0 + tok) * a.out_stride[0] + h * a.out_stride[1];
             uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at + half * (HD / 2);
+            const int64_t slot = ((int64_t)split * a.tokens + q0 + tok) * a.n_heads + h;
+            float* part = whole ? nullptr : p.part_o + slot * a.head_dim;
             bool bad = false;
 #pragma unroll 1
-            for (int x = 0; x < HD / 64; ++x) {
-                uint32_t o[32];
+            for (int x = 0; x < HD / 32; ++x) {              // 16 columns
+                uint32_t o[16];
                 if (ok && n[i] > 0) {
-                    tmem_ld32(to + 32 * x, o);
+                    tmem_ld8(to + 16 * x, *reinterpret_cast<uint32_t (*)[8]>(o));
+                    tmem_ld8(to + 16 * x + 8, *reinterpret_cast<uint32_t (*)[8]>(o + 8));
                     tmem_ld_wait();
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                    for (int e = 0; e < 16; ++e) o[e] = 0;
                 }
-                uint32_t w[16];
+                float v[16];
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float v0 = __uint_as_float(o[e]), v1 = __uint_as_float(o[e + 1]);
-                    bad |= !(fabsf(v0) + fabsf(v1) <= 3.4e38f);
-                    v0 = limit == 0 || inv == 0.f ? 0.f : v0 * inv;
-                    v1 = limit == 0 || inv == 0.f ? 0.f : v1 * inv;
-                    w[e / 2] = pack2(v0, v1, kHalfType ? RVQ_F16 : RVQ_BF16);
+                for (int e = 0; e < 16; ++e) {
+                    v[e] = __uint_as_float(o[e]);
+                    bad |= !(fabsf(v[e]) <= 3.4e38f);
+                    v[e] = none ? 0.f : whole ? v[e] * inv : v[e];
                 }
-                if (valid) {
+                const int d = half * (HD / 2) + 16 * x;
+                if (valid && whole) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (half * (HD / 2) + 32 * x + 8 * e < a.head_dim)
-                            *reinterpret_cast<uint4*>(out + 32 * x + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                    for (int e = 0; e < 16; e += 8)
+                        if (d + e < a.head_dim) {
+                            constexpr int kOut = kHalfType ? RVQ_F16 : RVQ_BF16;
+                            *reinterpret_cast<uint4*>(out + 16 * x + e) = make_uint4(pack2(v[e], v[e + 1], kOut), pack2(v[e + 2], v[e + 3], kOut),
+                                                                                    pack2(v[e + 4], v[e + 5], kOut), pack2(v[e + 6], v[e + 7], kOut));
+                        }
+                } else if (valid) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        if (d + e < a.head_dim) *reinterpret_cast<float4*>(part + d + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                 }
             }
-            if (valid && half == 0 && a.lse != nullptr)
-                a.lse[(int64_t)h * a.tokens + q0 + tok] = limit == 0 || sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+            if (valid && half == 0 && whole && a.lse != nullptr)
+                a.lse[(int64_t)h * a.tokens + q0 + tok] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+            if (valid && half == 0 && !whole) p.part_ml[slot] = make_float2(m, limit == 0 ? 0.f : sum);
             // values between this row's last key and the end of its last tile may have leaked in
-            const int hidden_end = min(lk, n[i] * kKeys);
-            uint32_t again = __ballot_sync(0xffffffffu, ok && valid && bad && limit > 0 && limit < hidden_end && fabsf(sum) <= 3.4e38f);
+            const int begin = j0 * kKeys, hidden_end = min(lk, (j0 + n[i]) * kKeys), seen_end = min(limit, hidden_end);
+            uint32_t again = __ballot_sync(0xffffffffu, ok && valid && bad && seen_end > begin && seen_end < hidden_end && fabsf(sum) <= 3.4e38f);
             while (again) {
                 const int l = __ffs(again) - 1;
                 again &= again - 1;
                 __syncwarp();
-                repair(a, q0 + __shfl_sync(0xffffffffu, tok, l), __shfl_sync(0xffffffffu, h, l), k0, __shfl_sync(0xffffffffu, limit, l),
-                       hidden_end, a.scaling < 0.f ? -c : c, __shfl_sync(0xffffffffu, m, l), __shfl_sync(0xffffffffu, inv, l));
+                const int64_t row = q0 + __shfl_sync(0xffffffffu, tok, l);
+                const int head = __shfl_sync(0xffffffffu, h, l);
+                repair(a, row, head, k0, begin, __shfl_sync(0xffffffffu, seen_end, l), hidden_end, a.scaling < 0.f ? -c : c,
+                       __shfl_sync(0xffffffffu, m, l), __shfl_sync(0xffffffffu, inv, l),
+                       whole ? nullptr : p.part_o + (((int64_t)split * a.tokens + row) * a.n_heads + head) * a.head_dim);
             }
         }
     }
@@ -529,6 +555,46 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     __syncthreads();
     tc_fence_after();
     if (warp == kSoftmaxWarps + 1) tmem_dealloc(tmem, 512);
+}
+
+// The parts of every row joined, in order: a warp a (token, head).  Rows in no sequence have none.
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p) {
+    const rvq_prompt_attn_args& a = p.a;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (unit >= a.tokens * a.n_heads) return;
+    const int64_t tok = unit / a.n_heads;
+    const int h = (int)(unit - tok * a.n_heads);
+    if (a.cu_q != nullptr) {
+        int lo = 0, hi = a.n_seq;                            // the last sequence that starts at or before tok
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (__ldg(a.cu_q + mid) <= tok) lo = mid;
+            else hi = mid;
+        }
+        if (tok < __ldg(a.cu_q + lo) || tok >= __ldg(a.cu_q + lo + 1)) return;
+    }
+    const int64_t step = a.tokens * a.n_heads;
+    float m = -INFINITY, total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[s * step + unit].x);
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 ml = p.part_ml[s * step + unit];
+        if (ml.y == 0.f) continue;                           // nothing seen in this part
+        const float f = ml.x == m ? 1.f : exp2_approx(ml.x - m);
+        total = fmaf(f, ml.y, total);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (lane + 32 * j < a.head_dim) o[j] = fmaf(f, p.part_o[(s * step + unit) * a.head_dim + lane + 32 * j], o[j]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (lane + 32 * j < a.head_dim)
+            store_from_f32(a.out, tok * a.out_stride[0] + h * a.out_stride[1] + lane + 32 * j, a.kind, inv == 0.f ? 0.f : o[j] * inv);
+    if (lane == 0 && a.lse != nullptr)
+        a.lse[(int64_t)h * a.tokens + tok] = total == 0.f ? -INFINITY : (m + log2f(total)) * 0.6931471805599453f;
 }
 
 int check(const rvq_prompt_attn_args* a) {
@@ -579,15 +645,48 @@ bool encode(CUtensorMap* map, const void* ptr, const rvq_prompt_attn_args& a, in
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int status(cudaError_t e) {
+    if (e != cudaSuccess) last_cuda_error_slot() = (int)e;
+    return e == cudaSuccess ? RVQ_OK : RVQ_ERR_CUDA;
+}
+
 template <int HD, bool kHalfType>
 int run(const Params& p, cudaStream_t s) {
     auto* kernel = prompt_kernel<HD, kHalfType>;
     const int smem = (int)sizeof(Smem<HD>) + 1024;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
-        e = launch_pdl(kernel, dim3((unsigned)p.pairs * (unsigned)p.a.n_kv), dim3(kThreads), (size_t)smem, s, p);
-    if (e != cudaSuccess) last_cuda_error_slot() = (int)e;
-    return e == cudaSuccess ? RVQ_OK : RVQ_ERR_CUDA;
+        e = launch_pdl(kernel, dim3((unsigned)(p.pairs * p.a.n_kv * p.splits)), dim3(kThreads), (size_t)smem, s, p);
+    if (e == cudaSuccess && p.splits > 1)
+        e = launch_pdl(join_kernel, dim3((unsigned)((p.a.tokens * p.a.n_heads + 3) / 4)), dim3(128), 0, s, p);
+    return status(e);
+}
+
+// Sizes of the launch: the pairs of tiles (each sequence has at most one that is not full) and the parts of the keys.  With
+// fewer CTAs than half the SMs and keys enough, the keys are split so that every SM has a CTA, into parts of at
+// least 4 tiles (the mean sequence's) each.
+int plan(const rvq_prompt_attn_args& a, Params* p) {
+    p->rep = a.n_heads / a.n_kv;
+    p->tile_tokens = kRows / p->rep;
+    const int64_t per = 2 * p->tile_tokens;
+    const int64_t pairs = a.n_seq == 1 ? (a.tokens + per - 1) / per : a.tokens / per + a.n_seq;
+    if (pairs * a.n_kv >= (1ll << 31)) return RVQ_ERR_TOO_LARGE;
+    p->pairs = (int32_t)pairs;
+    p->splits = 1;
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return status(e);
+    const int64_t units = pairs * a.n_kv, tiles = (a.keys / a.n_seq + kKeys - 1) / kKeys;
+    if (units * 2 <= sms && tiles >= 8) {
+        const int64_t most = sms / units, parts = tiles / 4;
+        p->splits = (int32_t)(most < parts ? most : parts);
+    }
+    return RVQ_OK;
+}
+
+size_t part_bytes(const rvq_prompt_attn_args& a, const Params& p) {
+    return p.splits == 1 ? 0 : (size_t)p.splits * a.tokens * a.n_heads * (a.head_dim + 2) * 4;
 }
 
 }  // namespace prompt
@@ -597,7 +696,9 @@ using namespace rvq;
 using namespace rvq::prompt;
 
 extern "C" size_t rvq_prompt_attention_workspace_size(const rvq_prompt_attn_args* a) {
-    return 0;
+    Params p;
+    if (check(a) != RVQ_OK || a->tokens == 0 || plan(*a, &p) != RVQ_OK) return 0;
+    return part_bytes(*a, p);
 }
 
 extern "C" int rvq_prompt_attention(const rvq_prompt_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -608,13 +709,13 @@ extern "C" int rvq_prompt_attention(const rvq_prompt_attn_args* a, void* workspa
     Params p;
     memset(&p, 0, sizeof(p));
     p.a = *a;
-    p.rep = a->n_heads / a->n_kv;
-    p.tile_tokens = kRows / p.rep;
-    // each sequence has at most one pair of tiles that is not full
-    const int64_t pairs = a->n_seq == 1 ? (a->tokens + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens)
-                                        : a->tokens / (2 * p.tile_tokens) + a->n_seq;
-    if (pairs * a->n_kv >= (1ll << 31)) return RVQ_ERR_TOO_LARGE;
-    p.pairs = (int32_t)pairs;
+    rc = plan(*a, &p);
+    if (rc != RVQ_OK) return rc;
+    if (part_bytes(*a, p) > 0) {
+        if (workspace == nullptr || workspace_bytes < part_bytes(*a, p) || ((uintptr_t)workspace & 15)) return RVQ_ERR_INVALID;
+        p.part_o = reinterpret_cast<float*>(workspace);
+        p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)p.splits * a->tokens * a->n_heads * a->head_dim);
+    }
     // without keys nothing is loaded: any valid map will do
     const bool none = a->keys == 0;
     if (!encode(&p.q, a->q, *a, a->tokens, a->n_heads, a->q_stride, p.rep, p.tile_tokens) ||

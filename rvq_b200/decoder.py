@@ -106,12 +106,25 @@ class Qwen3Decoder:
     one cooperative launch, rvq_b200/persist.py, bit-identical to "native") or
     "torch" (the PyTorch ops of the prompt path).  ``slot_decode_ctas``: CTA
     budget of the slot mode's side-stream layer decode (None: half the SMs,
-    the budget at which it overlaps the main stream best; 0: every SM)."""
+    the budget at which it overlaps the main stream best; 0: every SM).
+    ``prompt_attention``: "engine" (the engine's ops: score matrices of the
+    whole prompt, bit-identical logits) or "fused" (``PromptAttentionOp``:
+    one pass, scores and softmax in fp32, memory linear in the prompt).
+    ``kv_cache``: "bf16", or "int4": keys and values held in 4 bits
+    (rvq_b200/attention.py ``Cache4``; native step, head_dim 64 or 128),
+    scores and softmax of a step in fp32.  ``kv_budget`` (int4): rows that stay
+    in the cache: after every ``kv_slack`` steps whose live rows exceed it, the
+    last ``kv_recent`` rows (None: half the budget) and those with the largest
+    attention weight summed over the steps since the prompt are kept, per layer and kv head.
+    Positions then run on past the rows: ``max_positions`` (None: max_len)
+    sizes the rotary tables, ``max_len`` the cache."""
 
     def __init__(self, config, artifact, device, mode: str = "fused", max_len: int = 512,
                  runtime_dtype: torch.dtype = torch.bfloat16, causal: bool = False,
                  step_impl: str = "native", tp_group=None, artifact_is_shard: bool = False,
-                 tp_reduce: str = "push", slot_decode_ctas: Optional[int] = None):
+                 tp_reduce: str = "push", slot_decode_ctas: Optional[int] = None, prompt_attention: str = "engine",
+                 kv_cache: str = "bf16", kv_budget: Optional[int] = None, kv_recent: Optional[int] = None,
+                 kv_slack: int = 64, max_positions: Optional[int] = None):
         if mode not in MODES:
             raise ValueError(f"mode must be one of {MODES}")
         if step_impl not in ("native", "torch", "persistent"):
@@ -123,6 +136,33 @@ class Qwen3Decoder:
             raise NotImplementedError("fused_exact runs on the native decode step")
         if step_impl == "persistent" and (mode != "fused" or tp_group is not None):
             raise NotImplementedError("the persistent decode step runs fused mode on one GPU")
+        if prompt_attention not in ("engine", "fused"):
+            raise ValueError("prompt_attention is 'engine' or 'fused'")
+        if kv_cache not in ("bf16", "int4"):
+            raise ValueError("kv_cache is 'bf16' or 'int4'")
+        if kv_cache == "int4" and step_impl != "native":
+            raise NotImplementedError("the int4 cache runs on the native decode step")
+        if kv_cache == "int4" and config.head_dim not in (64, 128):
+            raise NotImplementedError("the int4 cache holds heads of 64 or 128")
+        if prompt_attention == "fused" and (config.head_dim % 8 or config.head_dim > 128):
+            raise NotImplementedError("the fused prompt attention takes head_dim a multiple of 8, at most 128")
+        if prompt_attention == "fused" and runtime_dtype not in (torch.bfloat16, torch.float16):
+            raise NotImplementedError("the fused prompt attention computes in bf16 or fp16")
+        if kv_budget is None:
+            if kv_recent is not None:
+                raise ValueError("kv_recent goes with kv_budget")
+        else:
+            kv_recent = kv_budget // 2 if kv_recent is None else kv_recent
+            if kv_cache != "int4":
+                raise ValueError("kv_budget goes with kv_cache='int4'")
+            if not (1 <= kv_budget < max_len and 0 <= kv_recent <= kv_budget and kv_slack >= 1):
+                raise ValueError("1 <= kv_budget < max_len, 0 <= kv_recent <= kv_budget and kv_slack >= 1")
+        if max_positions is None:
+            max_positions = max_len
+        if max_positions < max_len or (max_positions > max_len and kv_budget is None):
+            raise ValueError("max_positions is at least max_len, and beyond it only with a kv_budget")
+        self.prompt_attention, self.kv_cache, self.kv_budget = prompt_attention, kv_cache, kv_budget
+        self.kv_recent, self.kv_slack, self.max_positions = kv_recent, kv_slack, max_positions
         self.step_impl = step_impl
         self.native = native
         self.slot_decode_ctas = slot_decode_ctas
@@ -164,21 +204,32 @@ class Qwen3Decoder:
         # HF default rotary: inv_freq = theta^(-2i/hd); cos/sin in fp32, then the runtime dtype
         inv = 1.0 / (d.theta ** (torch.arange(0, d.head_dim, 2, dtype=torch.int64, device=dev).float()
                                  / d.head_dim))
-        freqs = torch.outer(torch.arange(max_len, device=dev).float(), inv)
+        freqs = torch.outer(torch.arange(max_positions, device=dev).float(), inv)
         emb = torch.cat((freqs, freqs), dim=-1)
         self.cos, self.sin = emb.cos().to(dt), emb.sin().to(dt)
         self.scaling = d.head_dim ** -0.5
-        self.k_cache = torch.zeros(d.n_layers, d.n_kv, max_len, d.head_dim, dtype=dt, device=dev)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.cache4 = self.kv_weights = None
+        if kv_cache == "int4":
+            from .attention import Cache4
+            self.cache4 = Cache4(d.n_layers, d.n_kv, max_len, d.head_dim, dev)
+            if kv_budget is not None:
+                self.kv_weights = torch.zeros(d.n_layers, d.n_kv, max_len, dtype=torch.float32, device=dev)
+        else:
+            self.k_cache = torch.zeros(d.n_layers, d.n_kv, max_len, d.head_dim, dtype=dt, device=dev)
+            self.v_cache = torch.zeros_like(self.k_cache)
+        self._dropped = self._since_evict = 0             # rows evicted since the prompt; steps since the last eviction
         self.positions = torch.arange(max_len, device=dev)
         self.causal = causal
         self.valid_bias = torch.tensor(0.0 if causal else 1.0, dtype=dt, device=dev)
         self.neg_inf = torch.tensor(float("-inf"), dtype=dt, device=dev)
-        self.causal_bias = torch.full((max_len, max_len), float("-inf"), dtype=dt, device=dev).triu(1)
+        if prompt_attention == "engine":
+            self.causal_bias = torch.full((max_len, max_len), float("-inf"), dtype=dt, device=dev).triu(1)
         self._tok = torch.zeros(1, dtype=torch.long, device=dev)
         self._pos = torch.zeros(1, dtype=torch.long, device=dev)
+        self._row = torch.zeros(1, dtype=torch.long, device=dev)              # the int4 cache's row of the step's token
         self._setup_weights()
         self.persist = None
+        self._evict_op = None
         if native:
             self._build_step_ops()
         if step_impl == "persistent":
@@ -265,11 +316,23 @@ class Qwen3Decoder:
         sin = self.sin.index_select(0, idx).view(1, 1, T, d.head_dim)
         q = q * cos + rotate_half(q) * sin                 # [1, nh, T, hd]
         k = k * cos + rotate_half(k) * sin                 # [1, nkv, T, hd]
-        kc, vc = self.k_cache[l], self.v_cache[l]
+        if pos is None and self.cache4 is not None:
+            from .attention import Cache4WriteOp
+            Cache4WriteOp(self.cache4.seq(l), k[0].transpose(0, 1), v[0].transpose(0, 1)).launch()
+        else:
+            kc, vc = self.k_cache[l], self.v_cache[l]
         if pos is None:
-            # the prompt: exactly the engine's ops (repeat_kv, batched matmuls)
-            kc[:, :T].copy_(k[0])
-            vc[:, :T].copy_(v[0])
+            if self.cache4 is None:
+                kc[:, :T].copy_(k[0])
+                vc[:, :T].copy_(v[0])
+            if self.prompt_attention == "fused":
+                # (the engine's mask adds the same to every score: none to the softmax)
+                from .attention import PromptAttentionOp
+                out = torch.empty(T, d.n_heads, d.head_dim, dtype=q.dtype, device=q.device)
+                PromptAttentionOp(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1), out,
+                                  scaling=self.scaling, causal=self.causal).launch()
+                return out.view(T, d.n_heads * d.head_dim)
+            # exactly the engine's ops (repeat_kv, batched matmuls)
             kr = k[:, :, None].expand(1, d.n_kv, rep, T, d.head_dim).reshape(1, d.n_heads, T, d.head_dim)
             vr = v[:, :, None].expand(1, d.n_kv, rep, T, d.head_dim).reshape(1, d.n_heads, T, d.head_dim)
             s = torch.matmul(q, kr.transpose(2, 3)) * self.scaling
@@ -362,7 +425,7 @@ class Qwen3Decoder:
     # -- the native decode step --------------------------------------------------------
     def _build_step_ops(self) -> None:
         """Kernel descriptors of the native decode step (one token at ``self._pos``)."""
-        from .step import AttentionOp, NormOp, SiluMulOp
+        from .step import NormOp, SiluMulOp
         d, dev, dt = self.dims, self.device, self.dtype
         self.h = torch.zeros(d.hidden, dtype=dt, device=dev)
         self.x_final = torch.zeros(d.hidden, dtype=dt, device=dev)
@@ -410,11 +473,7 @@ class Qwen3Decoder:
                                 add=None if first or land_d else down, add_tiles=tiles(down),
                                 token=self._tok if first else None, embed=self.embed if first else None,
                                 landing=None if first else land_d),
-                "attn": AttentionOp(q, k, v, L["self_attn.q_norm.weight"],
-                                    L["self_attn.k_norm.weight"], self.cos, self.sin, self._pos,
-                                    self.k_cache[l], self.v_cache[l], self.attn_out, n_heads=d.n_heads,
-                                    n_kv=d.n_kv, head_dim=d.head_dim, eps=d.eps, scaling=self.scaling,
-                                    valid_bias=0.0 if self.causal else 1.0, q_tiles=tiles(q), kv_tiles=tiles(k)),
+                "attn": self._attention_op(l, q, k, v, tiles(q), tiles(k)),
                 "norm2": NormOp(self.h, L["post_attention_layernorm.weight"], self.x_mlp, d.eps,
                                 add=None if land_o else o, add_tiles=tiles(o), landing=land_o),
             }
@@ -434,6 +493,34 @@ class Qwen3Decoder:
             self.step_ops.append(ops)
         self.final_op = NormOp(self.h, self.final_norm, self.x_final, d.eps, add=None if land_d else down,
                                add_tiles=tiles(down), landing=land_d)
+
+    def _attention_op(self, l: int, q, k, v, q_tiles: int, kv_tiles: int):
+        """Step attention of layer ``l`` over the decoder's cache."""
+        d, L = self.dims, self.layers[l]
+        qn, kn = L["self_attn.q_norm.weight"], L["self_attn.k_norm.weight"]
+        if self.cache4 is not None:
+            from .attention import Cache4AttentionOp
+            return Cache4AttentionOp(q, k, v, self.cache4.seq(l), self._row, self.attn_out, scaling=self.scaling,
+                                     n_heads=d.n_heads, weights=None if self.kv_weights is None else self.kv_weights[l:l + 1],
+                                     q_norm=qn, k_norm=kn, cos=self.cos, sin=self.sin, pos=self._pos, eps=d.eps,
+                                     q_tiles=q_tiles, kv_tiles=kv_tiles)
+        from .step import AttentionOp
+        return AttentionOp(q, k, v, qn, kn, self.cos, self.sin, self._pos, self.k_cache[l], self.v_cache[l],
+                           self.attn_out, n_heads=d.n_heads, n_kv=d.n_kv, head_dim=d.head_dim, eps=d.eps,
+                           scaling=self.scaling, valid_bias=0.0 if self.causal else 1.0, q_tiles=q_tiles,
+                           kv_tiles=kv_tiles)
+
+    def _evict(self, live: int) -> None:
+        """Keep ``kv_budget`` of every layer's ``live`` cache rows (one launch pair for all layers)."""
+        if self._evict_op is None:
+            from .attention import Cache4EvictOp
+            self._live = torch.zeros(self.dims.n_layers, dtype=torch.long, device=self.device)
+            self._evict_op = Cache4EvictOp(self.cache4, self.kv_weights, self._live, keep=self.kv_budget,
+                                           recent=self.kv_recent)
+        self._live.fill_(live)
+        self._evict_op.launch()
+        self._dropped += live - self.kv_budget
+        self._since_evict = 0
 
     def _cb_tiles(self, cid: str) -> torch.Tensor:
         """The codebook handed to rvq_gemv_tiles: fp16 when every value is an
@@ -508,12 +595,17 @@ class Qwen3Decoder:
         """Prompt ids [T] (device) -> last-position logits; cache rows 0..T-1 written."""
         if prompt.numel() > self.max_len:
             raise ValueError("prompt longer than the cache")
+        self._dropped = self._since_evict = 0
+        if self.kv_weights is not None:
+            self.kv_weights.zero_()
         with torch.inference_mode():
             return self._forward(prompt.view(-1), None)
 
     def capture(self) -> "Qwen3Decoder":
         """Record one decode step (token ``self._tok`` at ``self._pos``) as a CUDA graph."""
-        kv = (self.k_cache.clone(), self.v_cache.clone())
+        kept = [t for t in ((self.k_cache, self.v_cache) if self.cache4 is None else (self.cache4.data, self.kv_weights))
+                if t is not None]
+        kv = [t.clone() for t in kept]
         run = {"native": self._step_native, "persistent": self._step_persistent}.get(
             self.step_impl, lambda: self._forward(self._tok, self._pos))
         with torch.inference_mode():
@@ -527,19 +619,26 @@ class Qwen3Decoder:
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph):
                 self._logits = run()
-        self.k_cache.copy_(kv[0])                         # warm-up steps wrote row 0
-        self.v_cache.copy_(kv[1])
+        for t, was in zip(kept, kv):                      # warm-up steps wrote row 0
+            t.copy_(was)
         return self
 
     def step(self, token: torch.Tensor, pos: int) -> torch.Tensor:
         """One decode step by graph replay; ``token`` a device tensor of one id."""
         if self.graph is None:
             self.capture()
-        if not 0 <= pos < self.max_len:
+        row = pos - self._dropped                         # evicted rows moved the later ones down
+        if not (0 <= row < self.max_len and pos < self.max_positions):
             raise ValueError("position outside the cache")
         self._tok.copy_(token.view(1))
         self._pos.fill_(pos)
+        if self.cache4 is not None:
+            self._row.fill_(row)
         self.graph.replay()
+        if self.kv_budget is not None:
+            self._since_evict += 1
+            if row + 1 > self.kv_budget and (self._since_evict >= self.kv_slack or row + 1 == self.max_len):
+                self._evict(row + 1)
         return self._logits
 
     def check_waits(self) -> None:
@@ -560,6 +659,10 @@ class Qwen3Decoder:
                 from .gemv import take_wait_timeout
                 if take_wait_timeout():
                     failed.append("a fused GEMV code-copy wait")
+            if self.prompt_attention == "fused":
+                from .attention import take_timeout as take_attention_timeout
+                if take_attention_timeout():
+                    failed.append("a prompt attention wait")
             if self.persist is not None and self.persist.take_error():
                 failed.append("a persistent-step phase or code-copy wait")
         if failed:

@@ -56,6 +56,17 @@ struct Params {
     float2* part_ml;                         // [splits][tokens][n_heads]: maximum (times c) and sum
 };
 
+// A CTA's part of the call.
+struct Work {
+    int64_t q0, k0;                          // first query and key of the sequence
+    int32_t lq, lk;                          // their number
+    int32_t tok0;                            // first token of tile 0 in the sequence
+    int32_t j0;                              // first tile of keys
+    int32_t n[2];                            // tiles of keys that the two tiles of queries take from there on (0, 0: nothing to do)
+    int32_t live;                            // there is such a pair of tiles at all
+    int32_t clean;                           // the last tile of keys reaches into another sequence
+};
+
 template <int HD>
 struct Smem {
     static constexpr int kTileBytes = HD / 64 * kHalf;
@@ -66,8 +77,8 @@ struct Smem {
     uint64_t first_full, first_empty;        // K of tile 0
     uint64_t kv_full[2], kv_empty[2];        // V of tile j and K of tile j + 1, at j & 1
     float top[2][2][kRows];                  // a row's maximum (at the end: sum) over either half of the columns
+    Work work;
     uint32_t tmem;
-    int32_t seq, pair;                       // this CTA's sequence (-1: none) and pair of tiles in it
     int32_t dead;                            // a bounded wait gave up
 };
 
@@ -194,19 +205,24 @@ __device__ __forceinline__ float row_exp(float (&s)[2][32], int seen, float c, f
     return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// The sequence of pair number `want` (pairs counted over the sequences in order) by one warp: -1 if there is none.
-__device__ __forceinline__ void find_pair(const rvq_prompt_attn_args& a, int per_pair, int want, int32_t* seq, int32_t* pair) {
-    const int lane = threadIdx.x & 31;
+// Pair number `want` (pairs counted over the sequences in order) and part `split` of its keys, by one warp.
+__device__ __forceinline__ Work find_work(const Params& p, int want, int split) {
+    const rvq_prompt_attn_args& a = p.a;
+    const int lane = threadIdx.x & 31, T = p.tile_tokens;
+    const int32_t* cu_k = a.cu_k != nullptr ? a.cu_k : a.cu_q;
+    Work w = {};
     int64_t before = 0;
-    *seq = -1;
     for (int base = 0; base < a.n_seq; base += 32) {
         const int b = base + lane;
-        int64_t q0 = 0, q1 = 0;
+        int64_t q0 = 0, q1 = 0, k0 = 0, k1 = 0;
         if (b < a.n_seq) {
-            q0 = a.cu_q != nullptr ? max(0, __ldg(a.cu_q + b)) : 0;
-            q1 = a.cu_q != nullptr ? min(a.tokens, (int64_t)__ldg(a.cu_q + b + 1)) : a.tokens;
+            q1 = a.tokens, k1 = a.keys;
+            if (a.cu_q != nullptr) {
+                q0 = max(0, __ldg(a.cu_q + b)), q1 = min(q1, (int64_t)__ldg(a.cu_q + b + 1));
+                k0 = max(0, __ldg(cu_k + b)), k1 = min(k1, (int64_t)__ldg(cu_k + b + 1));
+            }
         }
-        const int64_t mine = q1 > q0 ? (q1 - q0 + per_pair - 1) / per_pair : 0;
+        const int64_t mine = q1 > q0 ? (q1 - q0 + 2 * T - 1) / (2 * T) : 0;
         int64_t upto = mine;                                 // inclusive prefix sum over the lanes
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -214,15 +230,33 @@ __device__ __forceinline__ void find_pair(const rvq_prompt_attn_args& a, int per
             if (lane >= o) upto += x;
         }
         const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
-        if (want < before + total) {
-            const uint32_t has = __ballot_sync(0xffffffffu, want < before + upto);
-            const int l = __ffs(has) - 1;
-            *seq = base + l;
-            *pair = (int32_t)(want - before - __shfl_sync(0xffffffffu, upto - mine, l));
-            return;
+        if (want >= before + total) {
+            before += total;
+            continue;
         }
-        before += total;
+        const int l = __ffs(__ballot_sync(0xffffffffu, want < before + upto)) - 1;
+        w.live = 1;
+        w.q0 = __shfl_sync(0xffffffffu, q0, l);
+        w.k0 = __shfl_sync(0xffffffffu, k0, l);
+        w.lq = (int)(__shfl_sync(0xffffffffu, q1, l) - w.q0);
+        w.lk = (int)max((int64_t)0, __shfl_sync(0xffffffffu, k1, l) - w.k0);
+        w.tok0 = (int)(want - before - __shfl_sync(0xffffffffu, upto - mine, l)) * 2 * T;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                        // what tile i's last token sees
+            const int last = min(w.lq, w.tok0 + (i + 1) * T) - 1;
+            const int see = last < w.tok0 + i * T ? 0 : a.causal ? min(w.lk, max(0, last + 1 + w.lk - w.lq)) : w.lk;
+            w.n[i] = (see + kKeys - 1) / kKeys;
+        }
+        const int64_t most = max(w.n[0], w.n[1]);
+        w.j0 = (int)(most * split / p.splits);
+        const int j1 = (int)(most * (split + 1) / p.splits);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w.n[i] = max(0, min(w.n[i], j1) - w.j0);
+        const int total_tiles = max(w.n[0], w.n[1]);
+        w.clean = w.lk % kKeys != 0 && total_tiles > 0 && (w.j0 + total_tiles) * kKeys > w.lk && w.k0 + w.lk < a.keys;
+        return w;
     }
+    return w;
 }
 
 // Output row of a query whose hidden values (keys [n, hidden_end) of the last tiles) may have leaked in, by a whole warp:
@@ -278,87 +312,70 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const int kv = unit % a.n_kv;
     const int T = p.tile_tokens;
     pdl_launch_dependents();
-    if (tid == 0) {
-        mbar_init(smem_addr(&S.q_full), 1);
-        mbar_init(smem_addr(&S.v_clean), 1);
-        mbar_init(smem_addr(&S.drain), 1);
-        mbar_init(smem_addr(&S.first_full), 1);
-        mbar_init(smem_addr(&S.first_empty), 1);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_addr(&S.kv_full[i]), 1);
-            mbar_init(smem_addr(&S.kv_empty[i]), 1);
-            mbar_init(smem_addr(&S.s_full[i]), 1);
-            mbar_init(smem_addr(&S.p_full[i]), kSoftmaxWarps / 2);
-            mbar_init(smem_addr(&S.o_full[i]), 1);
-        }
-        S.dead = 0;
-        mbar_init_fence();
-    }
-    if (warp == kSoftmaxWarps + 1) tmem_alloc(smem_addr(&S.tmem), 512);
-    pdl_wait();
+    auto load = [&](const CUtensorMap& map, uint8_t* dst, int64_t row, uint64_t& bar) {      // 128 keys, or a tile's tokens
+        for (int h = 0; h < HD / 64; ++h)
+            tma_load_3d(smem_addr(dst + h * kHalf), &map, 64 * h, &map == &p.q ? kv * p.rep : kv, (int)row, smem_addr(&bar));
+    };
+    auto load_step = [&](const Work& w, int j, int total) {  // V of tile j and K of tile j + 1
+        mbar_expect_tx(smem_addr(&S.kv_full[j & 1]), (j + 1 < total ? 2 : 1) * Smem<HD>::kTileBytes);
+        load(p.v, S.v[j & 1], w.k0 + (int64_t)(w.j0 + j) * kKeys, S.kv_full[j & 1]);
+        if (j + 1 < total) load(p.k, S.k[(j + 1) & 1], w.k0 + (int64_t)(w.j0 + j + 1) * kKeys, S.kv_full[j & 1]);
+    };
     if (warp == kSoftmaxWarps) {
+        // what there is to do, and its first loads, while the other warps get ready
+        if (lane == 0) {
+            mbar_init(smem_addr(&S.q_full), 1);
+            mbar_init(smem_addr(&S.v_clean), 1);
+            mbar_init(smem_addr(&S.drain), 1);
+            mbar_init(smem_addr(&S.first_full), 1);
+            mbar_init(smem_addr(&S.first_empty), 1);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(smem_addr(&S.kv_full[i]), 1);
+                mbar_init(smem_addr(&S.kv_empty[i]), 1);
+                mbar_init(smem_addr(&S.s_full[i]), 1);
+                mbar_init(smem_addr(&S.p_full[i]), kSoftmaxWarps / 2);
+                mbar_init(smem_addr(&S.o_full[i]), 1);
+            }
+            S.dead = 0;
+            mbar_init_fence();
+            fence_async_shared();
+        }
+        pdl_wait();
         // the last pairs of a causal sequence see the most keys: they start first
-        int32_t seq, pair = 0;
-        find_pair(a, 2 * T, p.pairs - 1 - unit / a.n_kv, &seq, &pair);
-        if (lane == 0) S.seq = seq, S.pair = pair;
+        const Work w = find_work(p, p.pairs - 1 - unit / a.n_kv, split);
+        if (lane == 0) {
+            S.work = w;
+            const int total = max(w.n[0], w.n[1]);
+            if (total > 0) {
+                const int tiles = w.tok0 + T < w.lq ? 2 : 1;
+                mbar_expect_tx(smem_addr(&S.q_full), tiles * (HD / 64) * (uint32_t)(T * p.rep * 128));
+                for (int i = 0; i < tiles; ++i) load(p.q, S.q[i], w.q0 + w.tok0 + i * T, S.q_full);
+                mbar_expect_tx(smem_addr(&S.first_full), Smem<HD>::kTileBytes);
+                load(p.k, S.k[0], w.k0 + (int64_t)w.j0 * kKeys, S.first_full);
+                load_step(w, 0, total);
+            }
+        }
+    } else {
+        if (warp == kSoftmaxWarps + 1) tmem_alloc(smem_addr(&S.tmem), 512);
+        pdl_wait();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = S.tmem;
-    const int seq = S.seq;
-    if (seq >= 0) {
-        int64_t q0 = 0, q1 = a.tokens, k0 = 0, k1 = a.keys;
-        if (a.cu_q != nullptr) {
-            const int32_t* cu_k = a.cu_k != nullptr ? a.cu_k : a.cu_q;
-            q0 = max(0, __ldg(a.cu_q + seq)), q1 = min(a.tokens, (int64_t)__ldg(a.cu_q + seq + 1));
-            k0 = max(0, __ldg(cu_k + seq)), k1 = min(a.keys, (int64_t)__ldg(cu_k + seq + 1));
-        }
-        const int lq = (int)(q1 - q0), lk = (int)max((int64_t)0, k1 - k0);
-        const int tok0 = S.pair * 2 * T;                     // first token of tile 0 in its sequence
-        // keys that tile i's last token sees, in tiles
-        int n[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int last = min(lq, tok0 + (i + 1) * T) - 1;
-            const int see = last < tok0 + i * T ? 0 : a.causal ? min(lk, max(0, last + 1 + lk - lq)) : lk;
-            n[i] = (see + kKeys - 1) / kKeys;
-        }
-        // this CTA's part of them: tiles j0 .. of the keys (from here on counted from j0)
-        const int j0 = (int)((int64_t)max(n[0], n[1]) * split / p.splits);
-        const int j1 = (int)((int64_t)max(n[0], n[1]) * (split + 1) / p.splits);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) n[i] = max(0, min(n[i], j1) - j0);
+    if (S.work.live) {
+        const int64_t q0 = S.work.q0, k0 = S.work.k0;
+        const int lq = S.work.lq, lk = S.work.lk, tok0 = S.work.tok0, j0 = S.work.j0;
+        const int n[2] = {S.work.n[0], S.work.n[1]};
         const int total = max(n[0], n[1]);
-        // values of others in the last tile
-        const bool clean = lk % kKeys != 0 && (j0 + total) * kKeys > lk && total > 0 && k0 + lk < a.keys;
+        const bool clean = S.work.clean;
 
         if (warp == kSoftmaxWarps) {
-            if (lane == 0 && total > 0) {
-                mbar_expect_tx(smem_addr(&S.q_full), (n[1] > 0 ? 2 : 1) * HD / 64 * (uint32_t)(T * p.rep * 128));
-                for (int i = 0; i < (n[1] > 0 ? 2 : 1); ++i)
-                    for (int h = 0; h < HD / 64; ++h)
-                        tma_load_3d(smem_addr(S.q[i] + h * kHalf), &p.q, 64 * h, kv * p.rep, (int)q0 + tok0 + i * T,
-                                    smem_addr(&S.q_full));
-            }
-            auto load = [&](const CUtensorMap& map, uint8_t* dst, int j, uint64_t& bar) {
-                for (int h = 0; h < HD / 64; ++h)
-                    tma_load_3d(smem_addr(dst + h * kHalf), &map, 64 * h, kv, (int)k0 + (j0 + j) * kKeys, smem_addr(&bar));
-            };
-            if (lane == 0 && total > 0) {
-                mbar_expect_tx(smem_addr(&S.first_full), Smem<HD>::kTileBytes);
-                load(p.k, S.k[0], 0, S.first_full);
-            }
-            int loaded = 0;
-            for (int j = 0; j < total; ++j) {
-                const int st = j & 1;
-                if (j >= 2 && !wait(S, S.kv_empty[st], (j / 2 - 1) & 1)) break;
+            int loaded = min(total, 1);
+            for (int j = 1; j < total; ++j) {
+                if (j >= 2 && !wait(S, S.kv_empty[j & 1], (j / 2 - 1) & 1)) break;
                 if (j == 1 && !wait(S, S.first_empty, 0)) break;            // K of tile 2 replaces that of tile 0
-                if (lane == 0) {
-                    mbar_expect_tx(smem_addr(&S.kv_full[st]), (j + 1 < total ? 2 : 1) * Smem<HD>::kTileBytes);
-                    load(p.v, S.v[st], j, S.kv_full[st]);
-                    if (j + 1 < total) load(p.k, S.k[st ^ 1], j + 1, S.kv_full[st]);
-                }
+                if (lane == 0) load_step(S.work, j, total);
                 loaded = j + 1;
             }
             if (clean && loaded == total && wait(S, S.kv_full[(total - 1) & 1], ((total - 1) / 2) & 1)) {

@@ -629,8 +629,8 @@ typedef struct rvq_prompt_attn_args {
 size_t rvq_prompt_attention_workspace_size(const rvq_prompt_attn_args* a);
 int rvq_prompt_attention(const rvq_prompt_attn_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Reads and clears the sticky flag set when a bounded wait of the prompt or
- * step attention gave up (that launch's result is then invalid).
+/* Reads and clears the sticky flag set when a bounded wait of the prompt
+ * attention gave up (that launch's result is then invalid).
  * Synchronises the current device.  Returns 1, 0 or -RVQ_ERR_CUDA. */
 int rvq_take_attention_timeout(void);
 
@@ -703,14 +703,16 @@ typedef struct rvq_cache4_attn_args {
     const int64_t* rows;      /* device [n_seq] */
     void* out;                /* device [n_seq][n_heads][head_dim], fp16 for fp16 q, else bf16 */
     float* weights;           /* device [n_seq][n_kv][max_len], or NULL */
-    float* scores;            /* device [n_seq][n_heads][max_len] of workspace; needed with weights */
     int32_t n_heads;          /* n_heads / n_kv <= 64 */
     int32_t table_len;
     float eps;
     float scaling;
 } rvq_cache4_attn_args;
 
-int rvq_cache4_attention(const rvq_cache4_attn_args* a, void* stream);
+/* Bytes of device workspace (16-byte aligned) that the call needs.  One call at a
+ * time uses a workspace; its contents need no initialisation. */
+size_t rvq_cache4_attention_workspace_size(const rvq_cache4_attn_args* a);
+int rvq_cache4_attention(const rvq_cache4_attn_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Eviction by accumulated attention weight, for every (sequence, kv head): of
  * n = rows[b] live rows the last `recent` stay, and of the n - recent rows

@@ -6,7 +6,7 @@ As in ``rvq_b200.step``, each ``*Op`` resolves its pointers once and
 ``launch()`` queues its kernels on the current stream of its tensors' device,
 so launches can be captured in a CUDA graph.  The tensors an op was built
 from must outlive it and keep their storage; an op with a workspace of its own
-(``PromptAttentionOp``, ``Cache4AttentionOp`` with weights) runs one launch at
+(``PromptAttentionOp``, ``Cache4AttentionOp``) runs one launch at
 a time and outlives its launches.
 """
 
@@ -49,7 +49,7 @@ class RvqCache4AttnArgs(ctypes.Structure):
     _fields_ = [("q", RvqVec), ("k", RvqVec), ("v", RvqVec), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
                 ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("cache", RvqCache4),
                 ("rows", ctypes.c_void_p), ("out", ctypes.c_void_p), ("weights", ctypes.c_void_p),
-                ("scores", ctypes.c_void_p), ("n_heads", ctypes.c_int32), ("table_len", ctypes.c_int32),
+                ("n_heads", ctypes.c_int32), ("table_len", ctypes.c_int32),
                 ("eps", ctypes.c_float), ("scaling", ctypes.c_float)]
 
 
@@ -78,8 +78,10 @@ def _lib():
         for name in ("rvq_cache4_write", "rvq_cache4_read"):
             getattr(lib, name).restype = i32
             getattr(lib, name).argtypes = [P(RvqCache4RowsArgs), vp]
+        lib.rvq_cache4_attention_workspace_size.restype = ctypes.c_size_t
+        lib.rvq_cache4_attention_workspace_size.argtypes = [P(RvqCache4AttnArgs)]
         lib.rvq_cache4_attention.restype = i32
-        lib.rvq_cache4_attention.argtypes = [P(RvqCache4AttnArgs), vp]
+        lib.rvq_cache4_attention.argtypes = [P(RvqCache4AttnArgs), vp, ctypes.c_size_t, vp]
         lib.rvq_cache4_evict.restype = i32
         lib.rvq_cache4_evict.argtypes = [P(RvqCache4EvictArgs), vp]
         _bound = True
@@ -181,6 +183,13 @@ class _Op:
             raise ValueError("every tensor must be on the same device")
         self.device = dev
 
+    def _workspace(self, size) -> int:
+        """Allocates what ``self.args`` needs; its bytes."""
+        with torch.cuda.device(self.device):
+            n = size(ctypes.byref(self.args))
+        self._ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        return n
+
     def _bind(self, where: str, *args) -> None:
         """The C entry point and its arguments but the stream, resolved once."""
         self._where, self._fn, self._args = where, getattr(_lib(), where), args
@@ -252,9 +261,7 @@ class PromptAttentionOp(_Op):
         self.args = RvqPromptAttnArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cu_q), _ptr(cu_k), tokens,
                                       keys, _strides(q), _strides(k), _strides(v), _strides(out), n_seq, nh, nkv, hd,
                                       float(scaling), int(bool(causal)), _native.kind_of(q), 0)
-        with torch.cuda.device(self.device):
-            n = _lib().rvq_prompt_attention_workspace_size(ctypes.byref(self.args))
-        self._ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        n = self._workspace(_lib().rvq_prompt_attention_workspace_size)
         self._bind("rvq_prompt_attention", ctypes.byref(self.args), _ptr(self._ws), n)
 
 
@@ -396,13 +403,11 @@ class Cache4AttentionOp(_Op):
             for b, bn in written[i + 1:] + [(t, tn) for t, tn in ((q, "q"), (k, "k"), (v, "v")) if t is not None]:
                 _apart(a, b, f"{an} and {bn}")
         self._on(q, k, v, cache.data, rows, out, weights, q_norm, k_norm, cos, sin, pos)
-        self._scores = None
-        if weights is not None:
-            self._scores = torch.empty(n, n_heads, cache.max_len, dtype=torch.float32, device=self.device)
         self.args = RvqCache4AttnArgs(qv, kv_, vv, _ptr(q_norm), _ptr(k_norm), _ptr(cos), _ptr(sin), _ptr(pos),
-                                      cache.struct(), _ptr(rows), _ptr(out), _ptr(weights), _ptr(self._scores), n_heads,
-                                      table, float(eps), float(scaling))
-        self._bind("rvq_cache4_attention", ctypes.byref(self.args))
+                                      cache.struct(), _ptr(rows), _ptr(out), _ptr(weights), n_heads, table, float(eps),
+                                      float(scaling))
+        n = self._workspace(_lib().rvq_cache4_attention_workspace_size)
+        self._bind("rvq_cache4_attention", ctypes.byref(self.args), _ptr(self._ws), n)
 
 
 class Cache4EvictOp(_Op):

@@ -2,13 +2,9 @@
 
 #include <string.h>
 
-#include <cooperative_groups.h>
-
 #include "rvq_cache4.cuh"
 #include "rvq_sm100.cuh"
 #include "rvq_stepops.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace rvq {
 namespace cache4 {
@@ -17,24 +13,20 @@ using namespace stepops;
 using sm100::smem_addr;
 
 // ---------------------------------------------------------------------------
-// A cluster of C CTAs per (kv head, group of at most 8 query heads, sequence)
-// splits the live rows into contiguous ranges of 32-row tiles; in a CTA the
-// warps take the range's tiles in turn, each through a ring of its own that
-// bulk copies fill (a tile's records are contiguous).  Both products run on
-// mma.m16n8k16 with the heads as rows:
+// The live rows of a (kv head, group of at most 8 query heads, sequence) are
+// split into contiguous ranges of 16-row tiles, a CTA each; in a CTA the warps
+// take the range's tiles in turn, each through a ring of its own (cp.async).
+// Both products run on mma.m16n8k16:
 //
 //   scores   q . k = sum over groups of  step (q . c) + zero (q . 1)
 //   output   sum_j p_j v_j = sum_j (p_j step_j) c_j + sum_j p_j zero_j
 //
-// so an operand is a 4-bit code, never a rounded value.  A code becomes a bf16
-// number by placing it in the mantissa of 1.0: 1 + c / 16, exact, one shift and
-// one lop3 for two codes; the 1 is taken out again by starting the score
-// accumulator at -(q . 1) and by subtracting 16 p step in the zeros' sum.
-// p step is split into a bf16 part in rows 0..7 and the bf16 remainder in rows
-// 8..15 of the same operand (16 bits of it, at no further MMA); an fp16 q the
-// same way.  Softmax: one pass, running maximum and sum per warp, partial
-// results joined warp by warp and CTA by CTA in fixed order through shared
-// and distributed shared memory, so results do not depend on scheduling.
+// so an operand is a 4-bit code (exact), never a rounded value; the sums with
+// the zeros are one more MMA each, on the parameter words as they lie there.
+// p step is split into two bf16 parts (16 bits), q . 1 into three (24 bits), an
+// fp16 q into two (exact).  Softmax: one pass, running maximum and sum per warp;
+// partial results are joined in fixed order, warp by warp in the CTA and range
+// by range in a second launch, so results do not depend on scheduling.
 // ---------------------------------------------------------------------------
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
@@ -54,8 +46,6 @@ struct Smem {
     float kv[2][HD];                         // the new key and value
     float norm[4][HD];
     float wm[kWarps][kHeads], wl[kWarps][kHeads];
-    float m[kHeads], l[kHeads];              // this CTA's maximum and sum
-    float fm[kHeads], fr[kHeads];            // the final maximum and 1 / sum
 };
 
 // c / 64 for the codes c in bits 4 I .. and 4 I + 16 .. (I = 0 or 1) of a word, as a bf16 pair.  A code in a bf16
@@ -294,43 +284,57 @@ __device__ __forceinline__ void encode(const float* x, uint8_t* codes, uint32_t*
     if (lane % LG == 0) params[lane / LG] = p;
 }
 
+// Workspace: the ranges' partial results, then the scores (with weights only), in powers of two.
+struct Work {
+    float2* ml;                              // [splits][n_seq][n_heads]: maximum and sum
+    float* o;                                // [splits][n_seq][n_heads][head_dim]
+    float* scores;                           // [n_seq][n_heads][max_len]
+    int32_t splits;
+};
+
+// Whether the sequence has something to attend to: 1; zeros in its output: 0; left alone: -1.
+__device__ __forceinline__ int state_of(const rvq_cache4_attn_args& a, int b, int64_t* rows) {
+    *rows = a.rows[b];
+    if (*rows < 0) return -1;
+    const bool append = a.k.ptr != nullptr;
+    const int64_t pos = a.pos != nullptr ? a.pos[b] : 0;
+    return *rows + append >= 1 && *rows + append <= a.cache.max_len && pos >= 0 && (a.pos == nullptr || pos < a.table_len);
+}
+
 template <int HD, bool kSplitQ>
-__global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_attn_args a, int passes) {
+__global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_attn_args a, Work work) {
     constexpr int G = HD / kGroup, REC = record_bytes(HD);
     extern __shared__ __align__(128) uint8_t smem_raw[];
     Smem<HD>& S = *reinterpret_cast<Smem<HD>*>(smem_raw);
-    cg::cluster_group cluster = cg::this_cluster();
-    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int nkv = a.cache.n_kv, rep = a.n_heads / nkv;
-    const int kv = blockIdx.y % nkv, b = blockIdx.z;
+    const int split = blockIdx.x, kv = blockIdx.y % nkv, group = blockIdx.y / nkv, b = blockIdx.z;
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t rows = a.rows[b];
-    if (rows < 0) return;                                    // the same in every CTA of the cluster
+    int64_t rows;
+    const int state = state_of(a, b, &rows);
+    if (state < 0) return;
     const bool append = a.k.ptr != nullptr;
-    const int64_t pos = a.pos != nullptr ? a.pos[b] : 0;
-    const int64_t kv_at = ((int64_t)b * nkv + kv) * HD;
-    const int out_kind = a.q.kind == RVQ_F16 ? RVQ_F16 : RVQ_BF16;
-    // heads [h0, h1) of the kv head: all of them in `passes` passes of this CTA, or one group of them per CTA
     const int groups = (rep + kHeads - 1) / kHeads, per = (rep + groups - 1) / groups;
-    const int first = passes == groups ? 0 : blockIdx.y / nkv;
-    if (rows + append < 1 || rows + append > a.cache.max_len || pos < 0 || (a.pos != nullptr && pos >= a.table_len)) {
-        if (rank == 0) {
-            const int h0 = first * per, h1 = min(rep, (first + passes) * per);
-            const int64_t at = ((int64_t)b * a.n_heads + kv * rep) * HD;
-            for (int i = h0 * HD + tid; i < h1 * HD; i += kThreads) store_from_f32(a.out, at + i, out_kind, 0.f);
-        }
+    const int h0 = group * per, heads = min(per, rep - h0);
+    const int64_t head0 = (int64_t)b * a.n_heads + kv * rep + h0, q_at = head0 * HD;      // of all sequences' heads
+    const int out_kind = a.q.kind == RVQ_F16 ? RVQ_F16 : RVQ_BF16;
+    if (state == 0) {
+        if (split == 0)
+            for (int i = tid; i < heads * HD; i += kThreads) store_from_f32(a.out, q_at + i, out_kind, 0.f);
+        return;
+    }
+    const int live = (int)rows, tiles = (live + kTile - 1) / kTile;
+    const int t0 = (int)((int64_t)tiles * split / work.splits), t1 = (int)((int64_t)tiles * (split + 1) / work.splits);
+    const bool owner = append && split == 0;                 // this CTA attends to the new row
+    float2* ml = work.ml + ((int64_t)split * a.cache.n_seq * a.n_heads + head0);
+    if (t0 == t1 && !owner) {                                // fewer tiles than ranges
+        if (tid < heads) ml[tid] = make_float2(-INFINITY, 0.f);
         return;
     }
     uint8_t* cache = reinterpret_cast<uint8_t*>(a.cache.data) + ((int64_t)b * nkv + kv) * a.cache.max_len * REC;
-    const int tiles = (int)((rows + kTile - 1) / kTile);
-    const int t0 = (int)((int64_t)tiles * rank / C), t1 = (int)((int64_t)tiles * (rank + 1) / C);
-    const bool owner = append && rank == 0;                  // this CTA attends to the new row
-
     uint32_t shift;
     asm volatile("mov.u32 %0, 65536;" : "=r"(shift));
-    const int live = (int)rows;
     // this lane's 16-byte pieces of tile number `tile`, into a stage of the warp's ring; a group for every stage, so that
     // the number of groups behind a tile is known
     const uint32_t ring = smem_addr(S.ring[warp][0]) + 16 * lane;
@@ -345,173 +349,226 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
+    for (int i = 0; i < kStages - 1; ++i) fetch(t0 + warp + i * kWarps, i);
 
-    for (int pass = 0; pass < passes; ++pass) {
-        const int h0 = (first + pass) * per, heads = min(per, rep - h0);
-        const int64_t q_at = ((int64_t)b * a.n_heads + kv * rep + h0) * HD;
-        for (int i = 0; i < kStages - 1; ++i) fetch(t0 + warp + i * kWarps, i);
+    // the heads' q, and the new record
+    const bool rotate = a.q_norm != nullptr || a.cos != nullptr;
+    if (rotate) {
+        const int64_t pos = a.pos != nullptr ? a.pos[b] : 0;
+        for (int i = tid; i < HD; i += kThreads) {
+            S.norm[0][i] = a.q_norm != nullptr ? bf16_at(a.q_norm, i) : 0.f;
+            S.norm[1][i] = a.q_norm != nullptr ? bf16_at(a.k_norm, i) : 0.f;
+            S.norm[2][i] = a.cos != nullptr ? bf16_at(a.cos, pos * HD + i) : 0.f;
+            S.norm[3][i] = a.cos != nullptr ? bf16_at(a.sin, pos * HD + i) : 0.f;
+        }
+    }
+    for (int i = tid; i < kHeads * HD; i += kThreads)
+        (&S.q[0][0])[i] = i < heads * HD ? vec_value_deep(a.q, q_at + i) : 0.f;
+    if (owner) {
+        const int64_t kv_at = ((int64_t)b * nkv + kv) * HD;
+        for (int i = tid; i < 2 * HD; i += kThreads) (&S.kv[0][0])[i] = vec_value_deep(i < HD ? a.k : a.v, kv_at + i % HD);
+        for (int i = tid; i < kTile * REC / 4; i += kThreads) reinterpret_cast<uint32_t*>(S.fresh)[i] = 0;
+    }
+    __syncthreads();
+    if (rotate) {
+        norm_rope<HD>(S.q[warp], S.norm[0], a, S.norm[2], S.norm[3]);
+        if (owner && warp == 0) norm_rope<HD>(S.kv[0], S.norm[1], a, S.norm[2], S.norm[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        const float x = warp_sum(S.q[warp][kGroup * i + lane]);
+        if (lane == 0) S.qsum[warp][i] = x;
+    }
+    if (owner && warp < 2)                                   // the warp that rotated the key, and another
+        encode<HD>(S.kv[warp], S.fresh + warp * (HD / 2), reinterpret_cast<uint32_t*>(S.fresh + HD + warp * (HD / 8)));
+    __syncthreads();
+    if (owner && group == 0 && tid < REC / 16)
+        reinterpret_cast<uint4*>(cache + rows * REC)[tid] = reinterpret_cast<const uint4*>(S.fresh)[tid];
 
-        // the heads' q, and the new record
-        if (pass == 0 && (a.q_norm != nullptr || a.cos != nullptr)) {
-            for (int i = tid; i < HD; i += kThreads) {
-                S.norm[0][i] = a.q_norm != nullptr ? bf16_at(a.q_norm, i) : 0.f;
-                S.norm[1][i] = a.q_norm != nullptr ? bf16_at(a.k_norm, i) : 0.f;
-                S.norm[2][i] = a.cos != nullptr ? bf16_at(a.cos, pos * HD + i) : 0.f;
-                S.norm[3][i] = a.cos != nullptr ? bf16_at(a.sin, pos * HD + i) : 0.f;
-            }
-        }
-        for (int i = tid; i < kHeads * HD; i += kThreads)
-            (&S.q[0][0])[i] = i < heads * HD ? vec_value_deep(a.q, q_at + i) : 0.f;
-        if (owner && pass == 0) {
-            for (int i = tid; i < 2 * HD; i += kThreads) (&S.kv[0][0])[i] = vec_value_deep(i < HD ? a.k : a.v, kv_at + i % HD);
-            for (int i = tid; i < kTile * REC / 4; i += kThreads) reinterpret_cast<uint32_t*>(S.fresh)[i] = 0;
-        }
-        __syncthreads();
-        if (a.q_norm != nullptr || a.cos != nullptr) {
-            norm_rope<HD>(S.q[warp], S.norm[0], a, S.norm[2], S.norm[3]);
-            if (owner && pass == 0 && warp == 0) norm_rope<HD>(S.kv[0], S.norm[1], a, S.norm[2], S.norm[3]);
-        }
-        {
-            float v[G];
+    // operand rows 0..7: q (its bf16 part), rows 8..15: the remainder; column pairs in the code words' order
+    uint32_t qa[HD / 16][kSplitQ ? 4 : 2];
+    // (q . 1) / 64 of group t against the pairs (zero, step), in three bf16 parts: 24 bits
+    uint32_t qz[3] = {0u, 0u, 0u};
+    if (t < G) {
+        const float x = S.qsum[g][t] * 0.015625f;
+        const float hi = bf16r(x), lo = bf16r(x - hi);
+        qz[0] = pack_bf16(hi, 0.f), qz[1] = pack_bf16(lo, 0.f), qz[2] = pack_bf16(x - hi - lo, 0.f);
+    }
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                v[i] = warp_sum(S.q[warp][kGroup * i + lane]);
-                if (lane == 0) S.qsum[warp][i] = v[i];
-            }
+    for (int i = 0; i < HD / 16; ++i) {
+        const float* q = &S.q[g][i / 2 * kGroup + 8 * t + 2 * (i & 1)];
+        if constexpr (kSplitQ) {
+            split_bf16(q[0], q[4], &qa[i][0], &qa[i][2], 65536u);
+            split_bf16(q[1], q[5], &qa[i][1], &qa[i][3], 65536u);
+        } else {
+            qa[i][0] = pack_bf16(q[0], q[4]);
+            qa[i][1] = pack_bf16(q[1], q[5]);
         }
-        if (owner && pass == 0 && warp < 2)                  // the warp that rotated the key, and another
-            encode<HD>(S.kv[warp], S.fresh + warp * (HD / 2), reinterpret_cast<uint32_t*>(S.fresh + HD + warp * (HD / 8)));
-        __syncthreads();
-        if (owner && pass == 0 && first == 0 && tid < REC / 16)
-            reinterpret_cast<uint4*>(cache + rows * REC)[tid] = reinterpret_cast<const uint4*>(S.fresh)[tid];
+    }
+    State<HD> st;
+    st.m = -INFINITY, st.l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) st.zero[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) st.o[i][j][c] = 0.f;
+    const float scale64 = a.scaling * 64.f * 1.4426950408889634f;      // scores in powers of two
+    float* sc = a.weights != nullptr && g < heads ? work.scores + (head0 + g) * a.cache.max_len : nullptr;
+    // the last warp begins with the appended record
+    bool extra = owner && warp == kWarps - 1;
+    for (int tile = t0 + warp, stage = 0; tile < t1 || extra;) {
+        uint32_t rec = smem_addr(S.fresh);
+        int row = live, valid = 1;
+        if (!extra) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
+            __syncwarp();                                    // every lane's pieces are here, and the stage before this one is read
+            fetch(tile + (kStages - 1) * kWarps, stage == 0 ? kStages - 1 : stage - 1);
+            rec = smem_addr(S.ring[warp][stage]);
+            row = tile * kTile;
+            valid = min(kTile, live - row);
+            tile += kWarps;
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+        extra = false;
+        tile_step<HD, kSplitQ>(rec, valid, qa, qz, scale64, shift, st, sc ? sc + row : sc);
+    }
+    // lanes 4 g .. 4 g + 3 hold parts of head g's sum
+    float l = st.l;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const float zero = st.zero[0] + st.zero[2];              // head g, group t
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    __syncthreads();                                         // the rings are read: they take the warps' outputs
+    float* wo = reinterpret_cast<float*>(S.ring);            // [kWarps][kHeads][HD]
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        // the zeros' sums of heads 2 t and 2 t + 1
+        const float z0 = __shfl_sync(0xffffffffu, zero, 8 * t + i), z1 = __shfl_sync(0xffffffffu, zero, 8 * t + 4 + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float* d = wo + (warp * kHeads + 2 * t) * HD + kGroup * i + 4 * g + j;
+            d[0] = fmaf(64.f, st.o[i][j >> 1][2 * (j & 1)], z0);
+            d[HD] = fmaf(64.f, st.o[i][j >> 1][2 * (j & 1) + 1], z1);
+        }
+    }
+    if (t == 0) S.wm[warp][g] = st.m, S.wl[warp][g] = l;
+    __syncthreads();
+    // warp w joins head w over the warps
+    if (warp >= heads) return;
+    float m = S.wm[0][warp];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, S.wm[w][warp]);
+    float total = 0.f, o[HD / 32];
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const float f = S.wm[w][warp] == m ? 1.f : exp2_approx(S.wm[w][warp] - m);
+        total = fmaf(f, S.wl[w][warp], total);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) o[d] = fmaf(f, wo[(w * kHeads + warp) * HD + 32 * d + lane], o[d]);
+    }
+    if (lane == 0) ml[warp] = make_float2(m, total);
+    const float inv = total == 0.f ? 0.f : 1.f / total;      // no score above -infinity: zeros
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d) {
+        if (work.splits == 1)
+            store_from_f32(a.out, q_at + warp * HD + 32 * d + lane, out_kind, inv == 0.f ? 0.f : o[d] * inv);
+        else
+            work.o[((int64_t)split * a.cache.n_seq * a.n_heads + head0 + warp) * HD + 32 * d + lane] = o[d];
+    }
+}
 
-        // operand rows 0..7: q (its bf16 part), rows 8..15: the remainder; column pairs in the code words' order
-        uint32_t qa[HD / 16][kSplitQ ? 4 : 2];
-        // (q . 1) / 64 of group t against the pairs (zero, step), in three bf16 parts: 24 bits
-        uint32_t qz[3] = {0u, 0u, 0u};
-        if (t < G) {
-            const float x = S.qsum[g][t] * 0.015625f;
-            const float hi = bf16r(x), lo = bf16r(x - hi);
-            qz[0] = pack_bf16(hi, 0.f), qz[1] = pack_bf16(lo, 0.f), qz[2] = pack_bf16(x - hi - lo, 0.f);
+// The ranges joined.  Blocks x < out_blocks: 256 output values of the kv head's query heads each; the others: the weights of
+// kJoinRows rows each, heads in order.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 1024;
+constexpr int kMaxSplits = 320;              // plan keeps below it
+
+// Maximum and sum of a head over the ranges, by one warp; with f, the ranges' factors (0 for an empty one).
+__device__ __forceinline__ float2 join_head(const float2* ml, int64_t step, int splits, float* f) {
+    constexpr int U = kMaxSplits / 32;
+    const int lane = threadIdx.x & 31;
+    float2 x[U];
+    float m = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int s = 32 * u + lane;
+        x[u] = s < splits ? __ldcg(ml + s * step) : make_float2(-INFINITY, 0.f);
+        m = fmaxf(m, x[u].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const float g = x[u].y == 0.f ? 0.f : x[u].x == m ? 1.f : exp2_approx(x[u].x - m);
+        total = fmaf(g, x[u].y, total);
+        if (f != nullptr && 32 * u + lane < splits) f[32 * u + lane] = g;
+    }
+    return make_float2(m, warp_sum(total));
+}
+
+__global__ void __launch_bounds__(kJoinThreads) cache4_join_kernel(rvq_cache4_attn_args a, Work work, int out_blocks) {
+    constexpr int kBlockHeads = kJoinThreads / 64;           // heads that 256 output values may touch
+    __shared__ float fm[kMaxRep], fr[kMaxRep], f[kBlockHeads][kMaxSplits];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int nkv = a.cache.n_kv, rep = a.n_heads / nkv, hd = a.cache.head_dim;
+    const int kv = blockIdx.y, b = blockIdx.z;
+    int64_t rows;
+    if (state_of(a, b, &rows) != 1) return;
+    const int64_t head0 = (int64_t)b * a.n_heads + kv * rep, all = (int64_t)a.cache.n_seq * a.n_heads;
+    const bool append = a.k.ptr != nullptr;
+    const int64_t n = rows + append, first = (int64_t)((int)blockIdx.x - out_blocks) * kJoinRows;
+    if (first >= n) return;
+    const bool output = first < 0;
+    const int h0 = output ? blockIdx.x * (kJoinThreads / hd) : 0, h1 = output ? min(rep, h0 + kJoinThreads / hd) : rep;
+    for (int h = h0 + warp; h < h1; h += kJoinThreads / 32) {
+        const float2 x = join_head(work.ml + head0 + h, all, work.splits, output ? f[h - h0] : nullptr);
+        if (lane == 0) fm[h] = x.x, fr[h] = x.y == 0.f ? 0.f : 1.f / x.y;
+    }
+    __syncthreads();
+    if (output) {
+        const int i = blockIdx.x * kJoinThreads + tid, h = i / hd;
+        if (i >= rep * hd) return;
+        const float* o = work.o + head0 * hd + i;
+        const float* g = f[h - h0];
+        float sum = 0.f;
+#pragma unroll 8
+        for (int s = 0; s < work.splits; ++s) {
+            const float v = __ldcg(o + s * all * hd);        // of an empty range: whatever is there
+            sum = g[s] == 0.f ? sum : fmaf(g[s], v, sum);
         }
+        store_from_f32(a.out, head0 * hd + i, a.q.kind == RVQ_F16 ? RVQ_F16 : RVQ_BF16, fr[h] == 0.f ? 0.f : sum * fr[h]);
+        return;
+    }
+    float* w = a.weights + ((int64_t)b * nkv + kv) * a.cache.max_len;
+    const float* sc = work.scores + head0 * a.cache.max_len;
+    constexpr int U = kJoinRows / kJoinThreads;
+    float v[U];
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-            const float* q = &S.q[g][i / 2 * kGroup + 8 * t + 2 * (i & 1)];
-            if constexpr (kSplitQ) {
-                split_bf16(q[0], q[4], &qa[i][0], &qa[i][2], 65536u);
-                split_bf16(q[1], q[5], &qa[i][1], &qa[i][3], 65536u);
-            } else {
-                qa[i][0] = pack_bf16(q[0], q[4]);
-                qa[i][1] = pack_bf16(q[1], q[5]);
-            }
+    for (int u = 0; u < U; ++u) {
+        const int64_t row = first + u * kJoinThreads + tid;
+        v[u] = row < n && !(append && row == rows) ? w[row] : 0.f;
+    }
+#pragma unroll 4
+    for (int h = 0; h < rep; ++h) {
+        const float m = fm[h], r = fr[h];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = first + u * kJoinThreads + tid;
+            const float s = row < n ? __ldcg(sc + (int64_t)h * a.cache.max_len + row) : 0.f;
+            if (r != 0.f) v[u] += exp2_approx(s - m) * r;
         }
-        State<HD> st;
-        st.m = -INFINITY, st.l = 0.f;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st.zero[i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) st.o[i][j][c] = 0.f;
-        }
-        const float scale64 = a.scaling * 64.f * 1.4426950408889634f;      // scores in powers of two
-        float* sc = a.weights != nullptr && g < heads
-                        ? a.scores + ((int64_t)b * a.n_heads + kv * rep + h0 + g) * a.cache.max_len : nullptr;
-        // the last warp begins with the appended record
-        bool extra = owner && warp == kWarps - 1;
-        for (int tile = t0 + warp, stage = 0; tile < t1 || extra;) {
-            uint32_t rec = smem_addr(S.fresh);
-            int row = live, valid = 1;
-            if (!extra) {
-                asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
-                __syncwarp();                                // every lane's pieces are here, and the stage before this one is read
-                fetch(tile + (kStages - 1) * kWarps, stage == 0 ? kStages - 1 : stage - 1);
-                rec = smem_addr(S.ring[warp][stage]);
-                row = tile * kTile;
-                valid = min(kTile, live - row);
-                tile += kWarps;
-                stage = stage + 1 == kStages ? 0 : stage + 1;
-            }
-            extra = false;
-            tile_step<HD, kSplitQ>(rec, valid, qa, qz, scale64, shift, st, sc ? sc + row : sc);
-        }
-        // lanes 4 g .. 4 g + 3 hold parts of head g's sums
-        float l = st.l;
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const float zero = st.zero[0] + st.zero[2];          // head g, group t
-        __syncthreads();                                     // the rings are read: they take the warps' outputs
-        float* wo = reinterpret_cast<float*>(S.ring);        // [kWarps][kHeads][HD], then the CTA's [kHeads][HD]
-        float* co = wo + kWarps * kHeads * HD;
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-            // the zeros' sums of heads 2 t and 2 t + 1
-            const float z0 = __shfl_sync(0xffffffffu, zero, 8 * t + i), z1 = __shfl_sync(0xffffffffu, zero, 8 * t + 4 + i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float* d = wo + (warp * kHeads + 2 * t) * HD + kGroup * i + 4 * g + j;
-                d[0] = fmaf(64.f, st.o[i][j >> 1][2 * (j & 1)], z0);
-                d[HD] = fmaf(64.f, st.o[i][j >> 1][2 * (j & 1) + 1], z1);
-            }
-        }
-        if (t == 0) S.wm[warp][g] = st.m, S.wl[warp][g] = l;
-        __syncthreads();
-        {
-            // warp w joins head w over the warps
-            float m = S.wm[0][warp];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) m = fmaxf(m, S.wm[w][warp]);
-            float total = 0.f, o[HD / 32];
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float f = S.wm[w][warp] == m ? 1.f : exp2_approx(S.wm[w][warp] - m);
-                total = fmaf(f, S.wl[w][warp], total);
-#pragma unroll
-                for (int d = 0; d < HD / 32; ++d) o[d] = fmaf(f, wo[(w * kHeads + warp) * HD + 32 * d + lane], o[d]);
-            }
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d) co[warp * HD + 32 * d + lane] = o[d];
-            if (lane == 0) S.m[warp] = m, S.l[warp] = total;
-        }
-        cluster.sync();
-        if (tid < heads) {
-            float m = -INFINITY, total = 0.f;
-            for (int c = 0; c < C; ++c) m = fmaxf(m, cluster.map_shared_rank(S.m, c)[tid]);
-            for (int c = 0; c < C; ++c) {
-                const float mc = cluster.map_shared_rank(S.m, c)[tid];
-                total = fmaf(mc == m ? 1.f : exp2_approx(mc - m), cluster.map_shared_rank(S.l, c)[tid], total);
-            }
-            S.fm[tid] = m;
-            S.fr[tid] = total == 0.f ? 0.f : 1.f / total;    // no score above -infinity: zeros
-        }
-        __syncthreads();
-        const int n = heads * HD, chunk = (n + C - 1) / C;
-        for (int i = rank * chunk + tid; i < min(n, (rank + 1) * chunk); i += kThreads) {
-            const int h = i / HD;
-            float o = 0.f;
-            for (int c = 0; c < C; ++c) {
-                const float mc = cluster.map_shared_rank(S.m, c)[h];
-                o = fmaf(mc == S.fm[h] ? 1.f : exp2_approx(mc - S.fm[h]), cluster.map_shared_rank(co, c)[i], o);
-            }
-            store_from_f32(a.out, q_at + i, out_kind, S.fr[h] == 0.f ? 0.f : o * S.fr[h]);
-        }
-        if (a.weights != nullptr) {                          // this CTA's rows, heads in order
-            float* w = a.weights + ((int64_t)b * nkv + kv) * a.cache.max_len;
-            const float* s0 = a.scores + ((int64_t)b * a.n_heads + kv * rep + h0) * a.cache.max_len;
-            auto add = [&](int64_t row, float v) {
-                for (int h = 0; h < heads; ++h)
-                    if (S.fr[h] != 0.f) v += exp2_approx(s0[(int64_t)h * a.cache.max_len + row] - S.fm[h]) * S.fr[h];
-                w[row] = v;
-            };
-            const int64_t r1 = min(rows, (int64_t)t1 * kTile);
-            for (int64_t row = (int64_t)t0 * kTile + tid; row < r1; row += kThreads) add(row, w[row]);
-            if (owner && tid == 0) add(rows, pass == 0 ? 0.f : w[rows]);
-        }
-        cluster.sync();                                      // the others have read this CTA's parts: the rings may be filled again
+    for (int u = 0; u < U; ++u) {
+        const int64_t row = first + u * kJoinThreads + tid;
+        if (row < n) w[row] = v[u];
     }
 }
 
@@ -539,54 +596,76 @@ int check(const rvq_cache4_attn_args* a) {
     if ((a->cos == nullptr) != (a->sin == nullptr) || (a->cos == nullptr) != (a->pos == nullptr)) return RVQ_ERR_INVALID;
     if (a->cos != nullptr && a->table_len < 1) return RVQ_ERR_INVALID;
     if (a->q.kind == RVQ_F16 && (a->q_norm != nullptr || a->cos != nullptr)) return RVQ_ERR_UNSUPPORTED;
-    if (a->weights != nullptr && a->scores == nullptr) return RVQ_ERR_INVALID;
     if (c.n_seq > 65535 || a->n_heads > 65535) return RVQ_ERR_TOO_LARGE;
     return RVQ_OK;
 }
 
-template <int HD, bool kSplitQ>
-int run(const rvq_cache4_attn_args& a, cudaStream_t s) {
-    auto* kernel = cache4_attn_kernel<HD, kSplitQ>;
-    const int smem = (int)sizeof(Smem<HD>);
+// Ranges of the rows: as many CTAs as the SMs hold (two each), but none shorter than a tile for every warp of a full cache.
+int plan(const rvq_cache4_attn_args& a, int* splits) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return status(e);
     const int rep = a.n_heads / a.cache.n_kv, groups = (rep + kHeads - 1) / kHeads;
-    const int passes = a.weights != nullptr ? groups : 1;
-    const int64_t units = (int64_t)a.cache.n_seq * a.cache.n_kv * (groups / passes);
-    int c = 1;
-    while (c < 16 && units * c * 2 <= 2 * sms && (int64_t)c * kWarps * kTile < a.cache.max_len) c *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(c, a.cache.n_kv * (groups / passes), a.cache.n_seq);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = c;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return status(cudaLaunchKernelEx(&cfg, kernel, a, passes));
+    const int64_t units = (int64_t)a.cache.n_seq * a.cache.n_kv * groups;
+    const int64_t most = 2 * sms / units, parts = (a.cache.max_len + kWarps * kTile - 1) / (kWarps * kTile);
+    const int64_t s = most < parts ? most : parts;
+    *splits = s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : (int)s;
+    return RVQ_OK;
+}
+
+// Bytes of the workspace's parts: maxima and sums, outputs, scores.
+void sizes(const rvq_cache4_attn_args& a, int splits, size_t (&n)[3]) {
+    const size_t heads = (size_t)a.cache.n_seq * a.n_heads;
+    n[0] = (heads * splits * sizeof(float2) + 15) / 16 * 16;
+    n[1] = splits > 1 ? heads * splits * a.cache.head_dim * sizeof(float) : 0;
+    n[2] = a.weights != nullptr ? heads * a.cache.max_len * sizeof(float) : 0;
+}
+
+template <int HD, bool kSplitQ>
+int run(const rvq_cache4_attn_args& a, const Work& work, cudaStream_t s) {
+    auto* kernel = cache4_attn_kernel<HD, kSplitQ>;
+    const int smem = (int)sizeof(Smem<HD>), rep = a.n_heads / a.cache.n_kv, groups = (rep + kHeads - 1) / kHeads;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+        e = launch_pdl(kernel, dim3(work.splits, a.cache.n_kv * groups, a.cache.n_seq), dim3(kThreads), (size_t)smem, s, a, work);
+    const int out_blocks = work.splits > 1 ? (rep * HD + kJoinThreads - 1) / kJoinThreads : 0;
+    const int row_blocks = a.weights != nullptr ? (a.cache.max_len + kJoinRows - 1) / kJoinRows : 0;
+    if (e == cudaSuccess && out_blocks + row_blocks > 0)
+        e = launch_pdl(cache4_join_kernel, dim3(out_blocks + row_blocks, a.cache.n_kv, a.cache.n_seq), dim3(kJoinThreads), 0, s, a,
+                       work, out_blocks);
+    return status(e);
 }
 
 }  // namespace cache4
-
 }  // namespace rvq
 
 using namespace rvq;
 using namespace rvq::cache4;
 
-extern "C" int rvq_cache4_attention(const rvq_cache4_attn_args* a, void* stream) {
-    const int rc = check(a);
+extern "C" size_t rvq_cache4_attention_workspace_size(const rvq_cache4_attn_args* a) {
+    int splits = 1;
+    if (check(a) != RVQ_OK || plan(*a, &splits) != RVQ_OK) return 0;
+    size_t n[3];
+    sizes(*a, splits, n);
+    return n[0] + n[1] + n[2];
+}
+
+extern "C" int rvq_cache4_attention(const rvq_cache4_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check(a);
     if (rc != RVQ_OK) return rc;
+    Work work;
+    rc = plan(*a, &work.splits);
+    if (rc != RVQ_OK) return rc;
+    size_t n[3];
+    sizes(*a, work.splits, n);
+    if (workspace == nullptr || workspace_bytes < n[0] + n[1] + n[2] || ((uintptr_t)workspace & 15)) return RVQ_ERR_INVALID;
+    uint8_t* p = reinterpret_cast<uint8_t*>(workspace);
+    work.ml = reinterpret_cast<float2*>(p);
+    work.o = reinterpret_cast<float*>(p + n[0]);
+    work.scores = reinterpret_cast<float*>(p + n[0] + n[1]);
     cudaStream_t s = (cudaStream_t)stream;
     const bool split = a->q.kind == RVQ_F16;
-    if (a->cache.head_dim == 128) return split ? run<128, true>(*a, s) : run<128, false>(*a, s);
-    return split ? run<64, true>(*a, s) : run<64, false>(*a, s);
+    if (a->cache.head_dim == 128) return split ? run<128, true>(*a, work, s) : run<128, false>(*a, work, s);
+    return split ? run<64, true>(*a, work, s) : run<64, false>(*a, work, s);
 }

@@ -25,7 +25,7 @@ def test_struct_layouts():
     assert ctypes.sizeof(attention.RvqCache4) == 8 + 4 * 4
     assert ctypes.sizeof(attention.RvqPromptAttnArgs) == 7 * 8 + 2 * 8 + 8 * 8 + 8 * 4
     assert ctypes.sizeof(attention.RvqCache4RowsArgs) == 24 + 4 * 8 + 8 + 4 * 8 + 2 * 4
-    assert ctypes.sizeof(attention.RvqCache4AttnArgs) == 3 * 24 + 5 * 8 + 24 + 4 * 8 + 4 * 4
+    assert ctypes.sizeof(attention.RvqCache4AttnArgs) == 3 * 24 + 5 * 8 + 24 + 3 * 8 + 4 * 4
     assert ctypes.sizeof(attention.RvqCache4EvictArgs) == 2 * 24 + 5 * 8 + 2 * 4
     assert attention.record_bytes(128) == 160 and attention.record_bytes(64) == 80
     with pytest.raises(NotImplementedError):
@@ -294,17 +294,16 @@ def test_c_step_checks():
 
     def call(**kw):
         a = attention.RvqCache4AttnArgs(RvqVec(16, 512, 1, B), RvqVec(16, 256, 1, B), RvqVec(16, 256, 1, B), None, None,
-                                        None, None, None, c_cache(), 16, 16, None, None, 4, 0, 1e-6, 1.0)
+                                        None, None, None, c_cache(), 16, 16, None, 4, 0, 1e-6, 1.0)
         for name, v in kw.items():
             setattr(a, name, v)
-        return lib.rvq_cache4_attention(ctypes.byref(a), None)
-    assert lib.rvq_cache4_attention(None, None) == INV
+        return lib.rvq_cache4_attention(ctypes.byref(a), None, 0, None)
+    assert lib.rvq_cache4_attention(None, None, 0, None) == INV
     assert call(cache=c_cache(data=None)) == INV and call(cache=c_cache(head_dim=80)) == UNS and call(rows=None) == INV
     assert call(n_heads=3) == INV and call(n_heads=130, q=RvqVec(16, 2 * 130 * 64, 1, B)) == UNS
     assert call(q=RvqVec(16, 511, 1, B)) == INV and call(k=RvqVec(None, 0, 0, 0)) == INV
     assert call(k=RvqVec(16, 256, 1, _native.RVQ_F16)) == INV and call(q_norm=16) == INV and call(cos=16, sin=16) == INV
     assert call(cos=16, sin=16, pos=16) == INV                                  # table_len 0
-    assert call(weights=16) == INV                                              # no scores
     H = _native.RVQ_F16
     assert call(q=RvqVec(16, 512, 1, H), k=RvqVec(16, 256, 1, H), v=RvqVec(16, 256, 1, H), q_norm=16, k_norm=16) == UNS
 

@@ -104,16 +104,23 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-// What a warp carries over its tiles.  Lane 4 g + t: head g's maximum and this lane's part of its sum; of the sums of
-// p zero and p step, those of group t for head g (and the parts from p's remainder); and of the output, transposed: heads
-// 2 t and 2 t + 1, value 4 g + i of group G in o[G][i / 2][2 (i & 1) + (0, 1)].
+// What a warp carries over its tiles.  Lane 4 g + t has heads 2 t and 2 t + 1 everywhere: their maxima and the parts of
+// their sums from rows g and g + 8; the sums of p times halfword g of the parameters (zero of group g / 2 for even g) in
+// zero[0] and [1]; and of the output, transposed, value 4 g + i of group G in o[G][i / 2][2 (i & 1) + (0, 1)].
 template <int HD>
 struct State {
     static constexpr int G = HD / kGroup;
-    float m, l;
+    float m[2], l[2];
     float zero[4];
     float o[G][2][4];
 };
+
+// The 8 x 8 matrix of 16-bit values of which lane 4 g + t holds row g, columns 2 t and 2 t + 1, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
 template <int G>
 __device__ __forceinline__ void load_words(uint32_t (&w)[G], uint32_t addr) {
@@ -123,102 +130,123 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[G], uint32_t addr) {
         asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
 }
 
-// A tile of 16 rows, `valid` of them live (the records behind those hold zeros).
+// A tile of 16 rows, `valid` of them live (the records behind those hold zeros).  The rows are the M of the scores'
+// MMA and the K of the output's, the heads the N of both; between the two the probabilities, heads along the lanes'
+// registers, are transposed to rows along them.
 template <int HD, bool kSplitQ>
 __device__ __forceinline__ void tile_step(uint32_t base, int valid, const uint32_t (&qa)[HD / 16][kSplitQ ? 4 : 2],
                                           const uint32_t (&qz)[3], float scale64, uint32_t shift, State<HD>& st,
-                                          float* scores) {
+                                          float* const (&scores)[2]) {
     constexpr int G = HD / kGroup, REC = record_bytes(HD), kLo = kSplitQ ? 2 : 0;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    // columns n of a score tile hold row (n with its two low bits swapped): a quarter warp's 16-byte loads of two
-    // rows then fall into different banks, and this lane's columns 2 t and 2 t + 1 are rows ra and ra + 2
+    // row g of an MMA is row (g with its two low bits swapped) of the tile: a quarter warp's 16-byte loads of two rows then
+    // fall into different banks; rows 2 t and 2 t + 1 are so ra and ra + 2
     const int rn = (g & 4) | (g & 1) << 1 | (g >> 1 & 1);
     const int ra = (t >> 1) * 4 + (t & 1);
-    float s[4];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const uint32_t rk = base + (8 * n + rn) * REC, r0 = base + (8 * n + ra) * REC + HD;
-        uint32_t kc[G], pa[G], pb[G], pz;
-        load_words<G>(kc, rk + 4 * G * t);
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pz) : "r"(rk + HD + 4 * (t & (G - 1))));
-        load_words<G>(pa, r0);
-        load_words<G>(pb, r0 + 2 * REC);
+    const uint32_t r0 = base + rn * REC, r1 = r0 + 8 * REC;
+    float s[4];                                              // rows rn (heads 2 t, 2 t + 1) and rn + 8
+    {
+        uint32_t k0[G], k1[G], p0[G], p1[G], z0, z1;
+        load_words<G>(k0, r0 + 4 * G * t);
+        load_words<G>(k1, r1 + 4 * G * t);
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(z0) : "r"(r0 + HD + 4 * (t & (G - 1))));
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(z1) : "r"(r1 + HD + 4 * (t & (G - 1))));
+        load_words<G>(p0, r0 + HD);
+        load_words<G>(p1, r1 + HD);
         float z[4], c[G][4];                                 // zero . (q . 1) / 64; q . c / 64 of every group
-        mma_set(z, qz[0], qz[2], qz[1], 0u, pz, pz);
+        mma_set(z, z0, z1, z0, z1, qz[0], qz[1]);
 #pragma unroll
         for (int i = 0; i < G; ++i)
-            mma_set(c[i], qa[2 * i][0], kSplitQ ? qa[2 * i][kLo] : 0u, qa[2 * i][1], kSplitQ ? qa[2 * i][kLo + 1] : 0u,
-                    code_pair<0>(kc[i]), code_pair<1>(kc[i]));
+            mma_set(c[i], code_pair<0>(k0[i]), code_pair<0>(k1[i]), code_pair<1>(k0[i]), code_pair<1>(k1[i]), qa[2 * i][0], qa[2 * i][1]);
+        if constexpr (kSplitQ) {
 #pragma unroll
-        for (int i = 0; i < G; ++i)
-            mma_add(c[i], qa[2 * i + 1][0], kSplitQ ? qa[2 * i + 1][kLo] : 0u, qa[2 * i + 1][1],
-                    kSplitQ ? qa[2 * i + 1][kLo + 1] : 0u, code_pair<0>(kc[i] >> 8), code_pair<1>(kc[i] >> 8));
-        float sa = z[0] + z[2], sb = z[1] + z[3];
+            for (int i = 0; i < G; ++i)
+                mma_add(c[i], code_pair<0>(k0[i]), code_pair<0>(k1[i]), code_pair<1>(k0[i]), code_pair<1>(k1[i]), qa[2 * i][kLo], qa[2 * i][kLo + 1]);
+        }
+        mma_add(z, z0, z1, z0, z1, qz[2], 0u);
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            if constexpr (kSplitQ) c[i][0] += c[i][2], c[i][1] += c[i][3];
-            sa = fmaf(step_of(pa[i]), c[i][0], sa);
-            sb = fmaf(step_of(pb[i]), c[i][1], sb);
+            k0[i] >>= 8, k1[i] >>= 8;
+            mma_add(c[i], code_pair<0>(k0[i]), code_pair<0>(k1[i]), code_pair<1>(k0[i]), code_pair<1>(k1[i]), qa[2 * i + 1][0], qa[2 * i + 1][1]);
         }
-        s[2 * n] = sa * scale64;
-        s[2 * n + 1] = sb * scale64;
+        if constexpr (kSplitQ) {
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+                mma_add(c[i], code_pair<0>(k0[i]), code_pair<0>(k1[i]), code_pair<1>(k0[i]), code_pair<1>(k1[i]), qa[2 * i + 1][kLo], qa[2 * i + 1][kLo + 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            const float x = step_of(p0[i]), y = step_of(p1[i]);
+            z[0] = fmaf(x, c[i][0], z[0]), z[1] = fmaf(x, c[i][1], z[1]);
+            z[2] = fmaf(y, c[i][2], z[2]), z[3] = fmaf(y, c[i][3], z[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = z[i] * scale64;
     }
     if (valid < 16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (8 * (i >> 1) + ra + 2 * (i & 1) >= valid) s[i] = -INFINITY;
+        if (rn >= valid) s[0] = s[1] = -INFINITY;
+        if (rn + 8 >= valid) s[2] = s[3] = -INFINITY;
     }
-    if (scores != nullptr) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = 8 * (i >> 1) + ra + 2 * (i & 1);
-            if (row < valid) scores[row] = s[i];
+    for (int i = 0; i < 4; ++i)
+        if (scores[i & 1] != nullptr && rn + 8 * (i >> 1) < valid) scores[i & 1][rn + 8 * (i >> 1)] = s[i];
+    // the maximum that is subtracted follows the true one only when that has grown by 2^8 (p stays below 2^8): of 16
+    // rows and 8 heads some has a new maximum in most tiles
+    float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
+    if (__any_sync(0xffffffffu, top0 > st.m[0] + kGrow || top1 > st.m[1] + kGrow)) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
+            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
         }
-    }
-    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    // the maximum that is subtracted follows the true one only when that has grown by 2^8 (p stays below 2^8): of 32
-    // rows and heads some has a new maximum in most tiles, and following it at once costs a fifth of the loop
-    if (__any_sync(0xffffffffu, top > st.m + kGrow)) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float m = fmaxf(st.m, top);
-        const float f = st.m == m ? 1.f : exp2_approx(st.m - m);
-        st.m = m;
-        st.l *= f;
+        float f[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st.zero[i] *= f;
-        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+        for (int i = 0; i < 2; ++i) {
+            const float m = fmaxf(st.m[i], i ? top1 : top0);
+            f[i] = st.m[i] == m ? 1.f : exp2_approx(st.m[i] - m);
+            st.m[i] = m;
+            st.l[i] *= f[i];
+            st.zero[i] *= f[i];
+        }
 #pragma unroll
         for (int i = 0; i < G; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                st.o[i][j][0] *= f0, st.o[i][j][2] *= f0;
-                st.o[i][j][1] *= f1, st.o[i][j][3] *= f1;
-            }
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) st.o[i][j][c] *= f[c & 1];
     }
     // nothing but -infinities so far: p = exp(-infinity) = 0, not exp(-infinity + infinity)
-    const float sub = st.m == -INFINITY ? 0.f : st.m;
+    const float sub0 = st.m[0] == -INFINITY ? 0.f : st.m[0], sub1 = st.m[1] == -INFINITY ? 0.f : st.m[1];
     float p[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = exp2_approx(s[i] - sub);
-    st.l += (p[0] + p[1]) + (p[2] + p[3]);
-    uint32_t vc[4][G], vp[4][G], h[4], zs[4];
+    for (int i = 0; i < 4; ++i) p[i] = exp2_approx(s[i] - (i & 1 ? sub1 : sub0));
+    st.l[0] += p[0] + p[2];
+    st.l[1] += p[1] + p[3];
+    uint32_t vc[4][G], p0[G], p1[G], h[4], zs[4];
+    load_words<G>(p0, r0 + HD + HD / 8);
+    load_words<G>(p1, r1 + HD + HD / 8);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t r = base + (8 * (i >> 1) + ra + 2 * (i & 1)) * REC + HD / 2;
         load_words<G>(vc[i], r + 4 * G * (g >> 1));
-        load_words<G>(vp[i], r + HD / 2 + HD / 8);
         asm volatile("ld.shared.u16 %0, [%1];" : "=r"(zs[i]) : "r"(r + HD / 2 + HD / 8 + 2 * (g & (2 * G - 1))));
     }
-    // sums of p zero (columns 2 group) and p step (2 group + 1)
-    split_bf16(p[0], p[1], &h[0], &h[1], shift);
-    split_bf16(p[2], p[3], &h[2], &h[3], shift);
-    mma_add(st.zero, h[0], h[1], h[2], h[3], __byte_perm(zs[0], zs[1], 0x5410u), __byte_perm(zs[2], zs[3], 0x5410u));
+    // two parts of (x, y) in rows rn and of (u, v) in rows rn + 8, transposed: {part 0, part 1} of rows ra and ra + 2, then + 8
+    auto operand = [&](float x, float y, float u, float v) {
+        split_bf16(x, y, &h[0], &h[1], shift);
+        split_bf16(u, v, &h[2], &h[3], shift);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = transpose8(h[i]);
+    };
+    operand(p[0], p[1], p[2], p[3]);
+    const uint32_t za = __byte_perm(zs[0], zs[1], 0x5410u), zb = __byte_perm(zs[2], zs[3], 0x5410u);
+    mma_add(st.zero, za, 0u, zb, 0u, h[0], h[2]);
+    mma_add(st.zero, za, 0u, zb, 0u, h[1], h[3]);
     const uint32_t half_sel = g & 1 ? 0x7632u : 0x5410u;     // this lane's 4 values are half a code word
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-        split_bf16(p[0] * step_of(vp[0][i]), p[1] * step_of(vp[1][i]), &h[0], &h[1], shift);
-        split_bf16(p[2] * step_of(vp[2][i]), p[3] * step_of(vp[3][i]), &h[2], &h[3], shift);
+        const float x = step_of(p0[i]), y = step_of(p1[i]);
+        operand(p[0] * x, p[1] * x, p[2] * y, p[3] * y);
         const uint32_t w0 = __byte_perm(vc[0][i], vc[1][i], half_sel), w1 = __byte_perm(vc[2][i], vc[3][i], half_sel);
         const uint32_t v0 = code_pair<0>(w0), v1 = code_pair<1>(w0), v2 = code_pair<0>(w1), v3 = code_pair<1>(w1);
         const uint32_t x0 = code_pair<0>(w0 >> 8), x1 = code_pair<1>(w0 >> 8);
@@ -385,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
     if (owner && group == 0 && tid < REC / 16)
         reinterpret_cast<uint4*>(cache + rows * REC)[tid] = reinterpret_cast<const uint4*>(S.fresh)[tid];
 
-    // operand rows 0..7: q (its bf16 part), rows 8..15: the remainder; column pairs in the code words' order
+    // column g of the operand: q of head g (its bf16 part, then the remainder), in pairs in the code words' order
     uint32_t qa[HD / 16][kSplitQ ? 4 : 2];
     // (q . 1) / 64 of group t against the pairs (zero, step), in three bf16 parts: 24 bits
     uint32_t qz[3] = {0u, 0u, 0u};
@@ -406,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
         }
     }
     State<HD> st;
-    st.m = -INFINITY, st.l = 0.f;
+    st.m[0] = st.m[1] = -INFINITY, st.l[0] = st.l[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) st.zero[i] = 0.f;
 #pragma unroll
@@ -416,7 +444,10 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
 #pragma unroll
             for (int c = 0; c < 4; ++c) st.o[i][j][c] = 0.f;
     const float scale64 = a.scaling * 64.f * 1.4426950408889634f;      // scores in powers of two
-    float* sc = a.weights != nullptr && g < heads ? work.scores + (head0 + g) * a.cache.max_len : nullptr;
+    float* sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        sc[i] = a.weights != nullptr && 2 * t + i < heads ? work.scores + (head0 + 2 * t + i) * a.cache.max_len : nullptr;
     // the last warp begins with the appended record
     bool extra = owner && warp == kWarps - 1;
     for (int tile = t0 + warp, stage = 0; tile < t1 || extra;) {
@@ -433,20 +464,22 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
         extra = false;
-        tile_step<HD, kSplitQ>(rec, valid, qa, qz, scale64, shift, st, sc ? sc + row : sc);
+        float* const at[2] = {sc[0] ? sc[0] + row : nullptr, sc[1] ? sc[1] + row : nullptr};
+        tile_step<HD, kSplitQ>(rec, valid, qa, qz, scale64, shift, st, at);
     }
-    // lanes 4 g .. 4 g + 3 hold parts of head g's sum
-    float l = st.l;
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    const float zero = st.zero[0] + st.zero[2];              // head g, group t
+    // the lanes with the same t hold parts of heads 2 t and 2 t + 1
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+        st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], o);
+        st.l[1] += __shfl_xor_sync(0xffffffffu, st.l[1], o);
+    }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     __syncthreads();                                         // the rings are read: they take the warps' outputs
     float* wo = reinterpret_cast<float*>(S.ring);            // [kWarps][kHeads][HD]
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-        // the zeros' sums of heads 2 t and 2 t + 1
-        const float z0 = __shfl_sync(0xffffffffu, zero, 8 * t + i), z1 = __shfl_sync(0xffffffffu, zero, 8 * t + 4 + i);
+        // the sums with the group's zeros
+        const float z0 = __shfl_sync(0xffffffffu, st.zero[0], 8 * i + t), z1 = __shfl_sync(0xffffffffu, st.zero[1], 8 * i + t);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float* d = wo + (warp * kHeads + 2 * t) * HD + kGroup * i + 4 * g + j;
@@ -454,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
             d[HD] = fmaf(64.f, st.o[i][j >> 1][2 * (j & 1) + 1], z1);
         }
     }
-    if (t == 0) S.wm[warp][g] = st.m, S.wl[warp][g] = l;
+    if (g < 2) S.wm[warp][2 * t + g] = g ? st.m[1] : st.m[0], S.wl[warp][2 * t + g] = g ? st.l[1] : st.l[0];
     __syncthreads();
     // warp w joins head w over the warps
     if (warp >= heads) return;

@@ -136,7 +136,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[G], uint32_t addr) {
 template <int HD, bool kSplitQ>
 __device__ __forceinline__ void tile_step(uint32_t base, int valid, const uint32_t (&qa)[HD / 16][kSplitQ ? 4 : 2],
                                           const uint32_t (&qz)[3], float scale64, uint32_t shift, State<HD>& st,
-                                          float* const (&scores)[2]) {
+                                          bool keep, float* const (&scores)[2]) {
     constexpr int G = HD / kGroup, REC = record_bytes(HD), kLo = kSplitQ ? 2 : 0;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // row g of an MMA is row (g with its two low bits swapped) of the tile: a quarter warp's 16-byte loads of two rows then
@@ -187,9 +187,11 @@ __device__ __forceinline__ void tile_step(uint32_t base, int valid, const uint32
         if (rn >= valid) s[0] = s[1] = -INFINITY;
         if (rn + 8 >= valid) s[2] = s[3] = -INFINITY;
     }
+    if (keep) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (scores[i & 1] != nullptr && rn + 8 * (i >> 1) < valid) scores[i & 1][rn + 8 * (i >> 1)] = s[i];
+        for (int i = 0; i < 4; ++i)
+            if (scores[i & 1] != nullptr && rn + 8 * (i >> 1) < valid) scores[i & 1][rn + 8 * (i >> 1)] = s[i];
+    }
     // the maximum that is subtracted follows the true one only when that has grown by 2^8 (p stays below 2^8): of 16
     // rows and 8 heads some has a new maximum in most tiles
     float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
@@ -320,13 +322,11 @@ struct Work {
     int32_t splits;
 };
 
-// Whether the sequence has something to attend to: 1; zeros in its output: 0; left alone: -1.
-__device__ __forceinline__ int state_of(const rvq_cache4_attn_args& a, int b, int64_t* rows) {
-    *rows = a.rows[b];
-    if (*rows < 0) return -1;
+// Whether a sequence has something to attend to: 1; zeros in its output: 0; left alone: -1.
+__device__ __forceinline__ int state_of(const rvq_cache4_attn_args& a, int64_t rows, int64_t pos) {
+    if (rows < 0) return -1;
     const bool append = a.k.ptr != nullptr;
-    const int64_t pos = a.pos != nullptr ? a.pos[b] : 0;
-    return *rows + append >= 1 && *rows + append <= a.cache.max_len && pos >= 0 && (a.pos == nullptr || pos < a.table_len);
+    return rows + append >= 1 && rows + append <= a.cache.max_len && pos >= 0 && (a.pos == nullptr || pos < a.table_len);
 }
 
 template <int HD, bool kSplitQ>
@@ -339,13 +339,17 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
     const int split = blockIdx.x, kv = blockIdx.y % nkv, group = blockIdx.y / nkv, b = blockIdx.z;
     pdl_launch_dependents();
     pdl_wait();
-    int64_t rows;
-    const int state = state_of(a, b, &rows);
-    if (state < 0) return;
+    const int64_t rows = a.rows[b], pos = a.pos != nullptr ? a.pos[b] : 0;
     const bool append = a.k.ptr != nullptr;
     const int groups = (rep + kHeads - 1) / kHeads, per = (rep + groups - 1) / groups;
     const int h0 = group * per, heads = min(per, rep - h0);
     const int64_t head0 = (int64_t)b * a.n_heads + kv * rep + h0, q_at = head0 * HD;      // of all sequences' heads
+    float qv[kHeads * HD / kThreads];                        // on their way while rows is
+#pragma unroll
+    for (int i = 0; i < kHeads * HD / kThreads; ++i)
+        qv[i] = tid + i * kThreads < heads * HD ? vec_value_deep(a.q, q_at + tid + i * kThreads) : 0.f;
+    const int state = state_of(a, rows, pos);
+    if (state < 0) return;
     const int out_kind = a.q.kind == RVQ_F16 ? RVQ_F16 : RVQ_BF16;
     if (state == 0) {
         if (split == 0)
@@ -369,11 +373,15 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
     auto fetch = [&](int tile, int stage) {
         if (tile < t1) {
             const uint8_t* src = cache + (int64_t)tile * (kTile * REC) + 16 * lane;
-            const int bytes = (live - tile * kTile) * REC - 16 * lane;
+            const uint32_t dst = ring + stage * (kTile * REC);
+            const int bytes = (live - tile * kTile) * REC - 16 * lane;      // of live rows, from this lane's first piece on
+            const bool full = (tile + 1) * kTile <= live;
 #pragma unroll
             for (int i = 0; i < (kTile * REC + 511) / 512; ++i)
-                if ((i + 1) * 512 <= kTile * REC || lane < kTile * REC % 512 / 16)
-                    copy16(ring + stage * (kTile * REC) + 512 * i, bytes > 512 * i ? src + 512 * i : cache, bytes > 512 * i);
+                if ((i + 1) * 512 <= kTile * REC || lane < kTile * REC % 512 / 16) {
+                    if (full) copy16(dst + 512 * i, src + 512 * i, true);
+                    else copy16(dst + 512 * i, bytes > 512 * i ? src + 512 * i : cache, bytes > 512 * i);
+                }
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
@@ -382,7 +390,6 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
     // the heads' q, and the new record
     const bool rotate = a.q_norm != nullptr || a.cos != nullptr;
     if (rotate) {
-        const int64_t pos = a.pos != nullptr ? a.pos[b] : 0;
         for (int i = tid; i < HD; i += kThreads) {
             S.norm[0][i] = a.q_norm != nullptr ? bf16_at(a.q_norm, i) : 0.f;
             S.norm[1][i] = a.q_norm != nullptr ? bf16_at(a.k_norm, i) : 0.f;
@@ -390,8 +397,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
             S.norm[3][i] = a.cos != nullptr ? bf16_at(a.sin, pos * HD + i) : 0.f;
         }
     }
-    for (int i = tid; i < kHeads * HD; i += kThreads)
-        (&S.q[0][0])[i] = i < heads * HD ? vec_value_deep(a.q, q_at + i) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kHeads * HD / kThreads; ++i) (&S.q[0][0])[tid + i * kThreads] = qv[i];
     if (owner) {
         const int64_t kv_at = ((int64_t)b * nkv + kv) * HD;
         for (int i = tid; i < 2 * HD; i += kThreads) (&S.kv[0][0])[i] = vec_value_deep(i < HD ? a.k : a.v, kv_at + i % HD);
@@ -465,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
         }
         extra = false;
         float* const at[2] = {sc[0] ? sc[0] + row : nullptr, sc[1] ? sc[1] + row : nullptr};
-        tile_step<HD, kSplitQ>(rec, valid, qa, qz, scale64, shift, st, at);
+        tile_step<HD, kSplitQ>(rec, valid, qa, qz, scale64, shift, st, a.weights != nullptr, at);
     }
     // the lanes with the same t hold parts of heads 2 t and 2 t + 1
 #pragma unroll
@@ -552,19 +559,19 @@ __global__ void __launch_bounds__(kJoinThreads) cache4_join_kernel(rvq_cache4_at
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkv = a.cache.n_kv, rep = a.n_heads / nkv, hd = a.cache.head_dim;
     const int kv = blockIdx.y, b = blockIdx.z;
-    int64_t rows;
-    if (state_of(a, b, &rows) != 1) return;
+    const int64_t rows = a.rows[b], pos = a.pos != nullptr ? a.pos[b] : 0;
     const int64_t head0 = (int64_t)b * a.n_heads + kv * rep, all = (int64_t)a.cache.n_seq * a.n_heads;
     const bool append = a.k.ptr != nullptr;
     const int64_t n = rows + append, first = (int64_t)((int)blockIdx.x - out_blocks) * kJoinRows;
-    if (first >= n) return;
     const bool output = first < 0;
+    if (!output && first >= n) return;
     const int h0 = output ? blockIdx.x * (kJoinThreads / hd) : 0, h1 = output ? min(rep, h0 + kJoinThreads / hd) : rep;
     for (int h = h0 + warp; h < h1; h += kJoinThreads / 32) {
         const float2 x = join_head(work.ml + head0 + h, all, work.splits, output ? f[h - h0] : nullptr);
         if (lane == 0) fm[h] = x.x, fr[h] = x.y == 0.f ? 0.f : 1.f / x.y;
     }
     __syncthreads();
+    if (state_of(a, rows, pos) != 1) return;                 // (what was joined then is not used)
     if (output) {
         const int i = blockIdx.x * kJoinThreads + tid, h = i / hd;
         if (i >= rep * hd) return;

@@ -63,15 +63,17 @@ __global__ void __launch_bounds__(kRowsThreads) cache4_rows_kernel(rvq_cache4_ro
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
         const int64_t tok = ((int64_t)blockIdx.x * kTokens + u) * B + threadIdx.x / T;
-        row_ok[u] = false;
-        rec[u] = tok < a.tokens ? record_of(a, tok, g, record_bytes(HD), &row_ok[u]) : nullptr;
         x[u] = reinterpret_cast<uint4*>(base + tok * st[0]);
         raw[u] = make_uint4(0, 0, 0, 0);
+        if (kWrite && tok < a.tokens) raw[u] = *x[u];        // on its way while the row is looked up
+    }
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+        const int64_t tok = ((int64_t)blockIdx.x * kTokens + u) * B + threadIdx.x / T;
+        row_ok[u] = false;
+        rec[u] = tok < a.tokens ? record_of(a, tok, g, record_bytes(HD), &row_ok[u]) : nullptr;
         word[u] = par[u] = 0;
-        if (rec[u] == nullptr) continue;
-        if constexpr (kWrite) {
-            raw[u] = *x[u];
-        } else if (row_ok[u]) {
+        if (!kWrite && rec[u] != nullptr && row_ok[u]) {
             word[u] = *(reinterpret_cast<uint32_t*>(rec[u] + which * (HD / 2)) + w * G + grp);
             par[u] = *(reinterpret_cast<uint32_t*>(rec[u] + HD + which * (HD / 8)) + grp);
         }
@@ -80,12 +82,13 @@ __global__ void __launch_bounds__(kRowsThreads) cache4_rows_kernel(rvq_cache4_ro
     for (int u = 0; u < kTokens; ++u) {
         if constexpr (kWrite) {
             const uint32_t r[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            auto value = [&](uint32_t w, int i) {
+                const uint16_t h = (uint16_t)(w >> (16 * (i & 1)));
+                return a.kind == RVQ_F16 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
+            };
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint16_t h = (uint16_t)(r[i / 2] >> (16 * (i & 1)));
-                v[i] = a.kind == RVQ_F16 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
-            }
+            for (int i = 0; i < 8; ++i) v[i] = value(r[i / 2], i);
             float lo = v[0], hi = v[0];
 #pragma unroll
             for (int i = 1; i < 8; ++i) lo = min_nan(lo, v[i]), hi = max_nan(hi, v[i]);
@@ -96,8 +99,19 @@ __global__ void __launch_bounds__(kRowsThreads) cache4_rows_kernel(rvq_cache4_ro
             }
             const uint32_t p = params_of(lo, hi);
             const float zero = zero_of(p), step = step_of(p), inv = 1.0f / step;
+            uint32_t again = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) word[u] |= code_of(v[i], zero, step, inv) << (4 * i);
+            for (int i = 0; i < 8; ++i) {
+                bool near;
+                word[u] |= code_near(v[i], zero, step, inv, &near) << (4 * i);
+                again |= (uint32_t)near << i;
+            }
+            while (again) {                                  // few: these divide
+                const int i = __ffs(again) - 1;
+                again &= again - 1;
+                const float x = value(i < 4 ? i < 2 ? r[0] : r[1] : i < 6 ? r[2] : r[3], i);
+                word[u] = (word[u] & ~(15u << (4 * i))) | code_of(x, zero, step) << (4 * i);
+            }
             if (rec[u] != nullptr && row_ok[u]) {
                 *(reinterpret_cast<uint32_t*>(rec[u] + which * (HD / 2)) + w * G + grp) = word[u];
                 if (w == 0) *(reinterpret_cast<uint32_t*>(rec[u] + HD + which * (HD / 8)) + grp) = p;
@@ -115,14 +129,17 @@ __global__ void __launch_bounds__(kRowsThreads) cache4_rows_kernel(rvq_cache4_ro
 
 // ---------------------------------------------------------------------------
 // Eviction.  select: a CTA per (sequence, kv head) finds the (keep - recent)-th
-// largest weight of the older rows, 8 bits of it a pass by a histogram in shared
-// memory, then writes the kept rows' indices in order (each warp a contiguous
+// largest weight of the older rows, 11, 11 and 10 bits of it a pass by a histogram
+// in shared memory (and no further than it takes to tell the wanted rows from the
+// others), then writes the kept rows' indices in order (each warp a contiguous
 // part of the rows, whose counts are added up first) and gathers the weights.
+// Up to 8,192 rows stay in registers over the passes.
 // move: the records follow.  Rows only move down, so rows that are loaded before
 // any row behind them is stored over serve in place too.
 // ---------------------------------------------------------------------------
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kAhead = 8;                    // rows that a thread loads before it looks at them
 
 // Weights ordered as unsigned integers: -0 as 0, NaN above everything.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -137,10 +154,10 @@ __device__ __forceinline__ int64_t live_rows(const rvq_cache4_evict_args& a, int
 }
 
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(rvq_cache4_evict_args a) {
-    __shared__ int hist[256];
+    __shared__ int hist[2048];
     __shared__ int above[kEvictWarps], equal[kEvictWarps];
     __shared__ uint32_t sh_bar;
-    __shared__ int sh_want;
+    __shared__ int sh_want, sh_count;
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.x / a.cache.n_kv;
@@ -163,60 +180,73 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(rvq_cache4_
     int want = a.keep - a.recent;                           // among the keys with those bits
     const bool select = want > 0;
     if (select) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+        const bool resident = old <= kEvictThreads * kAhead;
+        float x[kAhead];
+        auto fill = [&](int base) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) x[u] = base + u * kEvictThreads + tid < old ? w[base + u * kEvictThreads + tid] : 0.f;
+        };
+        if (resident) fill(0);
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t digit = pass == 2 ? 1023u : 2047u;
+            hist[tid] = hist[tid + 1024] = 0;
             __syncthreads();
-            for (int base = 0; base < old; base += kEvictThreads) {
-                const int i = base + tid;
-                const uint32_t key = i < old ? order_key(w[i]) : 0;
-                const bool in = i < old && (key & mask) == bar;
-                // keys share their high bits: one addition for the lanes of a bin
-                const uint32_t act = __ballot_sync(0xffffffffu, in);
-                if (in) {
-                    const uint32_t bin = key >> shift & 255;
-                    const uint32_t same = __match_any_sync(act, bin);
-                    if (lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+            for (int base = 0; base < old; base += kEvictThreads * kAhead) {
+                if (!resident) fill(base);
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const uint32_t key = order_key(x[u]);
+                    if (base + u * kEvictThreads + tid < old && (key & mask) == bar) atomicAdd(&hist[key >> shift & digit], 1);
                 }
             }
             __syncthreads();
-            if (warp == 0) {
-                // the bin where the count from the top reaches want; lane l: bins 255 - 8 l .. 248 - 8 l
-                int c[8], sum = 0;
+            // the bin where the count from the top reaches want; thread t: bins 2047 - 2 t and 2046 - 2 t
+            const int c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];
+            int upto = c0 + c1;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) c[k] = hist[255 - 8 * lane - k], sum += c[k];
-                int upto = sum;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            if (lane == 31) above[warp] = upto;
+            __syncthreads();
+            int before = lane < warp ? above[lane] : 0;     // summed over the lanes: the warps before this one
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int x = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += x;
-                }
-                int before = upto - sum;
-                if (before < want && want <= upto) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        if (before < want && want <= before + c[k]) {
-                            sh_bar = bar | (uint32_t)(255 - 8 * lane - k) << shift;
-                            sh_want = want - before;
-                        }
-                        before += c[k];
-                    }
-                }
+            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+            before += upto - c0 - c1;
+            if (before < want && want <= before + c0 + c1) {
+                const bool second = want > before + c0;
+                sh_bar = bar | (uint32_t)(2047 - 2 * tid - second) << shift;
+                sh_want = want - before - (second ? c0 : 0);
+                sh_count = second ? c1 : c0;
             }
             __syncthreads();
             bar = sh_bar;
             want = sh_want;
-            mask |= 255u << shift;
+            mask |= digit << shift;
+            if (want == sh_count) {                         // every key with these bits is wanted: all above bar - 1
+                --bar;
+                want = 0;
+                break;
+            }
         }
     }
     // rows above bar, and the first `want` of those at it; each warp its part of the rows
     const int part = (n + kEvictThreads - 1) / kEvictThreads * 32;
     const int r0 = min(n, warp * part), r1 = min(n, r0 + part);
     int na = 0, ne = 0;
-    for (int base = r0; base < r1; base += 32) {
-        const int i = base + lane;
-        const uint32_t key = i < r1 && i < old ? order_key(w[i]) : 0;
-        na += __popc(__ballot_sync(0xffffffffu, i < r1 && (i >= old || (select && key > bar))));
-        ne += __popc(__ballot_sync(0xffffffffu, i < r1 && i < old && select && key == bar));
+    for (int base = r0; base < r1; base += 32 * kAhead) {
+        float x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) x[u] = base + 32 * u + lane < r1 ? w[base + 32 * u + lane] : 0.f;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = base + 32 * u + lane;
+            const uint32_t key = order_key(x[u]);
+            na += __popc(__ballot_sync(0xffffffffu, i < r1 && (i >= old || (select && key > bar))));
+            ne += __popc(__ballot_sync(0xffffffffu, i < r1 && i < old && select && key == bar));
+        }
     }
     if (lane == 0) above[warp] = na, equal[warp] = ne;
     __syncthreads();
@@ -226,20 +256,26 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(rvq_cache4_
         tied += equal[k];
     }
     pos += min(tied, want);
-    for (int base = r0; base < r1; base += 32) {
-        const int i = base + lane;
-        const uint32_t key = i < r1 && i < old ? order_key(w[i]) : 0;
-        const bool tie = i < r1 && i < old && select && key == bar;
-        const uint32_t tb = __ballot_sync(0xffffffffu, tie);
-        const uint32_t below = (1u << lane) - 1;
-        const bool keep = i < r1 && (i >= old || (select && key > bar) || (tie && tied + __popc(tb & below) < want));
-        const uint32_t kb = __ballot_sync(0xffffffffu, keep);
-        if (keep) kept[pos + __popc(kb & below)] = i;
-        pos += __popc(kb);
-        tied += __popc(tb);
+    for (int base = r0; base < r1; base += 32 * kAhead) {
+        float x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) x[u] = base + 32 * u + lane < r1 ? w[base + 32 * u + lane] : 0.f;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = base + 32 * u + lane;
+            const uint32_t key = order_key(x[u]);
+            const bool tie = i < r1 && i < old && select && key == bar;
+            const uint32_t tb = __ballot_sync(0xffffffffu, tie);
+            const uint32_t below = (1u << lane) - 1;
+            const bool keep = i < r1 && (i >= old || (select && key > bar) || (tie && tied + __popc(tb & below) < want));
+            const uint32_t kb = __ballot_sync(0xffffffffu, keep);
+            if (keep) kept[pos + __popc(kb & below)] = i;
+            pos += __popc(kb);
+            tied += __popc(tb);
+        }
     }
     __syncthreads();                                        // kept is complete, and the old weights are read
-    constexpr int U = 8;
+    constexpr int U = kAhead;
     for (int base = 0; base < a.keep; base += kEvictThreads * U) {
         float v[U];
 #pragma unroll
@@ -256,8 +292,8 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(rvq_cache4_
     }
 }
 
-constexpr int kMoveThreads = 512;
-constexpr int kMoveLoads = 8;
+constexpr int kMoveThreads = 256;
+constexpr int kMoveLoads = 4;
 
 // blockIdx.y: apart, a part of the rows; in place, a fifth of every record (its rows depend on one another, its columns do
 // not): 32 or 16 bytes wide, whole sectors of a head_dim 128 record.
@@ -381,10 +417,10 @@ extern "C" int rvq_cache4_evict(const rvq_cache4_evict_args* a, void* stream) {
     if (a->new_rows != nullptr && overlap(a->rows, 8ll * c.n_seq, a->new_rows, 8ll * c.n_seq)) return RVQ_ERR_INVALID;
     rc = status(launch_pdl(evict_select_kernel, dim3((unsigned)heads), dim3(kEvictThreads), 0, (cudaStream_t)stream, *a));
     if (rc != RVQ_OK) return rc;
-    // apart: blocks of 8 loads a thread, a few thousand of them at most; in place: the five columns
+    // apart: blocks of 4 loads a thread; in place: the five columns
     const int vecs = record_bytes(c.head_dim) / 16;
     const int64_t chunks = ((int64_t)a->keep * vecs + kMoveThreads * kMoveLoads - 1) / (kMoveThreads * kMoveLoads);
-    const unsigned parts = o.data == c.data ? 5 : (unsigned)(chunks < 64 ? chunks : 64);
+    const unsigned parts = o.data == c.data ? 5 : (unsigned)(chunks < 256 ? chunks : 256);
     auto* move = c.head_dim == 128 ? evict_move_kernel<10> : evict_move_kernel<5>;
     return status(launch_pdl(move, dim3((unsigned)heads, parts), dim3(kMoveThreads), 0, (cudaStream_t)stream, *a));
 }

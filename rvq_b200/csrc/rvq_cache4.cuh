@@ -28,18 +28,21 @@ __device__ __forceinline__ uint32_t code_of(float x, float zero, float step) {
     return step > 0.f && q > 0.f ? (uint32_t)fminf(q, 15.0f) : 0u;
 }
 
-// The same with inv = 1 / step (approximate): where the product is clearly nearer to one integer than to the next, that
-// integer is the quotient's too (|d - k s| < 0.4999 s leaves 2^-13 for the roundings of d inv, of d - k s and of the
-// quotient, 2^-22 each); only the others divide.
-__device__ __forceinline__ uint32_t code_of(float x, float zero, float step, float inv) {
-    const float d = __fsub_rn(x, zero), k = rintf(__fmul_rn(d, inv));
-    if (fabsf(fmaf(-k, step, d)) < 0.4999f * step && k < 64.f) return k > 0.f ? (uint32_t)fminf(k, 15.0f) : 0u;
-    return code_of(x, zero, step);
+// The same with inv = 1 / step (approximate), unless *near is set: where d inv is clearly nearer to one integer than to the
+// next, that integer is the quotient's too (|d - k s| < 0.4999 s leaves 2^-13 s for the roundings of inv, of d inv, of
+// d - k s and of the quotient, about 2^-22 s each).  Near the middle between two, and for a step that is 0 or not finite,
+// *near is set and the caller divides.
+__device__ __forceinline__ uint32_t code_near(float x, float zero, float step, float inv, bool* near) {
+    constexpr float kInt = 12582912.f;                       // 1.5 2^23: a sum with it ends at an integer
+    const float d = __fsub_rn(x, zero), k = __fsub_rn(fmaf(d, inv, kInt), kInt);
+    *near = !(fabsf(fmaf(-k, step, d)) < 0.4999f * step && k < 64.f);
+    return __float_as_uint(__fadd_rn(fminf(fmaxf(k, 0.f), 15.f), kInt)) & 15u;
 }
 
 // z + s c (s c is exact: 8 by 4 bits)
 __device__ __forceinline__ float value_of(uint32_t c, float zero, float step) {
-    return __fadd_rn(zero, __fmul_rn(step, (float)c));
+    const float f = __fsub_rn(__uint_as_float(0x4b000000u | c), 8388608.f);      // 2^23 + c less 2^23
+    return __fadd_rn(zero, __fmul_rn(step, f));
 }
 
 inline int status(cudaError_t e) {

@@ -640,7 +640,9 @@ int check(const rvq_cache4_attn_args* a) {
     return RVQ_OK;
 }
 
-// Ranges of the rows: as many CTAs as the SMs hold (two each), but none shorter than a tile for every warp of a full cache.
+// Ranges of the rows: as many CTAs as the SMs hold (two each), and two ranges where that is between one and two (160 heads
+// of 4,096 rows: 45 us whole, 40 us halved; of mixed lengths 38 and 26), but none shorter than a tile for every warp of a
+// full cache.  Above that a range is a whole sequence: halves cost 64 x 8 heads of 4,096 rows 113 -> 120 us.
 int plan(const rvq_cache4_attn_args& a, int* splits) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -648,7 +650,7 @@ int plan(const rvq_cache4_attn_args& a, int* splits) {
     if (e != cudaSuccess) return status(e);
     const int rep = a.n_heads / a.cache.n_kv, groups = (rep + kHeads - 1) / kHeads;
     const int64_t units = (int64_t)a.cache.n_seq * a.cache.n_kv * groups;
-    const int64_t most = 2 * sms / units, parts = (a.cache.max_len + kWarps * kTile - 1) / (kWarps * kTile);
+    const int64_t most = units > sms && units < 2 * sms ? 2 : 2 * sms / units, parts = (a.cache.max_len + kWarps * kTile - 1) / (kWarps * kTile);
     const int64_t s = most < parts ? most : parts;
     *splits = s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : (int)s;
     return RVQ_OK;

@@ -10,15 +10,39 @@ namespace cache4 {
 
 constexpr int kRowsThreads = 256;
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float d;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+// Two 16-bit minima or maxima; a NaN stays.
+template <int kKind, bool kMax>
+__device__ __forceinline__ uint32_t extreme2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (kKind == RVQ_F16) {
+        if constexpr (kMax) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    } else {
+        if constexpr (kMax) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    }
     return d;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
+
+template <int kKind>
+__device__ __forceinline__ float half_value(uint32_t w, int i) {
+    const uint16_t h = (uint16_t)(w >> (16 * (i & 1)));
+    return kKind == RVQ_F16 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
+}
+
+// The extreme of the group that four adjacent lanes hold, 8 values each.
+template <int kKind, bool kMax>
+__device__ __forceinline__ float group_extreme(const uint32_t (&r)[4]) {
+    uint32_t m = extreme2<kKind, kMax>(extreme2<kKind, kMax>(r[0], r[1]), extreme2<kKind, kMax>(r[2], r[3]));
+    m = extreme2<kKind, kMax>(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = extreme2<kKind, kMax>(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    return half_value<kKind>(extreme2<kKind, kMax>(m, m >> 16), 0);
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // Record of packed token `tok` and kv head g, or NULL where the token is in no sequence; *row_ok: the row lies in the cache.
@@ -43,10 +67,9 @@ __device__ __forceinline__ uint8_t* record_of(const rvq_cache4_rows_args& a, int
 
 // HD / 4 adjacent threads per token of the block's kv head: half of them K, half V; four adjacent ones hold a group, 8
 // values (one 16-byte load or store) each, which are one code word.  A block's tokens are neighbouring records, so code
-// words and parameters fill whole sectors; kTokens tokens a thread keep enough bytes in flight.
-constexpr int kTokens = 2;
+// words and parameters fill whole sectors.  (Two or four tokens a thread: 4,096 tokens as fast, 700 at half the speed.)
 
-template <int HD, bool kWrite>
+template <int HD, bool kWrite, int kKind>
 __global__ void __launch_bounds__(kRowsThreads) cache4_rows_kernel(rvq_cache4_rows_args a) {
     constexpr int T = HD / 4, G = HD / kGroup, B = kRowsThreads / T;
     pdl_launch_dependents();
@@ -55,75 +78,43 @@ __global__ void __launch_bounds__(kRowsThreads) cache4_rows_kernel(rvq_cache4_ro
     const int g = blockIdx.y;
     const int64_t* st = which ? a.v_stride : a.k_stride;
     uint16_t* base = reinterpret_cast<uint16_t*>(which ? a.v : a.k) + g * st[1] + grp * kGroup + 8 * w;
-    uint8_t* rec[kTokens];
-    bool row_ok[kTokens];
-    uint4* x[kTokens];
-    uint4 raw[kTokens];
-    uint32_t word[kTokens], par[kTokens];
+    const int64_t tok = (int64_t)blockIdx.x * B + threadIdx.x / T;
+    uint4* x = reinterpret_cast<uint4*>(base + tok * st[0]);
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (kWrite && tok < a.tokens) raw = *x;                  // on its way while the row is looked up
+    bool row_ok = false;
+    uint8_t* rec = tok < a.tokens ? record_of(a, tok, g, record_bytes(HD), &row_ok) : nullptr;
+    uint32_t* codes = reinterpret_cast<uint32_t*>(rec + which * (HD / 2)) + w * G + grp;
+    uint32_t* params = reinterpret_cast<uint32_t*>(rec + HD + which * (HD / 8)) + grp;
+    if constexpr (kWrite) {
+        const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+        const uint32_t p = params_of(group_extreme<kKind, false>(r), group_extreme<kKind, true>(r));
+        const float zero = zero_of(p), step = step_of(p), inv = rcp_approx(step);
+        uint32_t word = 0, again = 0;
 #pragma unroll
-    for (int u = 0; u < kTokens; ++u) {
-        const int64_t tok = ((int64_t)blockIdx.x * kTokens + u) * B + threadIdx.x / T;
-        x[u] = reinterpret_cast<uint4*>(base + tok * st[0]);
-        raw[u] = make_uint4(0, 0, 0, 0);
-        if (kWrite && tok < a.tokens) raw[u] = *x[u];        // on its way while the row is looked up
-    }
-#pragma unroll
-    for (int u = 0; u < kTokens; ++u) {
-        const int64_t tok = ((int64_t)blockIdx.x * kTokens + u) * B + threadIdx.x / T;
-        row_ok[u] = false;
-        rec[u] = tok < a.tokens ? record_of(a, tok, g, record_bytes(HD), &row_ok[u]) : nullptr;
-        word[u] = par[u] = 0;
-        if (!kWrite && rec[u] != nullptr && row_ok[u]) {
-            word[u] = *(reinterpret_cast<uint32_t*>(rec[u] + which * (HD / 2)) + w * G + grp);
-            par[u] = *(reinterpret_cast<uint32_t*>(rec[u] + HD + which * (HD / 8)) + grp);
+        for (int i = 0; i < 8; ++i) {
+            bool near;
+            word |= code_near<kKind == RVQ_F16>(half_value<kKind>(r[i / 2], i), zero, step, inv, &near) << (4 * i);
+            again |= (uint32_t)near << i;
         }
-    }
-#pragma unroll
-    for (int u = 0; u < kTokens; ++u) {
-        if constexpr (kWrite) {
-            const uint32_t r[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-            auto value = [&](uint32_t w, int i) {
-                const uint16_t h = (uint16_t)(w >> (16 * (i & 1)));
-                return a.kind == RVQ_F16 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
-            };
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = value(r[i / 2], i);
-            float lo = v[0], hi = v[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) lo = min_nan(lo, v[i]), hi = max_nan(hi, v[i]);
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            }
-            const uint32_t p = params_of(lo, hi);
-            const float zero = zero_of(p), step = step_of(p), inv = 1.0f / step;
-            uint32_t again = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                bool near;
-                word[u] |= code_near(v[i], zero, step, inv, &near) << (4 * i);
-                again |= (uint32_t)near << i;
-            }
-            while (again) {                                  // few: these divide
-                const int i = __ffs(again) - 1;
-                again &= again - 1;
-                const float x = value(i < 4 ? i < 2 ? r[0] : r[1] : i < 6 ? r[2] : r[3], i);
-                word[u] = (word[u] & ~(15u << (4 * i))) | code_of(x, zero, step) << (4 * i);
-            }
-            if (rec[u] != nullptr && row_ok[u]) {
-                *(reinterpret_cast<uint32_t*>(rec[u] + which * (HD / 2)) + w * G + grp) = word[u];
-                if (w == 0) *(reinterpret_cast<uint32_t*>(rec[u] + HD + which * (HD / 8)) + grp) = p;
-            }
-        } else if (rec[u] != nullptr) {
-            uint32_t o[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                o[i] = pack2(value_of(word[u] >> (8 * i) & 15, zero_of(par[u]), step_of(par[u])),
-                             value_of(word[u] >> (8 * i + 4) & 15, zero_of(par[u]), step_of(par[u])), a.kind);
-            *x[u] = make_uint4(o[0], o[1], o[2], o[3]);
+        while (again) {                                      // few: these divide
+            const int i = __ffs(again) - 1;
+            again &= again - 1;
+            const float v = half_value<kKind>(i < 4 ? i < 2 ? r[0] : r[1] : i < 6 ? r[2] : r[3], i);
+            word = (word & ~(15u << (4 * i))) | code_of(v, zero, step) << (4 * i);
         }
+        if (rec != nullptr && row_ok) {
+            *codes = word;
+            if (w == 0) *params = p;
+        }
+    } else if (rec != nullptr) {
+        const uint32_t word = row_ok ? *codes : 0, p = row_ok ? *params : 0;
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o[i] = pack2(value_of(word >> (8 * i) & 15, zero_of(p), step_of(p)), value_of(word >> (8 * i + 4) & 15, zero_of(p), step_of(p)),
+                         kKind);
+        *x = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
@@ -366,10 +357,12 @@ template <bool kWrite>
 int run_rows(const rvq_cache4_rows_args* a, void* stream) {
     const int rc = check_rows(a);
     if (rc != RVQ_OK || a->tokens == 0) return rc;
-    const int per_block = kTokens * kRowsThreads / (a->cache.head_dim / 4);
+    const int per_block = kRowsThreads / (a->cache.head_dim / 4);
     const int64_t blocks = (a->tokens + per_block - 1) / per_block;
     if (a->cache.n_kv > 65535) return RVQ_ERR_TOO_LARGE;
-    auto* kernel = a->cache.head_dim == 128 ? cache4_rows_kernel<128, kWrite> : cache4_rows_kernel<64, kWrite>;
+    auto* kernel = a->cache.head_dim == 128
+                       ? a->kind == RVQ_F16 ? cache4_rows_kernel<128, kWrite, RVQ_F16> : cache4_rows_kernel<128, kWrite, RVQ_BF16>
+                       : a->kind == RVQ_F16 ? cache4_rows_kernel<64, kWrite, RVQ_F16> : cache4_rows_kernel<64, kWrite, RVQ_BF16>;
     return status(launch_pdl(kernel, dim3((unsigned)blocks, a->cache.n_kv), dim3(kRowsThreads), 0, (cudaStream_t)stream, *a));
 }
 

@@ -30,13 +30,15 @@ __device__ __forceinline__ uint32_t code_of(float x, float zero, float step) {
 
 // The same with inv = 1 / step (approximate), unless *near is set: where d inv is clearly nearer to one integer than to the
 // next, that integer is the quotient's too (|d - k s| < 0.4999 s leaves 2^-13 s for the roundings of inv, of d inv, of
-// d - k s and of the quotient, about 2^-22 s each).  Near the middle between two, and for a step that is 0 or not finite,
-// *near is set and the caller divides.
+// d - k s and of the quotient, about 2^-22 s each).  Near the middle between two, and for a step that is 0, subnormal (inv is
+// infinite then) or not finite, *near is set and the caller divides.  kClamp false: zero is the group's minimum itself
+// (bf16 values), so that 0 <= d <= 15 s (1 + 2^-8) and the integer is in range.
+template <bool kClamp>
 __device__ __forceinline__ uint32_t code_near(float x, float zero, float step, float inv, bool* near) {
     constexpr float kInt = 12582912.f;                       // 1.5 2^23: a sum with it ends at an integer
-    const float d = __fsub_rn(x, zero), k = __fsub_rn(fmaf(d, inv, kInt), kInt);
-    *near = !(fabsf(fmaf(-k, step, d)) < 0.4999f * step && k < 64.f);
-    return __float_as_uint(__fadd_rn(fminf(fmaxf(k, 0.f), 15.f), kInt)) & 15u;
+    const float d = __fsub_rn(x, zero), t = fmaf(d, inv, kInt), k = __fsub_rn(t, kInt);
+    *near = !(fabsf(fmaf(-k, step, d)) < 0.4999f * step);
+    return __float_as_uint(kClamp ? __fadd_rn(fminf(fmaxf(k, 0.f), 15.f), kInt) : t) & 15u;
 }
 
 // z + s c (s c is exact: 8 by 4 bits)

@@ -624,8 +624,9 @@ typedef struct rvq_prompt_attn_args {
     int32_t reserved;         /* 0 */
 } rvq_prompt_attn_args;
 
-/* Bytes of device workspace that the call needs (0: none).  One call at a time
- * uses a workspace; its contents need no initialisation. */
+/* Bytes of device workspace that the call needs (0: none), 16-byte aligned and
+ * zero-filled before its first call; every call leaves what the next one needs.
+ * One call at a time uses a workspace. */
 size_t rvq_prompt_attention_workspace_size(const rvq_prompt_attn_args* a);
 int rvq_prompt_attention(const rvq_prompt_attn_args* a, void* workspace, size_t workspace_bytes, void* stream);
 

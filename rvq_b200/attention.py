@@ -187,7 +187,7 @@ class _Op:
         """Allocates what ``self.args`` needs; its bytes."""
         with torch.cuda.device(self.device):
             n = size(ctypes.byref(self.args))
-        self._ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        self._ws = torch.zeros(n, dtype=torch.uint8, device=self.device) if n else None
         return n
 
     def _bind(self, where: str, *args) -> None:

@@ -28,7 +28,10 @@ __device__ int g_attention_timeout;          // sticky: a bounded wait gave up
 //                   written over S in TMEM
 //   O += P V        tcgen05.mma, P from TMEM, V as it lies in shared memory
 //
-// While one tile's softmax runs, the tensor cores work for the other one.  The
+// A CTA takes such pairs of tiles one after the other (the longest first, by a
+// ticket from the second on); the next one's loads and its first S run beside this
+// one's last softmax and output.  While one tile's softmax runs, the tensor cores
+// work for the other one.  The
 // maximum that is subtracted only follows the true one when that has grown by
 // 2^8: O is then rescaled by the row's own thread, which is rare after the first
 // tiles; p stays below 2^8, exact in fp32 sums and with unchanged relative rounding.
@@ -52,6 +55,9 @@ struct Params {
     int32_t tile_tokens;                     // 128 / rep
     int32_t pairs;                           // upper bound of the pairs of tiles of all sequences
     int32_t splits;                          // parts of the keys, each with CTAs of its own
+    int32_t sms;
+    int32_t units;                           // pairs x kv heads x parts: what the CTAs take one after the other
+    uint32_t* tickets;                       // units beyond the first one of every CTA given out, CTAs done; NULL: there are none
     float* part_o;                           // splits > 1: [splits][tokens][n_heads][head_dim], not yet divided by the sum
     float2* part_ml;                         // [splits][tokens][n_heads]: maximum (times c) and sum
 };
@@ -63,7 +69,8 @@ struct Work {
     int32_t tok0;                            // first token of tile 0 in the sequence
     int32_t j0;                              // first tile of keys
     int32_t n[2];                            // tiles of keys that the two tiles of queries take from there on (0, 0: nothing to do)
-    int32_t live;                            // there is such a pair of tiles at all
+    int32_t live;                            // 1; 0: the pair is in no sequence; -1: no unit is left
+    int32_t kv, split;
     int32_t clean;                           // the last tile of keys reaches into another sequence
 };
 
@@ -74,10 +81,12 @@ struct Smem {
     uint8_t k[2][kTileBytes];
     uint8_t v[2][kTileBytes];
     uint64_t q_full, drain, v_clean, s_full[2], p_full[2], o_full[2];
-    uint64_t first_full, first_empty;        // K of tile 0
-    uint64_t kv_full[2], kv_empty[2];        // V of tile j and K of tile j + 1, at j & 1
+    uint64_t first_full, first_empty;        // K of a unit's tile 0
+    uint64_t kv_full[2], kv_empty[2];        // steps, counted over all units: V of tile j and K of tile j + 1
+    uint64_t work_full[2], work_empty[2];
     float top[2][2][kRows];                  // a row's maximum (at the end: sum) over either half of the columns
-    Work work;
+    Work work[2];
+    int32_t fail[8];                         // of two warps of the same rows one has given up
     uint32_t tmem;
     int32_t dead;                            // a bounded wait gave up
 };
@@ -308,156 +317,238 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     Smem<HD>& S = *reinterpret_cast<Smem<HD>*>(smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023));
     const rvq_prompt_attn_args& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-    const int kv = unit % a.n_kv;
     const int T = p.tile_tokens;
     pdl_launch_dependents();
-    auto load = [&](const CUtensorMap& map, uint8_t* dst, int64_t row, uint64_t& bar) {      // 128 keys, or a tile's tokens
+    if (warp == kSoftmaxWarps && lane == 0) {
+        mbar_init(smem_addr(&S.q_full), 1);
+        mbar_init(smem_addr(&S.v_clean), 1);
+        mbar_init(smem_addr(&S.drain), 1);
+        mbar_init(smem_addr(&S.first_full), 1);
+        mbar_init(smem_addr(&S.first_empty), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_addr(&S.kv_full[i]), 1);
+            mbar_init(smem_addr(&S.kv_empty[i]), 1);
+            mbar_init(smem_addr(&S.s_full[i]), 1);
+            mbar_init(smem_addr(&S.p_full[i]), kSoftmaxWarps / 2);
+            mbar_init(smem_addr(&S.o_full[i]), 1);
+            mbar_init(smem_addr(&S.work_full[i]), 1);
+            mbar_init(smem_addr(&S.work_empty[i]), kSoftmaxWarps + 1);
+        }
+        S.dead = 0;
+        for (int i = 0; i < 8; ++i) S.fail[i] = 0;
+        mbar_init_fence();
+        fence_async_shared();
+    }
+    if (warp == kSoftmaxWarps + 1) tmem_alloc(smem_addr(&S.tmem), 512);
+    // Work of a unit, by the loading warp, and its loads that need no other buffers than free ones
+    auto find = [&](int unit) {
+        Work w = {};
+        w.live = -1;
+        if (unit < p.units) {
+            const int split = unit % p.splits, rest = unit / p.splits;
+            // the last pairs of a causal sequence see the most keys: they start first
+            w = find_work(p, p.pairs - 1 - rest / a.n_kv, split);
+            w.kv = rest % a.n_kv, w.split = split;
+        }
+        return w;
+    };
+    auto load = [&](const CUtensorMap& map, int head, uint8_t* dst, int64_t row, uint64_t& bar) {     // 128 keys, or a tile's tokens
         for (int h = 0; h < HD / 64; ++h)
-            tma_load_3d(smem_addr(dst + h * kHalf), &map, 64 * h, &map == &p.q ? kv * p.rep : kv, (int)row, smem_addr(&bar));
+            tma_load_3d(smem_addr(dst + h * kHalf), &map, 64 * h, head, (int)row, smem_addr(&bar));
     };
-    auto load_step = [&](const Work& w, int j, int total) {  // V of tile j and K of tile j + 1
-        mbar_expect_tx(smem_addr(&S.kv_full[j & 1]), (j + 1 < total ? 2 : 1) * Smem<HD>::kTileBytes);
-        load(p.v, S.v[j & 1], w.k0 + (int64_t)(w.j0 + j) * kKeys, S.kv_full[j & 1]);
-        if (j + 1 < total) load(p.k, S.k[(j + 1) & 1], w.k0 + (int64_t)(w.j0 + j + 1) * kKeys, S.kv_full[j & 1]);
+    auto load_step = [&](const Work& w, int step, int j, int total) {      // V of tile j and K of tile j + 1
+        uint64_t& bar = S.kv_full[step & 1];
+        mbar_expect_tx(smem_addr(&bar), (j + 1 < total ? 2 : 1) * Smem<HD>::kTileBytes);
+        load(p.v, w.kv, S.v[step & 1], w.k0 + (int64_t)(w.j0 + j) * kKeys, bar);
+        if (j + 1 < total) load(p.k, w.kv, S.k[(step + 1) & 1], w.k0 + (int64_t)(w.j0 + j + 1) * kKeys, bar);
     };
-    if (warp == kSoftmaxWarps) {
-        // what there is to do, and its first loads, while the other warps get ready
+    auto load_first = [&](const Work& w, int step, int total) {
+        const int tiles = w.tok0 + T < w.lq ? 2 : 1;
+        mbar_expect_tx(smem_addr(&S.q_full), tiles * (HD / 64) * (uint32_t)(T * p.rep * 128));
+        for (int i = 0; i < tiles; ++i) load(p.q, w.kv * p.rep, S.q[i], w.q0 + w.tok0 + i * T, S.q_full);
+        mbar_expect_tx(smem_addr(&S.first_full), Smem<HD>::kTileBytes);
+        load(p.k, w.kv, S.k[step & 1], w.k0 + (int64_t)w.j0 * kKeys, S.first_full);
+        load_step(w, step, 0, total);
+    };
+    pdl_wait();
+    Work first = {};
+    if (warp == kSoftmaxWarps) {                             // the first unit's loads, while the other warps get ready
+        __syncwarp();
+        first = find(blockIdx.x);
+        const int total = max(first.n[0], first.n[1]);
         if (lane == 0) {
-            mbar_init(smem_addr(&S.q_full), 1);
-            mbar_init(smem_addr(&S.v_clean), 1);
-            mbar_init(smem_addr(&S.drain), 1);
-            mbar_init(smem_addr(&S.first_full), 1);
-            mbar_init(smem_addr(&S.first_empty), 1);
-            for (int i = 0; i < 2; ++i) {
-                mbar_init(smem_addr(&S.kv_full[i]), 1);
-                mbar_init(smem_addr(&S.kv_empty[i]), 1);
-                mbar_init(smem_addr(&S.s_full[i]), 1);
-                mbar_init(smem_addr(&S.p_full[i]), kSoftmaxWarps / 2);
-                mbar_init(smem_addr(&S.o_full[i]), 1);
-            }
-            S.dead = 0;
-            mbar_init_fence();
-            fence_async_shared();
+            S.work[0] = first;
+            mbar_arrive(smem_addr(&S.work_full[0]));
+            if (total > 0) load_first(first, 0, total);
         }
-        pdl_wait();
-        // the last pairs of a causal sequence see the most keys: they start first
-        const Work w = find_work(p, p.pairs - 1 - unit / a.n_kv, split);
-        if (lane == 0) {
-            S.work = w;
-            const int total = max(w.n[0], w.n[1]);
-            if (total > 0) {
-                const int tiles = w.tok0 + T < w.lq ? 2 : 1;
-                mbar_expect_tx(smem_addr(&S.q_full), tiles * (HD / 64) * (uint32_t)(T * p.rep * 128));
-                for (int i = 0; i < tiles; ++i) load(p.q, S.q[i], w.q0 + w.tok0 + i * T, S.q_full);
-                mbar_expect_tx(smem_addr(&S.first_full), Smem<HD>::kTileBytes);
-                load(p.k, S.k[0], w.k0 + (int64_t)w.j0 * kKeys, S.first_full);
-                load_step(w, 0, total);
-            }
-        }
-    } else {
-        if (warp == kSoftmaxWarps + 1) tmem_alloc(smem_addr(&S.tmem), 512);
-        pdl_wait();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = S.tmem;
-    if (S.work.live) {
-        const int64_t q0 = S.work.q0, k0 = S.work.k0;
-        const int lq = S.work.lq, lk = S.work.lk, tok0 = S.work.tok0, j0 = S.work.j0;
-        const int n[2] = {S.work.n[0], S.work.n[1]};
-        const int total = max(n[0], n[1]);
-        const bool clean = S.work.clean;
-
-        if (warp == kSoftmaxWarps) {
-            int loaded = min(total, 1);
-            for (int j = 1; j < total; ++j) {
-                if (j >= 2 && !wait(S, S.kv_empty[j & 1], (j / 2 - 1) & 1)) break;
-                if (j == 1 && !wait(S, S.first_empty, 0)) break;            // K of tile 2 replaces that of tile 0
-                if (lane == 0) load_step(S.work, j, total);
-                loaded = j + 1;
+    if (warp == kSoftmaxWarps) {
+        int steps = 0, loaded = 0, used = 0;                 // steps of the units before, steps loaded, units with tiles
+        int cleaned = -1;                                    // the last step whose values were cleaned
+        Work w = first;
+        bool ok = true;
+        for (int it = 0; ok; ++it) {
+            const int slot = it & 1;
+            if (it >= 2) ok = wait(S, S.work_empty[slot], (it / 2 - 1) & 1);
+            if (!ok) break;
+            if (it > 0 && lane == 0) {
+                S.work[slot] = w;
+                mbar_arrive(smem_addr(&S.work_full[slot]));
             }
-            if (clean && loaded == total && wait(S, S.kv_full[(total - 1) & 1], ((total - 1) / 2) & 1)) {
-                uint8_t* v = S.v[(total - 1) & 1];
-                const int r0 = lk - (j0 + total - 1) * kKeys;     // rows r0 .. 127 belong to others (a swizzled row stays a row)
-                for (int h = 0; h < HD / 64; ++h)
-                    for (int i = r0 * 8 + lane; i < kRows * 8; i += 32)
-                        reinterpret_cast<uint4*>(v + h * kHalf)[i] = make_uint4(0, 0, 0, 0);
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&S.v_clean));
-            }
-            if (*(volatile int32_t*)&S.dead && total > 0) {  // copies in flight end before this CTA's shared memory is given up
-                for (int j = max(0, loaded - 2); j < loaded; ++j)
-                    mbar_wait(smem_addr(&S.kv_full[j & 1]), (j / 2) & 1, kWaitPolls, &g_attention_timeout);
-                mbar_wait(smem_addr(&S.first_full), 0, kWaitPolls, &g_attention_timeout);
-                mbar_wait(smem_addr(&S.q_full), 0, kWaitPolls, &g_attention_timeout);
-            }
-        } else if (warp == kSoftmaxWarps + 1) {
-            // One thread from here to the end: what it does between two products, the tensor cores wait for.
-            constexpr uint32_t kTypes = kHalfType ? 0u : (1u << 7) | (1u << 10);
-            constexpr uint32_t kS = (1u << 4) | kTypes | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-            constexpr uint32_t kO = (1u << 4) | kTypes | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-            if (lane == 0 && total > 0) {
-                // c is |scaling|: a negative one negates Q on its way (so that the largest score stays the largest)
-                const uint32_t types_s = kS | (a.scaling < 0.f ? 1u << 13 : 0u);
-                const uint64_t dq = sw128_desc(smem_addr(S.q[0])), dk = sw128_desc(smem_addr(S.k[0]));
-                const uint64_t dv = sw128_desc_mn(smem_addr(S.v[0]), kHalf);
-                constexpr uint32_t kTile = Smem<HD>::kTileBytes >> 4;      // descriptors count 16 bytes
-                auto scores = [&](int i, int j) {            // S_i = Q_i K_j^T
-                    const uint64_t q = dq + i * kTile, k = dk + (j & 1) * kTile;
-#pragma unroll
-                    for (int x = 0; x < HD / 16; ++x)
-                        mma_bf16(tmem + i * kKeys, q + (x / 4) * (kHalf >> 4) + (x % 4) * 2, k + (x / 4) * (kHalf >> 4) + (x % 4) * 2,
-                                 types_s, x > 0);
-                    mma_commit(smem_addr(&S.s_full[i]));
-                };
-                bool ok = wait1(S, smem_addr(&S.q_full), 0) && wait1(S, smem_addr(&S.first_full), 0);
-                if (ok) {
-                    for (int i = 0; i < 2; ++i)
-                        if (n[i] > 0) scores(i, 0);
-                    mma_commit(smem_addr(&S.first_empty));
+            if (w.live < 0) break;
+            const int total = max(w.n[0], w.n[1]);
+            int next = p.units;
+            if (total > 0) {
+                if (it > 0) {
+                    // Q and the K buffers are free with the last S of the unit before: with its last step but one, or with its first
+                    // S where it has one tile; the V buffer with the step before the last
+                    if (steps >= 2) ok = wait(S, S.kv_empty[steps & 1], (steps / 2 - 1) & 1);
+                    if (ok && used > 0) ok = wait(S, S.first_empty, (used - 1) & 1);
+                    if (!ok) break;
+                    if (lane == 0) load_first(w, steps, total);
                 }
-                for (int j = 0; ok && j < total; ++j) {
-                    ok = wait1(S, smem_addr(&S.kv_full[j & 1]), (j / 2) & 1);
-                    if (ok && clean && j == total - 1) ok = wait1(S, smem_addr(&S.v_clean), 0);
-                    const uint64_t v = dv + (j & 1) * kTile;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (!ok || j >= n[i]) continue;
-                        ok = wait1(S, smem_addr(&S.p_full[i]), j & 1);
-                        if (!ok) continue;
-                        tc_fence_after();
-#pragma unroll
-                        for (int k = 0; k < kKeys / 16; ++k)
-                            mma_bf16_ts(tmem + 2 * kKeys + i * HD, tmem + i * kKeys + 8 * k, v + k * (2048 >> 4), kO, j > 0 || k > 0);
-                        if (j + 1 < n[i]) scores(i, j + 1);
-                        else mma_commit(smem_addr(&S.o_full[i]));
-                    }
-                    if (ok) mma_commit(smem_addr(&S.kv_empty[j & 1]));
+                loaded = steps + 1;
+                for (int j = 1; j < total && ok; ++j) {
+                    const int step = steps + j;
+                    if (step >= 2) ok = wait(S, S.kv_empty[step & 1], (step / 2 - 1) & 1);
+                    if (ok && j == 1) ok = wait(S, S.first_empty, used & 1);           // K of tile 2 replaces that of tile 0
+                    if (!ok) break;
+                    if (lane == 0) load_step(w, step, j, total);
+                    loaded = step + 1;
                 }
-                if (!ok) {                                   // products in flight end before TMEM is given up
-                    mma_commit(smem_addr(&S.drain));
-                    mbar_wait(smem_addr(&S.drain), 0, kWaitPolls, &g_attention_timeout);
+                steps += total;
+                ++used;
+            }
+            // the next unit only now that this one is loaded: who has long units takes fewer of them
+            if (ok && lane == 0 && p.tickets != nullptr) next = (int)(gridDim.x + atomicAdd(p.tickets, 1u));
+            if (total > 0) {
+                if (ok && w.clean) {
+                    const int last = steps - 1;
+                    // one clean tile at a time: the one before may be this one's neighbour, not yet used
+                    if (cleaned >= 0 && last < cleaned + 2) ok = wait(S, S.kv_empty[cleaned & 1], (cleaned / 2) & 1);
+                    if (ok) ok = wait(S, S.kv_full[last & 1], (last / 2) & 1);
+                    if (!ok) break;
+                    cleaned = last;
+                    const int r0 = w.lk - (w.j0 + total - 1) * kKeys;        // rows r0 .. 127 belong to others (a swizzled row stays a row)
+                    for (int h = 0; h < HD / 64; ++h)
+                        for (int i = r0 * 8 + lane; i < kRows * 8; i += 32)
+                            reinterpret_cast<uint4*>(S.v[last & 1] + h * kHalf)[i] = make_uint4(0, 0, 0, 0);
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_addr(&S.v_clean));
                 }
             }
-            __syncwarp();
-        } else {
-            // two threads a row, 64 columns of S and half of O's each
-            const int i = warp >> 3, half = warp >> 2 & 1, row = tid & 127;
-            const int in = row / p.rep, h = kv * p.rep + row % p.rep;
-            const int tok = tok0 + i * T + in;               // in the sequence
-            const bool valid = in < T && tok < lq;
-            const int limit = !valid ? 0 : a.causal ? min(lk, max(0, tok + 1 + lk - lq)) : lk;
-            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 2 * kKeys + i * HD + half * (HD / 2);
-            const int pair_bar = 1 + i * 4 + (warp & 3);     // named barrier of the two warps of these rows
-            const float c = fabsf(a.scaling) * 1.4426950408889634f;
-            float m = -INFINITY, sum = 0.f;                  // m: of the scores times c
+            if (ok) w = find(__shfl_sync(0xffffffffu, next, 0));
+        }
+        if (lane == 0 && p.tickets != nullptr) {             // the last CTA leaves the tickets as they were
+            __threadfence();
+            if (atomicAdd(p.tickets + 1, 1u) == gridDim.x - 1) p.tickets[0] = p.tickets[1] = 0;
+        }
+        if (!ok) {                                           // copies in flight end before this CTA's shared memory is given up
+            for (int j = max(0, loaded - 2); j < loaded; ++j)
+                mbar_wait(smem_addr(&S.kv_full[j & 1]), (j / 2) & 1, kWaitPolls, &g_attention_timeout);
+            if (loaded > 0) {
+                const int u = (used > 0 && loaded == steps ? used - 1 : used) & 1;
+                mbar_wait(smem_addr(&S.first_full), u, kWaitPolls, &g_attention_timeout);
+                mbar_wait(smem_addr(&S.q_full), u, kWaitPolls, &g_attention_timeout);
+            }
+        }
+    } else if (warp == kSoftmaxWarps + 1) {
+        // One thread from here to the end: what it does between two products, the tensor cores wait for.
+        constexpr uint32_t kTypes = kHalfType ? 0u : (1u << 7) | (1u << 10);
+        constexpr uint32_t kS = (1u << 4) | kTypes | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+        constexpr uint32_t kO = (1u << 4) | kTypes | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+        if (lane == 0) {
+            // c is |scaling|: a negative one negates Q on its way (so that the largest score stays the largest)
+            const uint32_t types_s = kS | (a.scaling < 0.f ? 1u << 13 : 0u);
+            const uint64_t dq = sw128_desc(smem_addr(S.q[0])), dk = sw128_desc(smem_addr(S.k[0]));
+            const uint64_t dv = sw128_desc_mn(smem_addr(S.v[0]), kHalf);
+            constexpr uint32_t kTile = Smem<HD>::kTileBytes >> 4;          // descriptors count 16 bytes
+            auto scores = [&](int i, int at) {               // S_i = Q_i K^T, K in buffer `at`
+                const uint64_t q = dq + i * kTile, k = dk + at * kTile;
+#pragma unroll
+                for (int x = 0; x < HD / 16; ++x)
+                    mma_bf16(tmem + i * kKeys, q + (x / 4) * (kHalf >> 4) + (x % 4) * 2, k + (x / 4) * (kHalf >> 4) + (x % 4) * 2,
+                             types_s, x > 0);
+                mma_commit(smem_addr(&S.s_full[i]));
+            };
+            int steps = 0, used = 0, cleaned = 0;
+            uint32_t pp = 0;                                 // parities of the tiles' next P
             bool ok = true;
-            for (int j = 0; j < n[i]; ++j) {
-                ok = ok && wait(S, S.s_full[i], j & 1);
+            for (int it = 0; ok; ++it) {
+                ok = wait1(S, smem_addr(&S.work_full[it & 1]), (it / 2) & 1);
+                if (!ok) break;
+                const Work& w = S.work[it & 1];
+                if (w.live < 0) break;
+                const int n[2] = {w.n[0], w.n[1]}, total = max(n[0], n[1]);
+                const bool clean = w.clean;
+                if (total > 0) {
+                    ok = wait1(S, smem_addr(&S.q_full), used & 1) && wait1(S, smem_addr(&S.first_full), used & 1);
+                    if (ok) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (n[i] > 0) scores(i, steps & 1);
+                        mma_commit(smem_addr(&S.first_empty));
+                    }
+                    for (int j = 0; ok && j < total; ++j, ++steps) {
+                        ok = wait1(S, smem_addr(&S.kv_full[steps & 1]), (steps / 2) & 1);
+                        if (ok && clean && j == total - 1) ok = wait1(S, smem_addr(&S.v_clean), cleaned++ & 1);
+                        const uint64_t v = dv + (steps & 1) * kTile;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if (!ok || j >= n[i]) continue;
+                            ok = wait1(S, smem_addr(&S.p_full[i]), pp >> i & 1);
+                            if (!ok) continue;
+                            pp ^= 1u << i;
+                            tc_fence_after();
+#pragma unroll
+                            for (int k = 0; k < kKeys / 16; ++k)
+                                mma_bf16_ts(tmem + 2 * kKeys + i * HD, tmem + i * kKeys + 8 * k, v + k * (2048 >> 4), kO, j > 0 || k > 0);
+                            if (j + 1 < n[i]) scores(i, (steps + 1) & 1);
+                            else mma_commit(smem_addr(&S.o_full[i]));
+                        }
+                        if (ok) mma_commit(smem_addr(&S.kv_empty[steps & 1]));
+                    }
+                    ++used;
+                }
+                if (ok) mbar_arrive(smem_addr(&S.work_empty[it & 1]));
+            }
+            if (!ok) {                                       // products in flight end before TMEM is given up
+                mma_commit(smem_addr(&S.drain));
+                mbar_wait(smem_addr(&S.drain), 0, kWaitPolls, &g_attention_timeout);
+            }
+        }
+        __syncwarp();
+    } else {
+        // two threads a row, 64 columns of S and half of O's each
+        const int i = warp >> 3, half = warp >> 2 & 1, row = tid & 127;
+        const int pair_bar = 1 + i * 4 + (warp & 3);         // named barrier of the two warps of these rows
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 2 * kKeys + i * HD + half * (HD / 2);
+        const float c = fabsf(a.scaling) * 1.4426950408889634f;
+        const int in = row / p.rep, head = row - in * p.rep;
+        uint32_t sp = 0, op = 0;                             // parities of the next S and O
+        bool ok = true;
+        for (int it = 0;; ++it) {
+            ok = ok && wait(S, S.work_full[it & 1], (it / 2) & 1);
+            if (!ok && lane == 0) *(volatile int32_t*)&S.fail[pair_bar - 1] = 1;
+            named_sync(pair_bar, 64);                        // both warps go on, or neither
+            if (*(volatile int32_t*)&S.fail[pair_bar - 1]) break;
+            const Work& w = S.work[it & 1];
+            if (w.live < 0) break;
+            const int64_t q0 = w.q0, k0 = w.k0;
+            const int lq = w.lq, lk = w.lk, tok0 = w.tok0, j0 = w.j0, n = w.n[i], h = w.kv * p.rep + head, split = w.split;
+            const bool live = w.live;
+            const int tok = tok0 + i * T + in;               // in the sequence
+            const bool valid = live && in < T && tok < lq;
+            const int limit = !valid ? 0 : a.causal ? min(lk, max(0, tok + 1 + lk - lq)) : lk;
+            float m = -INFINITY, sum = 0.f;                  // m: of the scores times c
+            for (int j = 0; j < n; ++j, sp ^= 1) {
+                ok = ok && wait(S, S.s_full[i], sp);
                 if (!ok) {                                   // the partner may still come to its barriers
                     named_sync(pair_bar, 64);
                     continue;
@@ -504,7 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&S.p_full[i]));
             }
-            if (ok && n[i] > 0) ok = wait(S, S.o_full[i], 0);
+            if (ok && n > 0) ok = wait(S, S.o_full[i], op);
+            op ^= n > 0;
             tc_fence_after();
             named_sync(pair_bar, 64);                        // the partner has read this half's last maximum
             S.top[i][half][row] = sum;
@@ -520,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll 1
             for (int x = 0; x < HD / 32; ++x) {              // 16 columns
                 uint32_t o[16];
-                if (ok && n[i] > 0) {
+                if (ok && n > 0) {
                     tmem_ld8(to + 16 * x, *reinterpret_cast<uint32_t (*)[8]>(o));
                     tmem_ld8(to + 16 * x + 8, *reinterpret_cast<uint32_t (*)[8]>(o + 8));
                     tmem_ld_wait();
@@ -554,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 a.lse[(int64_t)h * a.tokens + q0 + tok] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
             if (valid && half == 0 && !whole) p.part_ml[slot] = make_float2(m, limit == 0 ? 0.f : sum);
             // values between this row's last key and the end of its last tile may have leaked in
-            const int begin = j0 * kKeys, hidden_end = min(lk, (j0 + n[i]) * kKeys), seen_end = min(limit, hidden_end);
+            const int begin = j0 * kKeys, hidden_end = min(lk, (j0 + n) * kKeys), seen_end = min(limit, hidden_end);
             uint32_t again = __ballot_sync(0xffffffffu, ok && valid && bad && seen_end > begin && seen_end < hidden_end && fabsf(sum) <= 3.4e38f);
             while (again) {
                 const int l = __ffs(again) - 1;
@@ -566,6 +658,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                        __shfl_sync(0xffffffffu, m, l), __shfl_sync(0xffffffffu, inv, l),
                        whole ? nullptr : p.part_o + (((int64_t)split * a.tokens + row) * a.n_heads + head) * a.head_dim);
             }
+            tc_fence_before();                               // O is read: the next unit's products may come
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(smem_addr(&S.work_empty[it & 1]));
         }
     }
     tc_fence_before();
@@ -673,7 +768,7 @@ int run(const Params& p, cudaStream_t s) {
     const int smem = (int)sizeof(Smem<HD>) + 1024;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
-        e = launch_pdl(kernel, dim3((unsigned)(p.pairs * p.a.n_kv * p.splits)), dim3(kThreads), (size_t)smem, s, p);
+        e = launch_pdl(kernel, dim3((unsigned)(p.tickets != nullptr ? p.sms : p.units)), dim3(kThreads), (size_t)smem, s, p);
     if (e == cudaSuccess && p.splits > 1)
         e = launch_pdl(join_kernel, dim3((unsigned)((p.a.tokens * p.a.n_heads + 3) / 4)), dim3(128), 0, s, p);
     return status(e);
@@ -699,10 +794,13 @@ int plan(const rvq_prompt_attn_args& a, Params* p) {
         const int64_t most = sms / units, parts = tiles / 4;
         p->splits = (int32_t)(most < parts ? most : parts);
     }
+    p->sms = sms;
+    p->units = (int32_t)(units * p->splits);
     return RVQ_OK;
 }
 
 size_t part_bytes(const rvq_prompt_attn_args& a, const Params& p) {
+    if (p.units > p.sms) return 2 * sizeof(uint32_t);        // tickets
     return p.splits == 1 ? 0 : (size_t)p.splits * a.tokens * a.n_heads * (a.head_dim + 2) * 4;
 }
 
@@ -730,6 +828,7 @@ extern "C" int rvq_prompt_attention(const rvq_prompt_attn_args* a, void* workspa
     if (rc != RVQ_OK) return rc;
     if (part_bytes(*a, p) > 0) {
         if (workspace == nullptr || workspace_bytes < part_bytes(*a, p) || ((uintptr_t)workspace & 15)) return RVQ_ERR_INVALID;
+        if (p.units > p.sms) p.tickets = reinterpret_cast<uint32_t*>(workspace);
         p.part_o = reinterpret_cast<float*>(workspace);
         p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)p.splits * a->tokens * a->n_heads * a->head_dim);
     }

@@ -530,6 +530,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 2 * kKeys + i * HD + half * (HD / 2);
         const float c = fabsf(a.scaling) * 1.4426950408889634f;
+        // fp16 has few small numbers: p up to 2^15 instead of 2^kGrow, and so 2^-32 of the row's largest one instead of 2^-25
+        // for the rounding of the smallest
+        constexpr float kShift = kHalfType ? 15.f - kGrow : 0.f;
         const int in = row / p.rep, head = row - in * p.rep;
         uint32_t sp = 0, op = 0;                             // parities of the next S and O
         bool ok = true;
@@ -588,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     }
                     tmem_st_wait();
                 }
-                const float sub = m == -INFINITY ? 0.f : m;
+                const float sub = (m == -INFINITY ? 0.f : m) - kShift;
                 sum += masked ? row_exp<true, kHalfType>(s, seen, c, sub, ts + half * 32) : row_exp<false, kHalfType>(s, seen, c, sub, ts + half * 32);
                 tmem_st_wait();
                 tc_fence_before();
@@ -602,6 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             S.top[i][half][row] = sum;
             named_sync(pair_bar, 64);
             sum = S.top[i][0][row] + S.top[i][1][row];
+            m -= kShift;                                     // p and its sum are relative to that
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const bool whole = p.splits == 1, none = limit == 0 || (whole && inv == 0.f);
             const int64_t at = (q0 + tok) * a.out_stride[0] + h * a.out_stride[1];

@@ -69,7 +69,9 @@ def attend(q, k, v, scaling, causal):
     e = 2 d + 2^-21, and by u more where it is rounded to the operand type (u half a step); numerator and denominator
     both are, each over fp32 sums of lk terms (2^-24 sqrt(lk) in practice, lk 2^-24 at most).  One more rounding of
     the result: |error| <= u |out| + (u + 2 e + 2 lk 2^-24) sum p |v|.  2^-24 more absolutely, for results near zero
-    (16-bit subnormals and products below fp32's precision)."""
+    (16-bit subnormals and products below fp32's precision).  fp16 probabilities below 2^-14 round to multiples of 2^-24, by
+    at most 2^-25; they are held 2^7 times as large, and the largest of a row is at least 1, as is the sum that divides
+    them: 2^-32 sum |v| more."""
     u = half_step(q.dtype)
     rep = q.shape[1] // k.shape[1]
     lq, lk = q.shape[0], k.shape[0]
@@ -96,6 +98,8 @@ def attend(q, k, v, scaling, causal):
     d = (q.shape[2] + 8) * 2.0 ** -24 * size.amax(-1)
     e = 2 * d + 2.0 ** -21
     tol = u * out.abs() + (u + 2 * e + 2 * lk * 2.0 ** -24)[..., None] * mag + 2.0 ** -24
+    if q.dtype == torch.float16:
+        tol = tol + 2.0 ** -32 * vd.nan_to_num(0, 0, 0).abs().sum(1, keepdim=True)
     lse_tol = e + lk * 2.0 ** -24 + 2.0 ** -22 * lse.abs()
     return out.transpose(0, 1), lse, tol.transpose(0, 1), lse_tol
 

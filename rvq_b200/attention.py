@@ -152,6 +152,16 @@ def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _distinct(t: torch.Tensor, name: str) -> None:
+    """Refuses a written [tokens, heads, head_dim] view whose rows share elements."""
+    dims = sorted((t.stride(d), t.shape[d]) for d in (0, 1) if t.shape[d] > 1)
+    end = t.shape[2]
+    for stride, n in dims:
+        if stride < end:
+            raise ValueError(f"the rows of {name} must not overlap")
+        end = stride * (n - 1) + end
+
+
 def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two [tokens, heads, head_dim] views of one buffer with the same strides share no element (columns of one
     packed projection, say)."""
@@ -229,6 +239,7 @@ class PromptAttentionOp(_Op):
         keys, nkv = k.shape[:2]
         if out.shape != q.shape:
             raise ValueError("out must have q's shape")
+        _distinct(out, "out")
         if v.shape != k.shape or k.shape[2] != hd:
             raise ValueError("k and v must be [keys, n_kv, head_dim] with q's head_dim")
         if nkv < 1 or nh < 1 or nh % nkv:
@@ -237,8 +248,8 @@ class PromptAttentionOp(_Op):
             raise NotImplementedError("head_dim must be a multiple of 8, at most 128")
         if nh // nkv > 64:
             raise NotImplementedError("at most 64 query heads a kv head")
-        if max(tokens, keys) >= 2 ** 31:
-            raise ValueError("at most 2^31 - 1 tokens")
+        if max(tokens, keys) > 2 ** 30:
+            raise ValueError("at most 2^30 tokens")
         if cu_q is None:
             if cu_k is not None:
                 raise ValueError("cu_k needs cu_q")
@@ -271,8 +282,8 @@ class Cache4:
 
     def __init__(self, n_seq: int, n_kv: int, max_len: int, head_dim: int, device=None,
                  data: Optional[torch.Tensor] = None):
-        if min(n_seq, n_kv, max_len) < 1 or max(n_seq, n_kv, max_len) >= 2 ** 31:
-            raise ValueError("n_seq, n_kv and max_len must be positive")
+        if min(n_seq, n_kv, max_len) < 1 or max(n_seq, n_kv, max_len) > 2 ** 30:
+            raise ValueError("n_seq, n_kv and max_len must be 1 to 2^30")
         shape = (n_seq, n_kv, max_len, record_bytes(head_dim))
         if data is None:
             data = torch.zeros(shape, dtype=torch.uint8, device=device)
@@ -298,8 +309,8 @@ class _Cache4RowsOp(_Op):
         _heads3(v, "v", k.dtype)
         if k.shape != v.shape or k.shape[1] != cache.n_kv or k.shape[2] != cache.head_dim:
             raise ValueError("k and v must be [tokens, n_kv, head_dim] of the cache")
-        if k.shape[0] >= 2 ** 31:
-            raise ValueError("at most 2^31 - 1 tokens")
+        if k.shape[0] > 2 ** 30:
+            raise ValueError("at most 2^30 tokens")
         if cu is None and cache.n_seq != 1:
             raise ValueError("a cache of several sequences needs cu")
         if cu is not None:
@@ -310,6 +321,8 @@ class _Cache4RowsOp(_Op):
         _apart(v, cache.data, "v and the cache")
         if self.name == "rvq_cache4_read":
             _apart(k, v, "k and v")
+            _distinct(k, "k")
+            _distinct(v, "v")
         self._on(k, v, cache.data, cu, start)
         self.args = RvqCache4RowsArgs(cache.struct(), _ptr(k), _ptr(v), _ptr(cu), _ptr(start), k.shape[0], _strides(k),
                                       _strides(v), _native.kind_of(k), 0)

@@ -344,7 +344,7 @@ int check_rows(const rvq_cache4_rows_args* a) {
     if (a->tokens > 0 && (a->k == nullptr || a->v == nullptr)) return RVQ_ERR_INVALID;
     if (((uintptr_t)a->k | (uintptr_t)a->v) & 15) return RVQ_ERR_INVALID;
     if (a->cu == nullptr && a->cache.n_seq != 1) return RVQ_ERR_INVALID;
-    if (a->tokens >= (1ll << 31)) return RVQ_ERR_TOO_LARGE;
+    if (a->tokens > (1ll << 30)) return RVQ_ERR_TOO_LARGE;
     for (int i = 0; i < 2; ++i) {
         const int64_t s[2] = {a->k_stride[i], a->v_stride[i]};
         for (int j = 0; j < 2; ++j)
@@ -401,7 +401,7 @@ extern "C" int rvq_cache4_evict(const rvq_cache4_evict_args* a, void* stream) {
     if (o.n_seq != c.n_seq || o.n_kv != c.n_kv || o.head_dim != c.head_dim || o.max_len < a->keep) return RVQ_ERR_INVALID;
     if (a->keep < 1 || a->keep > c.max_len || a->recent < 0 || a->recent > a->keep) return RVQ_ERR_INVALID;
     const int64_t heads = (int64_t)c.n_seq * c.n_kv;
-    if (heads >= (1ll << 31)) return RVQ_ERR_TOO_LARGE;
+    if (heads >= (1ll << 31) || c.max_len > (1 << 30) || o.max_len > (1 << 30)) return RVQ_ERR_TOO_LARGE;
     if (o.data == c.data ? o.max_len != c.max_len : overlap(c.data, cache_bytes(c), o.data, cache_bytes(o)))
         return RVQ_ERR_INVALID;
     if (a->out_weights == a->weights ? o.max_len != c.max_len

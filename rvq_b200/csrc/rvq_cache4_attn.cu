@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
         if (tile < t1) {
             const uint8_t* src = cache + (int64_t)tile * (kTile * REC) + 16 * lane;
             const uint32_t dst = ring + stage * (kTile * REC);
-            const int bytes = (live - tile * kTile) * REC - 16 * lane;      // of live rows, from this lane's first piece on
+            const int bytes = min(kTile, live - tile * kTile) * REC - 16 * lane;      // of live rows, from this lane's first piece on
             const bool full = (tile + 1) * kTile <= live;
 #pragma unroll
             for (int i = 0; i < (kTile * REC + 511) / 512; ++i)
@@ -636,7 +636,7 @@ int check(const rvq_cache4_attn_args* a) {
     if ((a->cos == nullptr) != (a->sin == nullptr) || (a->cos == nullptr) != (a->pos == nullptr)) return RVQ_ERR_INVALID;
     if (a->cos != nullptr && a->table_len < 1) return RVQ_ERR_INVALID;
     if (a->q.kind == RVQ_F16 && (a->q_norm != nullptr || a->cos != nullptr)) return RVQ_ERR_UNSUPPORTED;
-    if (c.n_seq > 65535 || a->n_heads > 65535) return RVQ_ERR_TOO_LARGE;
+    if (c.n_seq > 65535 || a->n_heads > 65535 || c.max_len > (1 << 30)) return RVQ_ERR_TOO_LARGE;
     return RVQ_OK;
 }
 

@@ -42,6 +42,7 @@ __device__ int g_attention_timeout;          // sticky: a bounded wait gave up
 // ---------------------------------------------------------------------------
 constexpr int kRows = 128;                   // operand rows of a tile (MMA M)
 constexpr int kKeys = 128;                   // keys of a tile
+constexpr int kMaxSplits = 64;               // parts of the keys
 constexpr int kSoftmaxWarps = 16;            // 8 a tile
 constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
 constexpr int kHalf = kRows * 128;           // bytes of 64 columns of a tile
@@ -214,24 +215,30 @@ __device__ __forceinline__ float row_exp(float (&s)[2][32], int seen, float c, f
     return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// Pair number `want` (pairs counted over the sequences in order) and part `split` of its keys, by one warp.
-__device__ __forceinline__ Work find_work(const Params& p, int want, int split) {
+// Where find_work left off: sequences done with (from the last one on), and their pairs.
+struct Cursor {
+    int32_t base;
+    int64_t before;
+};
+
+// Pair number `want` and part `split` of its keys, by one warp.  Pairs are counted from the last one of the last sequence
+// down; a CTA's numbers only rise, so over all its units it goes over the sequences once.
+__device__ __forceinline__ Work find_work(const Params& p, int want, int split, Cursor& at) {
     const rvq_prompt_attn_args& a = p.a;
     const int lane = threadIdx.x & 31, T = p.tile_tokens;
     const int32_t* cu_k = a.cu_k != nullptr ? a.cu_k : a.cu_q;
     Work w = {};
-    int64_t before = 0;
-    for (int base = 0; base < a.n_seq; base += 32) {
-        const int b = base + lane;
+    for (; at.base < a.n_seq; at.base += 32) {
+        const int b = a.n_seq - 1 - at.base - lane;
         int64_t q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-        if (b < a.n_seq) {
+        if (b >= 0) {
             q1 = a.tokens, k1 = a.keys;
             if (a.cu_q != nullptr) {
                 q0 = max(0, __ldg(a.cu_q + b)), q1 = min(q1, (int64_t)__ldg(a.cu_q + b + 1));
                 k0 = max(0, __ldg(cu_k + b)), k1 = min(k1, (int64_t)__ldg(cu_k + b + 1));
             }
         }
-        const int64_t mine = q1 > q0 ? (q1 - q0 + 2 * T - 1) / (2 * T) : 0;
+        const int64_t mine = q1 > q0 ? (q1 - q0 + 2 * T - 1) / (2 * T) : 0, before = at.before;
         int64_t upto = mine;                                 // inclusive prefix sum over the lanes
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -240,7 +247,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int want, int split) 
         }
         const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
         if (want >= before + total) {
-            before += total;
+            at.before += total;
             continue;
         }
         const int l = __ffs(__ballot_sync(0xffffffffu, want < before + upto)) - 1;
@@ -249,7 +256,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int want, int split) 
         w.k0 = __shfl_sync(0xffffffffu, k0, l);
         w.lq = (int)(__shfl_sync(0xffffffffu, q1, l) - w.q0);
         w.lk = (int)max((int64_t)0, __shfl_sync(0xffffffffu, k1, l) - w.k0);
-        w.tok0 = (int)(want - before - __shfl_sync(0xffffffffu, upto - mine, l)) * 2 * T;
+        w.tok0 = (int)(before + __shfl_sync(0xffffffffu, upto, l) - 1 - want) * 2 * T;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {                        // what tile i's last token sees
             const int last = min(w.lq, w.tok0 + (i + 1) * T) - 1;
@@ -341,13 +348,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     if (warp == kSoftmaxWarps + 1) tmem_alloc(smem_addr(&S.tmem), 512);
     // Work of a unit, by the loading warp, and its loads that need no other buffers than free ones
+    Cursor cursor = {};
     auto find = [&](int unit) {
         Work w = {};
         w.live = -1;
         if (unit < p.units) {
             const int split = unit % p.splits, rest = unit / p.splits;
             // the last pairs of a causal sequence see the most keys: they start first
-            w = find_work(p, p.pairs - 1 - rest / a.n_kv, split);
+            w = find_work(p, rest / a.n_kv, split, cursor);
             w.kv = rest % a.n_kv, w.split = split;
         }
         return w;
@@ -692,17 +700,36 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Param
         }
         if (tok < __ldg(a.cu_q + lo) || tok >= __ldg(a.cu_q + lo + 1)) return;
     }
+    // maxima and sums: a part a lane, then the outputs with their factors
     const int64_t step = a.tokens * a.n_heads;
-    float m = -INFINITY, total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[s * step + unit].x);
-    for (int s = 0; s < p.splits; ++s) {
-        const float2 ml = p.part_ml[s * step + unit];
-        if (ml.y == 0.f) continue;                           // nothing seen in this part
-        const float f = ml.x == m ? 1.f : exp2_approx(ml.x - m);
-        total = fmaf(f, ml.y, total);
+    constexpr int U = kMaxSplits / 32;
+    float2 ml[U];
+    float m = -INFINITY, total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f}, f[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (lane + 32 * j < a.head_dim) o[j] = fmaf(f, p.part_o[(s * step + unit) * a.head_dim + lane + 32 * j], o[j]);
+    for (int u = 0; u < U; ++u) {
+        ml[u] = 32 * u + lane < p.splits ? __ldcg(p.part_ml + (32 * u + lane) * step + unit) : make_float2(-INFINITY, 0.f);
+        m = fmaxf(m, ml[u].x);
+    }
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        f[u] = ml[u].y == 0.f ? 0.f : ml[u].x == m ? 1.f : exp2_approx(ml[u].x - m);      // 0: nothing seen in this part
+        total = fmaf(f[u], ml[u].y, total);
+    }
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll 4
+        for (int s = 32 * u; s < min(p.splits, 32 * u + 32); ++s) {
+            const float g = __shfl_sync(0xffffffffu, f[u], s - 32 * u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float v = lane + 32 * j < a.head_dim ? __ldcg(p.part_o + (s * step + unit) * a.head_dim + lane + 32 * j) : 0.f;
+                o[j] = g == 0.f ? o[j] : fmaf(g, v, o[j]);
+            }
+        }
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
@@ -718,7 +745,7 @@ int check(const rvq_prompt_attn_args* a) {
     if (a->n_kv < 1 || a->n_heads < a->n_kv || a->n_heads % a->n_kv != 0) return RVQ_ERR_INVALID;
     if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8 || a->n_heads / a->n_kv > 64) return RVQ_ERR_UNSUPPORTED;
     if (a->kind != RVQ_BF16 && a->kind != RVQ_F16) return RVQ_ERR_UNSUPPORTED;
-    if (a->tokens >= (1ll << 31) || a->keys >= (1ll << 31)) return RVQ_ERR_TOO_LARGE;
+    if (a->tokens > (1ll << 30) || a->keys > (1ll << 30)) return RVQ_ERR_TOO_LARGE;
     if (a->tokens > 0 && (a->q == nullptr || a->out == nullptr)) return RVQ_ERR_INVALID;
     if (a->keys > 0 && (a->k == nullptr || a->v == nullptr)) return RVQ_ERR_INVALID;
     if (a->cu_q == nullptr && (a->n_seq != 1 || a->cu_k != nullptr)) return RVQ_ERR_INVALID;
@@ -796,7 +823,8 @@ int plan(const rvq_prompt_attn_args& a, Params* p) {
     const int64_t units = pairs * a.n_kv, tiles = (a.keys / a.n_seq + kKeys - 1) / kKeys;
     if (units * 2 <= sms && tiles >= 8) {
         const int64_t most = sms / units, parts = tiles / 4;
-        p->splits = (int32_t)(most < parts ? most : parts);
+        const int64_t s = most < parts ? most : parts;
+        p->splits = (int32_t)(s < kMaxSplits ? s : kMaxSplits);
     }
     p->sms = sms;
     p->units = (int32_t)(units * p->splits);

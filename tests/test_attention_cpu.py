@@ -89,6 +89,18 @@ def test_prompt_refuses_overlap():
         prompt(q=q, out=q)
 
 
+def test_refuses_outputs_that_overlap_themselves():
+    buf = z(4096)
+    for st in ((64, 8, 1), (8, 64, 1), (256, 56, 1), (200, 64, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            prompt(out=torch.as_strided(buf, (6, 4, 64), st))
+        with pytest.raises(ValueError, match="overlap"):
+            Cache4ReadOp(Cache4(1, 4, 8, 64), torch.as_strided(buf, (6, 4, 64), st), z(6, 4, 64))
+    for st in ((256, 64, 1), (64, 384, 1), (264, 64, 1)):
+        with pytest.raises(ValueError, match="CUDA"):
+            prompt(out=torch.as_strided(buf, (6, 4, 64), st))
+
+
 def test_interleaved_views():
     """Against the elements themselves, over many pairs of views of one buffer."""
     buf = torch.arange(4000)
@@ -256,7 +268,7 @@ def test_c_prompt_checks():
     assert c_prompt(q=None) == INV and c_prompt(k=None) == INV and c_prompt(v=24) == INV
     assert c_prompt(n_kv=3) == INV and c_prompt(n_kv=0) == INV and c_prompt(n_seq=0) == INV and c_prompt(n_seq=2) == INV
     assert c_prompt(head_dim=136) == UNS and c_prompt(head_dim=20) == UNS and c_prompt(kind=_native.RVQ_F32) == UNS
-    assert c_prompt(n_heads=130) == UNS and c_prompt(tokens=1 << 31) == BIG
+    assert c_prompt(n_heads=130) == UNS and c_prompt(tokens=(1 << 30) + 1) == BIG and c_prompt(keys=(1 << 30) + 1) == BIG
     assert c_prompt(q_stride=(ctypes.c_int64 * 2)(256, 68)) == INV
     assert c_prompt(out_stride=(ctypes.c_int64 * 2)(-256, 64)) == INV
     assert c_prompt(tokens=0) == _native.RVQ_OK

@@ -193,6 +193,13 @@ def test_prompt_long(cuda_device):
     prompt_case(cuda_device, [9], 8, 2, 64, BF, False, prefix=30000, seed=4)
 
 
+def test_prompt_many_sequences(cuda_device):
+    """More sequences than a warp has lanes, most of them short or empty, in front of and behind long ones."""
+    lens = [1, 0, 2] * 70 + [300] + [0, 5] * 40 + [130] + [1] * 33
+    prompt_case(cuda_device, lens, 4, 2, 64, BF, True, seed=6)
+    prompt_case(cuda_device, [0] * 100 + [70] + [0] * 100, 16, 2, 128, HF, False, seed=7)
+
+
 def test_prompt_bad_offsets_stay_in_bounds(cuda_device):
     """Offsets beyond the tensors are cut off at them."""
     dev = cuda_device

@@ -23,10 +23,19 @@ using sm100::smem_addr;
 //
 // so an operand is a 4-bit code (exact), never a rounded value; the sums with
 // the zeros are one more MMA each, on the parameter words as they lie there.
-// p step is split into two bf16 parts (16 bits), q . 1 into three (24 bits), an
-// fp16 q into two (exact).  Softmax: one pass, running maximum and sum per warp;
+// p step is split into two bf16 parts (16 bits), q . 1 into three (24 bits).  Softmax: one pass, running maximum and sum per warp;
 // partial results are joined in fixed order, warp by warp in the CTA and range
 // by range in a second launch, so results do not depend on scheduling.
+//
+// Bound by the issue of integer instructions (masks, shifts, conversions: of about
+// 540 instructions a tile 250 on the ALU pipe, 55 % of its peak, issue 60 %), not by
+// HBM: 64 sequences of 4,096 rows, 64/8 heads of 128, 113 us, 2.96 TB/s of records
+// (45 % of measured copy bandwidth).  One sequence of 40,000 rows with weights:
+// 27 us; of 300 rows: 9.9 us, a chain of latencies (row count, copies, one tile,
+// the joins).  Measured against this form: clusters of CTAs joining over
+// distributed shared memory left SMs idle (40,000 rows: 54 us); bulk copies with
+// mbarriers cost more instructions than cp.async (64 x 4,096: 154 against 134 us);
+// the heads as the M of both MMAs left half the operand rows zero (118 against 129).
 // ---------------------------------------------------------------------------
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
@@ -58,6 +67,14 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
     return r;
 }
 
+// The same as fp16 numbers, c / 512 (a code in the lowest 10 bits is a subnormal number): against an fp16 q.
+template <int I>
+__device__ __forceinline__ uint32_t code_pair_half(uint32_t w) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w & (I ? 0x00f000f0u : 0x000f000fu)), "r"(I ? 0x68006800u : 0x78007800u));
+    return r;
+}
+
 // Numbers of a parameter word: the shift as a multiplication (`shift` holds 65536 where the compiler cannot see it), which
 // runs on the FMA pipe; the masks and shifts of this kernel's integer pipe are what bounds it.
 __device__ __forceinline__ float zero_by(uint32_t p, uint32_t shift) {
@@ -67,19 +84,29 @@ __device__ __forceinline__ float zero_by(uint32_t p, uint32_t shift) {
 }
 
 // D += A B, and D = A B
+template <bool kHalf = false>
 __device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if constexpr (kHalf)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+template <bool kHalf = false>
 __device__ __forceinline__ void mma_set(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    if constexpr (kHalf)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -133,11 +160,11 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[G], uint32_t addr) {
 // A tile of 16 rows, `valid` of them live (the records behind those hold zeros).  The rows are the M of the scores'
 // MMA and the K of the output's, the heads the N of both; between the two the probabilities, heads along the lanes'
 // registers, are transposed to rows along them.
-template <int HD, bool kSplitQ>
-__device__ __forceinline__ void tile_step(uint32_t base, int valid, const uint32_t (&qa)[HD / 16][kSplitQ ? 4 : 2],
-                                          const uint32_t (&qz)[3], float scale64, uint32_t shift, State<HD>& st,
+template <int HD, bool kHalfQ>
+__device__ __forceinline__ void tile_step(uint32_t base, int valid, const uint32_t (&qa)[HD / 16][2],
+                                          const uint32_t (&qz)[3], float scale, uint32_t shift, State<HD>& st,
                                           bool keep, float* const (&scores)[2]) {
-    constexpr int G = HD / kGroup, REC = record_bytes(HD), kLo = kSplitQ ? 2 : 0;
+    constexpr int G = HD / kGroup, REC = record_bytes(HD);
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // row g of an MMA is row (g with its two low bits swapped) of the tile: a quarter warp's 16-byte loads of two rows then
     // fall into different banks; rows 2 t and 2 t + 1 are so ra and ra + 2
@@ -153,26 +180,17 @@ __device__ __forceinline__ void tile_step(uint32_t base, int valid, const uint32
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(z1) : "r"(r1 + HD + 4 * (t & (G - 1))));
         load_words<G>(p0, r0 + HD);
         load_words<G>(p1, r1 + HD);
-        float z[4], c[G][4];                                 // zero . (q . 1) / 64; q . c / 64 of every group
+        float z[4], c[G][4];                                 // zero . (q . 1) and q . c of every group, over 64 (512 for fp16)
+        auto c0 = [](uint32_t w) { return kHalfQ ? code_pair_half<0>(w) : code_pair<0>(w); };
+        auto c1 = [](uint32_t w) { return kHalfQ ? code_pair_half<1>(w) : code_pair<1>(w); };
         mma_set(z, z0, z1, z0, z1, qz[0], qz[1]);
 #pragma unroll
-        for (int i = 0; i < G; ++i)
-            mma_set(c[i], code_pair<0>(k0[i]), code_pair<0>(k1[i]), code_pair<1>(k0[i]), code_pair<1>(k1[i]), qa[2 * i][0], qa[2 * i][1]);
-        if constexpr (kSplitQ) {
-#pragma unroll
-            for (int i = 0; i < G; ++i)
-                mma_add(c[i], code_pair<0>(k0[i]), code_pair<0>(k1[i]), code_pair<1>(k0[i]), code_pair<1>(k1[i]), qa[2 * i][kLo], qa[2 * i][kLo + 1]);
-        }
+        for (int i = 0; i < G; ++i) mma_set<kHalfQ>(c[i], c0(k0[i]), c0(k1[i]), c1(k0[i]), c1(k1[i]), qa[2 * i][0], qa[2 * i][1]);
         mma_add(z, z0, z1, z0, z1, qz[2], 0u);
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             k0[i] >>= 8, k1[i] >>= 8;
-            mma_add(c[i], code_pair<0>(k0[i]), code_pair<0>(k1[i]), code_pair<1>(k0[i]), code_pair<1>(k1[i]), qa[2 * i + 1][0], qa[2 * i + 1][1]);
-        }
-        if constexpr (kSplitQ) {
-#pragma unroll
-            for (int i = 0; i < G; ++i)
-                mma_add(c[i], code_pair<0>(k0[i]), code_pair<0>(k1[i]), code_pair<1>(k0[i]), code_pair<1>(k1[i]), qa[2 * i + 1][kLo], qa[2 * i + 1][kLo + 1]);
+            mma_add<kHalfQ>(c[i], c0(k0[i]), c0(k1[i]), c1(k0[i]), c1(k1[i]), qa[2 * i + 1][0], qa[2 * i + 1][1]);
         }
 #pragma unroll
         for (int i = 0; i < G; ++i) {
@@ -181,7 +199,7 @@ __device__ __forceinline__ void tile_step(uint32_t base, int valid, const uint32
             z[2] = fmaf(y, c[i][2], z[2]), z[3] = fmaf(y, c[i][3], z[3]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = z[i] * scale64;
+        for (int i = 0; i < 4; ++i) s[i] = z[i] * scale;
     }
     if (valid < 16) {
         if (rn >= valid) s[0] = s[1] = -INFINITY;
@@ -329,7 +347,7 @@ __device__ __forceinline__ int state_of(const rvq_cache4_attn_args& a, int64_t r
     return rows + append >= 1 && rows + append <= a.cache.max_len && pos >= 0 && (a.pos == nullptr || pos < a.table_len);
 }
 
-template <int HD, bool kSplitQ>
+template <int HD, bool kHalfQ>
 __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_attn_args a, Work work) {
     constexpr int G = HD / kGroup, REC = record_bytes(HD);
     extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -420,25 +438,20 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
     if (owner && group == 0 && tid < REC / 16)
         reinterpret_cast<uint4*>(cache + rows * REC)[tid] = reinterpret_cast<const uint4*>(S.fresh)[tid];
 
-    // column g of the operand: q of head g (its bf16 part, then the remainder), in pairs in the code words' order
-    uint32_t qa[HD / 16][kSplitQ ? 4 : 2];
-    // (q . 1) / 64 of group t against the pairs (zero, step), in three bf16 parts: 24 bits
-    uint32_t qz[3] = {0u, 0u, 0u};
+    // column g of the operand: q of head g, in pairs in the code words' order; and (q . 1) of group t against the pairs
+    // (zero, step), in three bf16 parts: 24 bits
+    constexpr float kUnit = kHalfQ ? 512.f : 64.f;
+    uint32_t qa[HD / 16][2], qz[3] = {0u, 0u, 0u};
     if (t < G) {
-        const float x = S.qsum[g][t] * 0.015625f;
+        const float x = S.qsum[g][t] * (1.f / kUnit);
         const float hi = bf16r(x), lo = bf16r(x - hi);
         qz[0] = pack_bf16(hi, 0.f), qz[1] = pack_bf16(lo, 0.f), qz[2] = pack_bf16(x - hi - lo, 0.f);
     }
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) {
         const float* q = &S.q[g][i / 2 * kGroup + 8 * t + 2 * (i & 1)];
-        if constexpr (kSplitQ) {
-            split_bf16(q[0], q[4], &qa[i][0], &qa[i][2], 65536u);
-            split_bf16(q[1], q[5], &qa[i][1], &qa[i][3], 65536u);
-        } else {
-            qa[i][0] = pack_bf16(q[0], q[4]);
-            qa[i][1] = pack_bf16(q[1], q[5]);
-        }
+        qa[i][0] = pack2(q[0], q[4], kHalfQ ? RVQ_F16 : RVQ_BF16);
+        qa[i][1] = pack2(q[1], q[5], kHalfQ ? RVQ_F16 : RVQ_BF16);
     }
     State<HD> st;
     st.m[0] = st.m[1] = -INFINITY, st.l[0] = st.l[1] = 0.f;
@@ -450,13 +463,13 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int c = 0; c < 4; ++c) st.o[i][j][c] = 0.f;
-    const float scale64 = a.scaling * 64.f * 1.4426950408889634f;      // scores in powers of two
+    const float scale = a.scaling * kUnit * 1.4426950408889634f;       // scores in powers of two
     float* sc[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         sc[i] = a.weights != nullptr && 2 * t + i < heads ? work.scores + (head0 + 2 * t + i) * a.cache.max_len : nullptr;
-    // the last warp begins with the appended record
-    bool extra = owner && warp == kWarps - 1;
+    // the warp whose turn it would be after the last tile takes the appended record, first
+    bool extra = owner && warp == (t1 - t0) % kWarps;
     for (int tile = t0 + warp, stage = 0; tile < t1 || extra;) {
         uint32_t rec = smem_addr(S.fresh);
         int row = live, valid = 1;
@@ -472,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
         }
         extra = false;
         float* const at[2] = {sc[0] ? sc[0] + row : nullptr, sc[1] ? sc[1] + row : nullptr};
-        tile_step<HD, kSplitQ>(rec, valid, qa, qz, scale64, shift, st, a.weights != nullptr, at);
+        tile_step<HD, kHalfQ>(rec, valid, qa, qz, scale, shift, st, a.weights != nullptr, at);
     }
     // the lanes with the same t hold parts of heads 2 t and 2 t + 1
 #pragma unroll
@@ -664,9 +677,9 @@ void sizes(const rvq_cache4_attn_args& a, int splits, size_t (&n)[3]) {
     n[2] = a.weights != nullptr ? heads * a.cache.max_len * sizeof(float) : 0;
 }
 
-template <int HD, bool kSplitQ>
+template <int HD, bool kHalfQ>
 int run(const rvq_cache4_attn_args& a, const Work& work, cudaStream_t s) {
-    auto* kernel = cache4_attn_kernel<HD, kSplitQ>;
+    auto* kernel = cache4_attn_kernel<HD, kHalfQ>;
     const int smem = (int)sizeof(Smem<HD>), rep = a.n_heads / a.cache.n_kv, groups = (rep + kHeads - 1) / kHeads;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)

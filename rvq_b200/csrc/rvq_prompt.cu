@@ -20,25 +20,35 @@ __device__ int g_attention_timeout;          // sticky: a bounded wait gave up
 // A CTA takes 2 tiles of 128 operand rows of one kv head and walks the keys in
 // tiles of 128.  A row is (token, query head of the kv head): a tile holds
 // 128 / rep tokens with all their rep heads, so grouped heads share every K and
-// V tile and short sequences fill the rows.  Roles by warp: 0-3 and 4-7 the
-// softmax of the two tiles (a thread per row), 8 the TMA loads, 9 the MMAs.
+// V tile and short sequences fill the rows.  Roles by warp: 0-7 and 8-15 the
+// softmax of the two tiles (two threads a row, 64 columns each), 16 the TMA
+// loads, 17 (one thread) the MMAs.
 //
 //   S = Q K^T       tcgen05.mma, both operands in shared memory, S in TMEM
-//   P = 2^(c S - m) a row per thread, fp32; rounded to the operand type and
-//                   written over S in TMEM
+//   P = 2^(c S - m) fp32; rounded to the operand type and written over S in TMEM
 //   O += P V        tcgen05.mma, P from TMEM, V as it lies in shared memory
 //
-// A CTA takes such pairs of tiles one after the other (the longest first, by a
-// ticket from the second on); the next one's loads and its first S run beside this
-// one's last softmax and output.  While one tile's softmax runs, the tensor cores
-// work for the other one.  The
-// maximum that is subtracted only follows the true one when that has grown by
-// 2^8: O is then rescaled by the row's own thread, which is rare after the first
-// tiles; p stays below 2^8, exact in fp32 sums and with unchanged relative rounding.
-// Keys of other tokens that a tile brings along (behind the sequence, later
+// While one tile's softmax runs, the tensor cores work for the other one.  A CTA
+// takes such pairs of tiles one after the other (by a ticket from the second on,
+// the longest of a causal sequence first); the next one's loads and its first S
+// run beside this one's last softmax and output.
+//
+// The maximum that is subtracted only follows the true one when that has grown by
+// 2^8: O is then rescaled by the row's own threads, which is rare after the first
+// tiles; p stays below 2^8, and its rounding to the operand type, half a step
+// relative, is the same at any size (the sums take p unrounded).
+// Keys that a tile brings along but a row does not see (behind the sequence, later
 // than the query) get p = 0; values behind the sequence are zeroed in shared
 // memory, and a row that came out non-finite is looked at again (repair), so
 // that no hidden NaN or infinity reaches it through 0 * NaN.
+//
+// Bound by the chain S -> softmax -> P -> PV -> S of a tile: of 3,570 clocks a step of
+// both tiles the tensor cores work 2,048 (timestamps of one CTA: softmax 1,880, of
+// which the exponentials 1,300; PV and S 1,030; waits 300).  8,192 tokens, 32/8 heads
+// of 128: causal 466 us, 1,180 TFLOP/s (71 % of the measured matrix peak, 84 % of the
+// sustained one), not causal 876 us, 1,255.  Tried: a thread a row with its 128 columns
+// (1,094 not causal, before the MMA warp became one thread); a quarter or half of the
+// exponentials as a polynomial on the FMA pipe (no faster: registers spill).
 // ---------------------------------------------------------------------------
 constexpr int kRows = 128;                   // operand rows of a tile (MMA M)
 constexpr int kKeys = 128;                   // keys of a tile

@@ -197,7 +197,7 @@ class _Op:
         """Allocates what ``self.args`` needs; its bytes."""
         with torch.cuda.device(self.device):
             n = size(ctypes.byref(self.args))
-        self._ws = torch.zeros(n, dtype=torch.uint8, device=self.device) if n else None
+        self._ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
         return n
 
     def _bind(self, where: str, *args) -> None:
@@ -273,7 +273,17 @@ class PromptAttentionOp(_Op):
                                       keys, _strides(q), _strides(k), _strides(v), _strides(out), n_seq, nh, nkv, hd,
                                       float(scaling), int(bool(causal)), _native.kind_of(q), 0)
         n = self._workspace(_lib().rvq_prompt_attention_workspace_size)
+        self._fresh = n > 0
         self._bind("rvq_prompt_attention", ctypes.byref(self.args), _ptr(self._ws), n)
+
+    def launch(self) -> None:
+        if self._fresh:
+            # the workspace is zero-filled in front of its first call, on that call's stream (this one may not be the one the
+            # op was built on); a capture only records that, so the first call outside of one does it again
+            with torch.cuda.device(self.device):
+                self._ws.zero_()
+                self._fresh = torch.cuda.is_current_stream_capturing()
+        super().launch()
 
 
 class Cache4:

@@ -656,6 +656,38 @@ def test_captured_graphs_replay(cuda_device):
     assert not take_timeout()
 
 
+def test_prompt_workspace_on_the_stream_of_its_first_launch(cuda_device):
+    """More pairs of tiles than SMs (they are given out by a counter in the workspace, which starts as whatever the memory
+    held): an op built on one stream and launched on another, one whose first launch is captured, then both again."""
+    dev = cuda_device
+    g = gen(dev, 61)
+    q, k, v = randn(g, 1500, 32, 64), randn(g, 1500, 8, 64), randn(g, 1500, 8, 64)
+    want, _, tol, _ = ref.attend(q, k, v, 0.125, True)
+    junk = [torch.full((n,), 255, dtype=torch.uint8, device=dev) for n in (8, 16, 512)]
+    torch.cuda.synchronize()
+    del junk
+    out = torch.zeros_like(q)
+    op = PromptAttentionOp(q, k, v, out, scaling=0.125)
+    side = torch.cuda.Stream(dev)
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            op.launch()
+    torch.cuda.synchronize()
+    check(out, want, tol)
+    junk = [torch.full((n,), 255, dtype=torch.uint8, device=dev) for n in (8, 16, 512)]
+    torch.cuda.synchronize()
+    del junk
+    op = PromptAttentionOp(q, k, v, out, scaling=0.125)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        op.launch()
+    for how in (op.launch, graph.replay, graph.replay, op.launch, graph.replay):
+        out.zero_()
+        how()
+        check(out, want, tol)
+    assert not take_timeout()
+
+
 def test_two_streams_at_once(cuda_device):
     """The same kinds of op with their own buffers on two streams at the same time."""
     dev = cuda_device

@@ -123,17 +123,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-
 // 8 consecutive 32-bit columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
@@ -197,7 +186,7 @@ __device__ __forceinline__ float row_max(float (&s)[2][32], int seen) {
     return fmaxf(max3(t[0], t[1], t[2]), t[3]);
 }
 
-// p = 2^(c s - sub) over the scores in TMEM, in the operand type; returns their sum.
+// p = 2^(c s - sub) in the operand type, over scores in TMEM at ts; returns their sum.
 template <bool kMasked, bool kHalfType>
 __device__ __forceinline__ float row_exp(float (&s)[2][32], int seen, float c, float sub, uint32_t ts) {
     float part[4] = {0.f, 0.f, 0.f, 0.f};

@@ -31,8 +31,8 @@ using sm100::smem_addr;
 // 540 instructions a tile 250 on the ALU pipe, 55 % of its peak, issue 60 %), not by
 // HBM: 64 sequences of 4,096 rows, 64/8 heads of 128, 113 us, 2.96 TB/s of records
 // (45 % of measured copy bandwidth).  One sequence of 40,000 rows with weights:
-// 27 us; of 300 rows: 9.9 us, a chain of latencies (row count, copies, one tile,
-// the joins).  Measured against this form: clusters of CTAs joining over
+// 27 us; of 300 rows: 7.5 us, a chain of latencies (row count, copies, three tiles,
+// the join of the warps).  Measured against this form: clusters of CTAs joining over
 // distributed shared memory left SMs idle (40,000 rows: 54 us); bulk copies with
 // mbarriers cost more instructions than cp.async (64 x 4,096: 154 against 134 us);
 // the heads as the M of both MMAs left half the operand rows zero (118 against 129).
@@ -55,6 +55,7 @@ struct Smem {
     float kv[2][HD];                         // the new key and value
     float norm[4][HD];
     float wm[kWarps][kHeads], wl[kWarps][kHeads];
+    float m[kHeads], r[kHeads];              // of the heads joined: maximum and reciprocal sum
 };
 
 // c / 64 for the codes c in bits 4 I .. and 4 I + 16 .. (I = 0 or 1) of a word, as a bf16 pair.  A code in a bf16
@@ -347,6 +348,42 @@ __device__ __forceinline__ int state_of(const rvq_cache4_attn_args& a, int64_t r
     return rows + append >= 1 && rows + append <= a.cache.max_len && pos >= 0 && (a.pos == nullptr || pos < a.table_len);
 }
 
+constexpr int kRowLoads = 4;                 // rows of a thread in add_weights
+constexpr int kJoinRows = kRowLoads * kThreads;
+
+// Whether a CTA, which has all rows and all heads of its kv head, adds the weights itself, in one go: 64 x 8 heads of 500 rows
+// 31.5 -> 28.5 us.  Longer caches leave it to the second launch: of 4,096 rows 154 us, here 165.
+__host__ __device__ __forceinline__ bool weights_here(const rvq_cache4_attn_args& a, int splits) {
+    return splits == 1 && a.n_heads / a.cache.n_kv <= kHeads && a.cache.max_len <= kJoinRows;
+}
+
+// The weights of rows [first, first + kRowLoads * kThreads) below n: those from before (`was`; the appended row's: none)
+// and the heads', in order; m and r: the heads' maxima and reciprocal sums (0: nothing seen).
+__device__ __forceinline__ void old_weights(float (&was)[kRowLoads], const float* w, int64_t first, int64_t n, int64_t appended) {
+#pragma unroll
+    for (int u = 0; u < kRowLoads; ++u) {
+        const int64_t row = first + u * kThreads + threadIdx.x;
+        was[u] = row < n && row != appended ? __ldcg(w + row) : 0.f;
+    }
+}
+__device__ __forceinline__ void add_weights(float (&was)[kRowLoads], float* w, const float* scores, int64_t max_len, int64_t first,
+                                            int64_t n, int heads, const float* m, const float* r) {
+#pragma unroll 4
+    for (int h = 0; h < heads; ++h) {
+#pragma unroll
+        for (int u = 0; u < kRowLoads; ++u) {
+            const int64_t row = first + u * kThreads + threadIdx.x;
+            const float s = row < n ? __ldcg(scores + h * max_len + row) : 0.f;
+            if (r[h] != 0.f) was[u] += exp2_approx(s - m[h]) * r[h];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kRowLoads; ++u) {
+        const int64_t row = first + u * kThreads + threadIdx.x;
+        if (row < n) w[row] = was[u];
+    }
+}
+
 template <int HD, bool kHalfQ>
 __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_attn_args a, Work work) {
     constexpr int G = HD / kGroup, REC = record_bytes(HD);
@@ -355,8 +392,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int nkv = a.cache.n_kv, rep = a.n_heads / nkv;
     const int split = blockIdx.x, kv = blockIdx.y % nkv, group = blockIdx.y / nkv, b = blockIdx.z;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();                                 // after the wait: the join may read what this kernel does not write
     const int64_t rows = a.rows[b], pos = a.pos != nullptr ? a.pos[b] : 0;
     const bool append = a.k.ptr != nullptr;
     const int groups = (rep + kHeads - 1) / kHeads, per = (rep + groups - 1) / groups;
@@ -510,36 +547,45 @@ __global__ void __launch_bounds__(kThreads, 2) cache4_attn_kernel(rvq_cache4_att
     if (g < 2) S.wm[warp][2 * t + g] = g ? st.m[1] : st.m[0], S.wl[warp][2 * t + g] = g ? st.l[1] : st.l[0];
     __syncthreads();
     // warp w joins head w over the warps
-    if (warp >= heads) return;
-    float m = S.wm[0][warp];
+    if (warp < heads) {
+        float m = S.wm[0][warp];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, S.wm[w][warp]);
-    float total = 0.f, o[HD / 32];
+        for (int w = 1; w < kWarps; ++w) m = fmaxf(m, S.wm[w][warp]);
+        float total = 0.f, o[HD / 32];
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
+        for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const float f = S.wm[w][warp] == m ? 1.f : exp2_approx(S.wm[w][warp] - m);
-        total = fmaf(f, S.wl[w][warp], total);
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = S.wm[w][warp] == m ? 1.f : exp2_approx(S.wm[w][warp] - m);
+            total = fmaf(f, S.wl[w][warp], total);
 #pragma unroll
-        for (int d = 0; d < HD / 32; ++d) o[d] = fmaf(f, wo[(w * kHeads + warp) * HD + 32 * d + lane], o[d]);
+            for (int d = 0; d < HD / 32; ++d) o[d] = fmaf(f, wo[(w * kHeads + warp) * HD + 32 * d + lane], o[d]);
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;  // no score above -infinity: zeros
+        if (lane == 0) ml[warp] = make_float2(m, total), S.m[warp] = m, S.r[warp] = inv;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) {
+            if (work.splits == 1)
+                store_from_f32(a.out, q_at + warp * HD + 32 * d + lane, out_kind, inv == 0.f ? 0.f : o[d] * inv);
+            else
+                work.o[((int64_t)split * a.cache.n_seq * a.n_heads + head0 + warp) * HD + 32 * d + lane] = o[d];
+        }
     }
-    if (lane == 0) ml[warp] = make_float2(m, total);
-    const float inv = total == 0.f ? 0.f : 1.f / total;      // no score above -infinity: zeros
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d) {
-        if (work.splits == 1)
-            store_from_f32(a.out, q_at + warp * HD + 32 * d + lane, out_kind, inv == 0.f ? 0.f : o[d] * inv);
-        else
-            work.o[((int64_t)split * a.cache.n_seq * a.n_heads + head0 + warp) * HD + 32 * d + lane] = o[d];
+    if (a.weights != nullptr && weights_here(a, work.splits)) {
+        __syncthreads();
+        float* w = a.weights + ((int64_t)b * nkv + kv) * a.cache.max_len;
+        const int64_t n = live + (a.k.ptr != nullptr);
+        float was[kRowLoads];
+        old_weights(was, w, 0, n, a.k.ptr != nullptr ? live : -1);
+        add_weights(was, w, work.scores + head0 * a.cache.max_len, a.cache.max_len, 0, n, heads, S.m, S.r);
     }
 }
 
 // The ranges joined.  Blocks x < out_blocks: 256 output values of the kv head's query heads each; the others: the weights of
 // kJoinRows rows each, heads in order.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 1024;
+constexpr int kJoinThreads = kThreads;
 constexpr int kMaxSplits = 320;              // plan keeps below it
+constexpr int kEarly = 16;
 
 // Maximum and sum of a head over the ranges, by one warp; with f, the ranges' factors (0 for an empty one).
 __device__ __forceinline__ float2 join_head(const float2* ml, int64_t step, int splits, float* f) {
@@ -568,61 +614,50 @@ __global__ void __launch_bounds__(kJoinThreads) cache4_join_kernel(rvq_cache4_at
     constexpr int kBlockHeads = kJoinThreads / 64;           // heads that 256 output values may touch
     __shared__ float fm[kMaxRep], fr[kMaxRep], f[kBlockHeads][kMaxSplits];
     pdl_launch_dependents();
-    pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkv = a.cache.n_kv, rep = a.n_heads / nkv, hd = a.cache.head_dim;
     const int kv = blockIdx.y, b = blockIdx.z;
-    const int64_t rows = a.rows[b], pos = a.pos != nullptr ? a.pos[b] : 0;
+    // the rows and the weights are not the first kernel's, and what came before is complete (it waited for that): these loads
+    // run before its end
+    const int64_t rows = __ldcg(a.rows + b), pos = a.pos != nullptr ? __ldcg(a.pos + b) : 0;
     const int64_t head0 = (int64_t)b * a.n_heads + kv * rep, all = (int64_t)a.cache.n_seq * a.n_heads;
     const bool append = a.k.ptr != nullptr;
     const int64_t n = rows + append, first = (int64_t)((int)blockIdx.x - out_blocks) * kJoinRows;
-    const bool output = first < 0;
-    if (!output && first >= n) return;
+    const bool output = first < 0, used = state_of(a, rows, pos) == 1 && (output || first < n);
+    float* w = a.weights + ((int64_t)b * nkv + kv) * a.cache.max_len;
+    float was[kRowLoads];
+    if (used && !output) old_weights(was, w, first, n, append ? rows : -1);
+    pdl_wait();
+    if (!used) return;
+    // the first ranges' outputs come with their maxima and sums
+    const int at = blockIdx.x * kJoinThreads + tid;
+    const bool mine = output && at < rep * hd;
+    const float* o = work.o + head0 * hd + at;
+    float early[kEarly];
+#pragma unroll
+    for (int s = 0; s < kEarly; ++s) early[s] = mine && s < work.splits ? __ldcg(o + s * all * hd) : 0.f;
     const int h0 = output ? blockIdx.x * (kJoinThreads / hd) : 0, h1 = output ? min(rep, h0 + kJoinThreads / hd) : rep;
     for (int h = h0 + warp; h < h1; h += kJoinThreads / 32) {
         const float2 x = join_head(work.ml + head0 + h, all, work.splits, output ? f[h - h0] : nullptr);
         if (lane == 0) fm[h] = x.x, fr[h] = x.y == 0.f ? 0.f : 1.f / x.y;
     }
     __syncthreads();
-    if (state_of(a, rows, pos) != 1) return;                 // (what was joined then is not used)
-    if (output) {
-        const int i = blockIdx.x * kJoinThreads + tid, h = i / hd;
-        if (i >= rep * hd) return;
-        const float* o = work.o + head0 * hd + i;
-        const float* g = f[h - h0];
-        float sum = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < work.splits; ++s) {
-            const float v = __ldcg(o + s * all * hd);        // of an empty range: whatever is there
-            sum = g[s] == 0.f ? sum : fmaf(g[s], v, sum);
-        }
-        store_from_f32(a.out, head0 * hd + i, a.q.kind == RVQ_F16 ? RVQ_F16 : RVQ_BF16, fr[h] == 0.f ? 0.f : sum * fr[h]);
+    if (!output) {
+        add_weights(was, w, work.scores + head0 * a.cache.max_len, a.cache.max_len, first, n, rep, fm, fr);
         return;
     }
-    float* w = a.weights + ((int64_t)b * nkv + kv) * a.cache.max_len;
-    const float* sc = work.scores + head0 * a.cache.max_len;
-    constexpr int U = kJoinRows / kJoinThreads;
-    float v[U];
+    if (!mine) return;
+    const int h = at / hd;
+    const float* g = f[h - h0];
+    float sum = 0.f;                                         // of an empty range: whatever is there
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t row = first + u * kJoinThreads + tid;
-        v[u] = row < n && !(append && row == rows) ? w[row] : 0.f;
+    for (int s = 0; s < kEarly; ++s) sum = s >= work.splits || g[s] == 0.f ? sum : fmaf(g[s], early[s], sum);
+#pragma unroll 8
+    for (int s = kEarly; s < work.splits; ++s) {
+        const float v = __ldcg(o + s * all * hd);
+        sum = g[s] == 0.f ? sum : fmaf(g[s], v, sum);
     }
-#pragma unroll 4
-    for (int h = 0; h < rep; ++h) {
-        const float m = fm[h], r = fr[h];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t row = first + u * kJoinThreads + tid;
-            const float s = row < n ? __ldcg(sc + (int64_t)h * a.cache.max_len + row) : 0.f;
-            if (r != 0.f) v[u] += exp2_approx(s - m) * r;
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t row = first + u * kJoinThreads + tid;
-        if (row < n) w[row] = v[u];
-    }
+    store_from_f32(a.out, head0 * hd + at, a.q.kind == RVQ_F16 ? RVQ_F16 : RVQ_BF16, fr[h] == 0.f ? 0.f : sum * fr[h]);
 }
 
 bool vec_fits(const rvq_vec& v, int64_t n) {
@@ -656,6 +691,8 @@ int check(const rvq_cache4_attn_args* a) {
 // Ranges of the rows: as many CTAs as the SMs hold (two each), and two ranges where that is between one and two (160 heads
 // of 4,096 rows: 45 us whole, 40 us halved; of mixed lengths 38 and 26), but none shorter than a tile for every warp of a
 // full cache.  Above that a range is a whole sequence: halves cost 64 x 8 heads of 4,096 rows 113 -> 120 us.
+// A short cache is one range, which needs no second launch: 8 heads, 300 rows 9.1 -> 7.5 us, 600 rows 9.7 -> 9.5, 750 rows
+// 9.3 -> 10.4; with weights 300 rows 9.5 -> 9.0, 500 rows 10.1 -> 10.9.
 int plan(const rvq_cache4_attn_args& a, int* splits) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -664,7 +701,8 @@ int plan(const rvq_cache4_attn_args& a, int* splits) {
     const int rep = a.n_heads / a.cache.n_kv, groups = (rep + kHeads - 1) / kHeads;
     const int64_t units = (int64_t)a.cache.n_seq * a.cache.n_kv * groups;
     const int64_t most = units > sms && units < 2 * sms ? 2 : 2 * sms / units, parts = (a.cache.max_len + kWarps * kTile - 1) / (kWarps * kTile);
-    const int64_t s = most < parts ? most : parts;
+    const bool alone = parts <= (a.weights == nullptr ? 5 : groups == 1 ? 3 : 0);
+    const int64_t s = alone ? 1 : most < parts ? most : parts;
     *splits = s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : (int)s;
     return RVQ_OK;
 }
@@ -685,7 +723,7 @@ int run(const rvq_cache4_attn_args& a, const Work& work, cudaStream_t s) {
     if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3(work.splits, a.cache.n_kv * groups, a.cache.n_seq), dim3(kThreads), (size_t)smem, s, a, work);
     const int out_blocks = work.splits > 1 ? (rep * HD + kJoinThreads - 1) / kJoinThreads : 0;
-    const int row_blocks = a.weights != nullptr ? (a.cache.max_len + kJoinRows - 1) / kJoinRows : 0;
+    const int row_blocks = a.weights != nullptr && !weights_here(a, work.splits) ? (a.cache.max_len + kJoinRows - 1) / kJoinRows : 0;
     if (e == cudaSuccess && out_blocks + row_blocks > 0)
         e = launch_pdl(cache4_join_kernel, dim3(out_blocks + row_blocks, a.cache.n_kv, a.cache.n_seq), dim3(kJoinThreads), 0, s, a,
                        work, out_blocks);

@@ -365,6 +365,15 @@ def test_step_lengths(rows, dtype, hd, cuda_device):
     step_case(cuda_device, rows, 8, 2, hd, dtype, max(rows) + 9, seed=sum(rows) + hd)
 
 
+@pytest.mark.parametrize("weigh", [False, True])
+@pytest.mark.parametrize("max_len", [128, 129, 384, 385, 640, 641, 1024, 1025])
+@pytest.mark.parametrize("seqs,nh,nkv", [(1, 8, 2), (2, 9, 1), (40, 8, 8)])
+def test_step_short_caches(seqs, nh, nkv, max_len, weigh, cuda_device):
+    # full to the last row, and a few rows of the same cache
+    rows = [max_len - 1 if b % 2 == 0 else max_len // 3 for b in range(seqs)]
+    step_case(cuda_device, rows, nh, nkv, 64, BF, max_len, seed=max_len + seqs, weigh=weigh)
+
+
 @pytest.mark.parametrize("nh,nkv", [(1, 1), (2, 1), (3, 1), (6, 2), (7, 1), (16, 2), (9, 1), (12, 1), (16, 1), (40, 2), (64, 1), (8, 8)])
 def test_step_heads(nh, nkv, cuda_device):
     step_case(cuda_device, [130, 61], nh, nkv, 128, BF, 140, seed=nh)

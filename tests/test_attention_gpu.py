@@ -1,6 +1,8 @@
 """GPU: prompt attention, the 4-bit cache and eviction against plain implementations in 64 bits (tests/_attention.py,
 where the tolerances are derived)."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -53,6 +55,29 @@ def prompt_case(dev, lens, nh, nkv, hd, dtype, causal, prefix=0, seed=0, tail=3,
         check(lse[:, a:a + n], wl, ltol)
         a, b = a + n, b + m
     assert bool((out[T:] == 7).all()) and bool((lse[:, T:] == 7).all())
+
+
+@pytest.mark.parametrize("hd", [16, 72, 80, 128])
+@pytest.mark.parametrize("tokens,prefix", [(70, 0), (9, 3000)])
+def test_prompt_output_alignment(tokens, prefix, hd, cuda_device):
+    """Output rows and a workspace at 16-byte steps that are no 32-byte steps get the same bits."""
+    g = gen(cuda_device, tokens + hd)
+    q, k, v = (randn(g, n, h, hd, dtype=BF) for n, h in ((tokens, 8), (tokens + prefix, 2), (tokens + prefix, 2)))
+    want = torch.empty_like(q)
+    PromptAttentionOp(q, k, v, want, scaling=0.1).launch()
+    value, _, tol, _ = ref.attend(q, k, v, 0.1, True)
+    check(want, value, tol)
+    for lead, gap in ((8, 0), (16, 8), (0, 8), (8, 24)):
+        room = torch.full((tokens, 8, lead + hd + gap), 7.0, dtype=BF, device=cuda_device)
+        out = room[:, :, lead:lead + hd]
+        op = PromptAttentionOp(q, k, v, out, scaling=0.1)
+        if op._ws is not None:
+            held = torch.zeros(op._ws.numel() + 16, dtype=torch.uint8, device=cuda_device)
+            op._bind("rvq_prompt_attention", ctypes.byref(op.args), held.data_ptr() + 16, op._ws.numel())
+        op.launch()
+        assert torch.equal(out, want)
+        assert bool((room[:, :, :lead] == 7).all()) and bool((room[:, :, lead + hd:] == 7).all())
+    assert not take_timeout()
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])

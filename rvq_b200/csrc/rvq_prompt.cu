@@ -45,8 +45,8 @@ __device__ int g_attention_timeout;          // sticky: a bounded wait gave up
 // Bound by the chain S -> softmax -> P -> PV -> S of a tile: of 3,570 clocks a step of
 // both tiles the tensor cores work 2,048 (timestamps of one CTA: softmax 1,880, of
 // which the exponentials 1,300; PV and S 1,030; waits 300).  8,192 tokens, 32/8 heads
-// of 128: causal 466 us, 1,180 TFLOP/s (71 % of the measured matrix peak, 84 % of the
-// sustained one), not causal 876 us, 1,255.  Tried: a thread a row with its 128 columns
+// of 128: causal 463 us, 1,187 TFLOP/s (71 % of the measured matrix peak, 85 % of the
+// sustained one), not causal 877 us, 1,254.  Tried: a thread a row with its 128 columns
 // (1,094 not causal, before the MMA warp became one thread); a quarter or half of the
 // exponentials as a polynomial on the FMA pipe (no faster: registers spill).
 // ---------------------------------------------------------------------------

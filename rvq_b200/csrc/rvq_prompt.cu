@@ -681,9 +681,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             if (valid && half == 0 && whole && a.lse != nullptr)
                 a.lse[(int64_t)h * a.tokens + q0 + tok] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
             if (valid && half == 0 && !whole) p.part_ml[slot] = make_float2(m, limit == 0 ? 0.f : sum);
-            // values between this row's last key and the end of its last tile may have leaked in
+            // values between this row's last key and the end of its last tile may have leaked in (a row without weights has zeros,
+            // one whose sum is infinite or NaN is not finite by itself)
             const int begin = j0 * kKeys, hidden_end = min(lk, (j0 + n) * kKeys), seen_end = min(limit, hidden_end);
-            uint32_t again = __ballot_sync(0xffffffffu, ok && valid && bad && seen_end > begin && seen_end < hidden_end && fabsf(sum) <= 3.4e38f);
+            uint32_t again = __ballot_sync(0xffffffffu, ok && valid && bad && seen_end > begin && seen_end < hidden_end && inv > 0.f);
             while (again) {
                 const int l = __ffs(again) - 1;
                 again &= again - 1;

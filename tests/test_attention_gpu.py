@@ -159,6 +159,29 @@ def test_prompt_hidden_values_may_be_anything(bad, hd, cuda_device):
             assert bool(torch.isnan(out[where:]).all())
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tokens,prefix,first", [(64, 0, 40), (128, 0, 128), (300, 0, 230), (40, 1060, 20), (40, 9000, 40)])
+def test_prompt_scores_of_minus_infinity_beside_hidden_values(tokens, prefix, first, hd, dtype, bad, cuda_device):
+    """The first queries' every score is -infinity (a key channel, where they are positive): zeros, whatever the value of the
+    last token holds.  The ones from `first` on, over the finite keys, are as if the others were not there."""
+    g = gen(cuda_device, tokens + prefix)
+    q, k, v = (randn(g, n, h, hd, dtype=dtype) for n, h in ((tokens, 4), (tokens + prefix, 2), (tokens + prefix, 2)))
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k[:prefix + first, :, 0] = float("-inf")
+    v[-1, 0, 3] = bad
+    v[-1, 1] = bad
+    out, lse = torch.full_like(q, 7.0), torch.full((4, tokens), 7.0, device=cuda_device)
+    PromptAttentionOp(q, k, v, out, scaling=0.1, causal=True, lse=lse).launch()
+    assert not take_timeout()
+    assert bool((out[:first] == 0).all()) and bool(torch.isneginf(lse[:, :first]).all())
+    if first < tokens:
+        want, wl, tol, ltol = ref.attend(q[first:], k[prefix + first:], v[prefix + first:], 0.1, True)
+        check(out[first:], want, tol)
+        check(lse[:, first:], wl, ltol)
+
+
 def test_prompt_large_and_equal_scores(cuda_device):
     """Scores far from zero (the running maximum moves by hundreds), rising and falling along the keys; all equal."""
     dev = cuda_device

@@ -101,6 +101,7 @@ struct Smem {
     int32_t fail[8];                         // of two warps of the same rows one has given up
     uint32_t tmem;
     int32_t dead;                            // a bounded wait gave up
+    int32_t busy;                            // warps that sum rows again
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int c0, int c1, int c2, uint32_t bar) {
@@ -146,13 +147,17 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                  : "memory");
 }
 
-// Bounded wait of a thread; once one wait of the CTA has given up, the others end at once.
+// Bounded wait of a thread; once one wait of the CTA has given up, the others end at once.  The bound does not count while a warp
+// sums rows again (repair), which waits for nothing but may take long.
 template <int HD>
 __device__ __forceinline__ bool wait1(Smem<HD>& S, uint32_t bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     for (int i = 0; i < kWaitPolls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63) == 63 && *(volatile int32_t*)&S.dead) return false;
+        if ((i & 63) == 63) {
+            if (*(volatile int32_t*)&S.dead) return false;
+            if (*(volatile int32_t*)&S.busy) i = 0;
+        }
     }
     atomicExch(&g_attention_timeout, 1);
     *(volatile int32_t*)&S.dead = 1;
@@ -289,47 +294,109 @@ __device__ __forceinline__ Work find_work(const Params& p, int want, int split, 
     return w;
 }
 
-// Output row of a query whose hidden values (keys [n, hidden_end) of the last tiles) may have leaked in, by a whole warp:
-// where one of them is not finite and no seen value in the last tile is NaN, the columns concerned are summed again over
-// the keys [begin, n) that the query sees, one by one; into out (times inv), or into part.
-__device__ __noinline__ void repair(const rvq_prompt_attn_args& a, int64_t tok, int h, int64_t k0, int64_t begin, int64_t n,
+// Element i of a pair of 16-bit numbers.
+template <bool kHalfType>
+__device__ __forceinline__ float half_at(uint32_t w, int i) {
+    if constexpr (kHalfType) return __half2float(__ushort_as_half((uint16_t)(w >> (16 * i))));
+    else return __uint_as_float(i ? w & 0xffff0000u : w << 16);
+}
+
+// A warp's half of the columns of an output row of a query whose hidden values (keys [n, hidden_end) of the last tiles) may have
+// leaked in: where one of them is not finite and no seen value in the last tile is NaN, the column is summed again over the keys
+// [begin, n) that the query sees; into out (times inv), or into part.  A NaN stays: once all such columns are, that is it.  Takes
+// 8 keys at a time, HD / 8 lanes a key for the scores: 16 take registers from the kernel around it (12 packed prompts 215 -> 218
+// us).  Slow, and that is for rows beside values that are not finite only: 2,048 causal tokens of 32/8 heads of 128 whose last
+// value is NaN throughout, 39 ms; 16,384 tokens 340 ms.
+template <int HD, bool kHalfType>
+__device__ __forceinline__ void repair(const rvq_prompt_attn_args& a, int64_t tok, int h, int64_t k0, int64_t begin, int64_t n,
                                     int64_t hidden_end, float c, float m, float inv, float* part) {
+    constexpr int J = HD / 64, L = HD / 8, P = 32 / L, U = 8 / P;
     const int lane = threadIdx.x & 31, g = h / (a.n_heads / a.n_kv), hd = a.head_dim;
-    const int64_t vr = g * a.v_stride[1], kr = g * a.k_stride[1];
-    bool leak[4];
+    const int d0 = (threadIdx.x >> 7 & 1) * (HD / 2) + lane;             // this lane's columns: d0, d0 + 32
+    const int64_t v0 = k0 * a.v_stride[0] + g * a.v_stride[1] + d0;
+    bool leak[J];
     bool any = false;
-    for (int j = 0; j < 4; ++j) {
-        const int d = lane + 32 * j;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
         leak[j] = false;
-        if (d >= hd) continue;
+        if (d0 + 32 * j >= hd) continue;
         for (int64_t i = n; i < hidden_end; ++i) {
-            const float v = load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + d, a.kind);
+            const float v = load_as_f32(a.v, v0 + i * a.v_stride[0] + 32 * j, a.kind);
             leak[j] |= !(fabsf(v) <= 3.4e38f);
         }
         for (int64_t i = max(begin, hidden_end - kKeys); leak[j] && i < n; ++i) {
-            const float v = load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + d, a.kind);
+            const float v = load_as_f32(a.v, v0 + i * a.v_stride[0] + 32 * j, a.kind);
             leak[j] = v == v;
         }
         any |= leak[j];
     }
     if (!__any_sync(0xffffffffu, any)) return;
-    float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < 4; ++j)
-        q[j] = lane + 32 * j < hd ? load_as_f32(a.q, tok * a.q_stride[0] + h * a.q_stride[1] + lane + 32 * j, a.kind) : 0.f;
-    for (int64_t i = begin; i < n; ++i) {
-        float x = 0.f;
-        for (int j = 0; j < 4; ++j)
-            if (lane + 32 * j < hd) x = fmaf(q[j], load_as_f32(a.k, (k0 + i) * a.k_stride[0] + kr + lane + 32 * j, a.kind), x);
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        const float p = exp2_approx(fmaf(x, c, -m));
-        for (int j = 0; j < 4; ++j)
-            if (leak[j]) acc[j] += p * load_as_f32(a.v, (k0 + i) * a.v_stride[0] + vr + lane + 32 * j, a.kind);
+    const int chunk = lane % L * 8;                                      // 8 values of q and of a key
+    const bool live = chunk < hd;
+    const uint16_t* k = reinterpret_cast<const uint16_t*>(a.k) + k0 * a.k_stride[0] + g * a.k_stride[1] + (live ? chunk : 0);
+    const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + tok * a.q_stride[0] + h * a.q_stride[1] + (live ? chunk : 0);
+    const uint4 qw = *reinterpret_cast<const uint4*>(qp);
+    float acc[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[j] = 0.f;
+    for (int64_t base = begin; base < n; base += U * P) {
+        float p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint4 kw = *reinterpret_cast<const uint4*>(k + min(base + u * P + lane / L, n - 1) * a.k_stride[0]);
+            const uint32_t kk[4] = {kw.x, kw.y, kw.z, kw.w}, qq[4] = {qw.x, qw.y, qw.z, qw.w};
+            float x = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x = fmaf(half_at<kHalfType>(qq[e / 2], e & 1), half_at<kHalfType>(kk[e / 2], e & 1), x);
+            p[u] = live ? x : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) p[u] += __shfl_xor_sync(0xffffffffu, p[u], o);
+            p[u] = exp2_approx(fmaf(p[u], c, -m));
+        }
+#pragma unroll
+        for (int l = 0; l < U * P; ++l) {
+            const float w = __shfl_sync(0xffffffffu, p[l / P], l % P * L);
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if (leak[j] && base + l < n)
+                    acc[j] = fmaf(w, load_as_f32(a.v, v0 + (base + l) * a.v_stride[0] + 32 * j, a.kind), acc[j]);
+        }
+        bool open = false;
+#pragma unroll
+        for (int j = 0; j < J; ++j) open |= leak[j] && acc[j] == acc[j];
+        if (!__any_sync(0xffffffffu, open)) break;
     }
-    for (int j = 0; j < 4; ++j)
-        if (leak[j] && part != nullptr)
-            part[lane + 32 * j] = acc[j];
-        else if (leak[j])
-            store_from_f32(a.out, tok * a.out_stride[0] + h * a.out_stride[1] + lane + 32 * j, a.kind, acc[j] * inv);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int d = d0 + 32 * j;
+        if (leak[j] && part != nullptr) part[d] = acc[j];
+        else if (leak[j]) store_from_f32(a.out, tok * a.out_stride[0] + h * a.out_stride[1] + d, a.kind, acc[j] * inv);
+    }
+}
+
+// The rows of the lanes in `again`, one after the other; tok, seen_end, m and inv: of the lane's row, head: of its kv head's.
+template <int HD, bool kHalfType>
+__device__ __noinline__ void repair_rows(const Params& p, Smem<HD>& S, const Work& w, uint32_t again, int head, int tok, int seen_end,
+                                         float m, float inv) {
+    const rvq_prompt_attn_args& a = p.a;
+    const int lane = threadIdx.x & 31, i = threadIdx.x >> 8;             // tile of queries
+    const float c = a.scaling * 1.4426950408889634f;
+    const int begin = w.j0 * kKeys, hidden_end = min(w.lk, (w.j0 + w.n[i]) * kKeys);
+    if (lane == 0) atomicAdd(&S.busy, 1);
+    while (again) {
+        const int l = __ffs(again) - 1;
+        again &= again - 1;
+        __syncwarp();
+        const int64_t row = w.q0 + __shfl_sync(0xffffffffu, tok, l);
+        const int h = w.kv * p.rep + __shfl_sync(0xffffffffu, head, l);
+        repair<HD, kHalfType>(a, row, h, w.k0, begin, __shfl_sync(0xffffffffu, seen_end, l), hidden_end, c,
+                              __shfl_sync(0xffffffffu, m, l), __shfl_sync(0xffffffffu, inv, l),
+                              p.splits == 1 ? nullptr : p.part_o + (((int64_t)w.split * a.tokens + row) * a.n_heads + h) * a.head_dim);
+    }
+    if (lane == 0) atomicSub(&S.busy, 1);
 }
 
 template <int HD, bool kHalfType>
@@ -355,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             mbar_init(smem_addr(&S.work_full[i]), 1);
             mbar_init(smem_addr(&S.work_empty[i]), kSoftmaxWarps + 1);
         }
-        S.dead = 0;
+        S.dead = S.busy = 0;
         for (int i = 0; i < 8; ++i) S.fail[i] = 0;
         mbar_init_fence();
         fence_async_shared();
@@ -565,12 +632,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             if (*(volatile int32_t*)&S.fail[pair_bar - 1]) break;
             const Work& w = S.work[it & 1];
             if (w.live < 0) break;
-            const int64_t q0 = w.q0, k0 = w.k0;
-            const int lq = w.lq, lk = w.lk, tok0 = w.tok0, j0 = w.j0, n = w.n[i], h = w.kv * p.rep + head, split = w.split;
-            const bool live = w.live;
-            const int tok = tok0 + i * T + in;               // in the sequence
-            const bool valid = live && in < T && tok < lq;
-            const int limit = !valid ? 0 : a.causal ? min(lk, max(0, tok + 1 + lk - lq)) : lk;
+            const int n = w.n[i], j0 = w.j0;
+            int limit;                                       // keys that the row sees
+            {
+                const int tok = w.tok0 + i * T + in;         // in the sequence
+                limit = !w.live || in >= T || tok >= w.lq ? 0 : a.causal ? min(w.lk, max(0, tok + 1 + w.lk - w.lq)) : w.lk;
+            }
             float m = -INFINITY, sum = 0.f;                  // m: of the scores times c
             for (int j = 0; j < n; ++j, sp ^= 1) {
                 ok = ok && wait(S, S.s_full[i], sp);
@@ -622,6 +689,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
             if (ok && n > 0) ok = wait(S, S.o_full[i], op);
             op ^= n > 0;
+            // read from shared memory again: kept over the steps, they cost the inner loop registers (16,384 tokens 2,061 -> 2,038 us)
+            const volatile Work& u = S.work[it & 1];
+            const int64_t q0 = u.q0;
+            const int h = u.kv * p.rep + head, split = u.split, lk = u.lk, tok = u.tok0 + i * T + in;
+            const bool valid = u.live && in < T && tok < u.lq;
             tc_fence_after();
             named_sync(pair_bar, 64);                        // the partner has read this half's last maximum
             S.top[i][half][row] = sum;
@@ -684,17 +756,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             // values between this row's last key and the end of its last tile may have leaked in (a row without weights has zeros,
             // one whose sum is infinite or NaN is not finite by itself)
             const int begin = j0 * kKeys, hidden_end = min(lk, (j0 + n) * kKeys), seen_end = min(limit, hidden_end);
-            uint32_t again = __ballot_sync(0xffffffffu, ok && valid && bad && seen_end > begin && seen_end < hidden_end && inv > 0.f);
-            while (again) {
-                const int l = __ffs(again) - 1;
-                again &= again - 1;
-                __syncwarp();
-                const int64_t row = q0 + __shfl_sync(0xffffffffu, tok, l);
-                const int head = __shfl_sync(0xffffffffu, h, l);
-                repair(a, row, head, k0, begin, __shfl_sync(0xffffffffu, seen_end, l), hidden_end, a.scaling < 0.f ? -c : c,
-                       __shfl_sync(0xffffffffu, m, l), __shfl_sync(0xffffffffu, inv, l),
-                       whole ? nullptr : p.part_o + (((int64_t)split * a.tokens + row) * a.n_heads + head) * a.head_dim);
-            }
+            const uint32_t again = __ballot_sync(0xffffffffu, ok && valid && bad && seen_end > begin && seen_end < hidden_end && inv > 0.f);
+            if (again) repair_rows<HD, kHalfType>(p, S, w, again, head, tok, seen_end, m, inv);
             tc_fence_before();                               // O is read: the next unit's products may come
             __syncwarp();
             if (ok && lane == 0) mbar_arrive(smem_addr(&S.work_empty[it & 1]));

@@ -182,6 +182,33 @@ def test_prompt_scores_of_minus_infinity_beside_hidden_values(tokens, prefix, fi
         check(lse[:, first:], wl, ltol)
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,where", [(16384, 16383), (17001, 9000)])
+def test_prompt_hidden_value_far_into_a_long_prompt(n, where, hd, bad, cuda_device):
+    """One value that is not finite, far into a prompt of many units a CTA: the queries before it in its key tile are summed again
+    over all their keys.  The waits of the warps beside that hold on; queries elsewhere keep their bits."""
+    dev = cuda_device
+    g = gen(dev, n + hd)
+    q, k, v = (randn(g, n, h, hd) for h in (8, 2, 2))
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    PromptAttentionOp(q, k, v, clean, scaling=0.1).launch()
+    v[where, 0, 3] = bad
+    v[where, 1] = bad
+    PromptAttentionOp(q, k, v, out, scaling=0.1).launch()
+    assert not take_timeout()
+    first = where - 200                                      # a key tile and a tile of queries before it
+    assert torch.equal(out[:first], clean[:first])
+    want, _, tol, _ = ref.attend(q[first:where], k[:where], v[:where], 0.1, True)
+    check(out[first:where], want, tol)
+    hit = torch.zeros(8, hd, dtype=torch.bool, device=dev)
+    hit[:4, 3] = True
+    hit[4:] = True
+    after = out[where:]
+    assert torch.equal(after[:, ~hit], clean[where:][:, ~hit])
+    assert not bool(torch.isfinite(after[:, hit]).any())
+
+
 def test_prompt_large_and_equal_scores(cuda_device):
     """Scores far from zero (the running maximum moves by hundreds), rising and falling along the keys; all equal."""
     dev = cuda_device

@@ -557,6 +557,59 @@ def test_step_with_norm_and_rotation(hd, tiles, cuda_device):
     assert torch.equal(cache.data, before)
 
 
+@pytest.mark.parametrize("norm,rotate", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tiles", [0, 5])
+def test_step_norm_and_rotation_bit_by_bit(tiles, hd, norm, rotate, cuda_device):
+    """Small whole numbers as projections: their sums of squares are exact in any order, so that norm and rotation have one
+    result, and a call that does them has the bits (outputs, weights, records) of one that is given the normed and rotated q and k.
+    Calls with other norms or positions do not."""
+    from rvq_b200.decoder import rmsnorm, rotate_half
+    dev = cuda_device
+    g = gen(dev, 7 * hd + tiles)
+    B, nh, nkv, max_len = 3, 8, 2, 700
+    data = filled(dev, g, B, nkv, max_len, hd).data
+    rows = torch.tensor([650, 1, 33], dtype=torch.int64, device=dev)
+    pos = torch.tensor([400, 3, 77], dtype=torch.int64, device=dev)
+    qn, kn = (torch.empty(hd, device=dev).uniform_(0.25, 2, generator=g).to(BF) for _ in range(2))
+    ang = torch.randn(500, hd // 2, generator=g, device=dev).repeat(1, 2)
+    cos, sin = ang.cos().to(BF), ang.sin().to(BF)
+    shapes = [(B, h, hd) for h in (nh, nkv, nkv)]
+    if tiles:
+        parts = [torch.randint(-3, 4, (tiles, *s), generator=g, device=dev).float() for s in shapes]
+        whole = [p.sum(0).to(BF) for p in parts]
+    else:
+        whole = parts = [torch.randint(-9, 10, s, generator=g, device=dev).to(BF) for s in shapes]
+
+    def call(q, k, v, q_tiles=1, **kw):
+        cache = Cache4(B, nkv, max_len, hd, data=data.clone())
+        out, w = torch.zeros(B, nh, hd, dtype=BF, device=dev), torch.ones(B, nkv, max_len, device=dev)
+        Cache4AttentionOp(q, k, v, cache, rows, out, n_heads=nh, scaling=hd ** -0.5, weights=w, q_tiles=q_tiles,
+                          kv_tiles=q_tiles, **kw).launch()
+        return out, w, cache.data
+
+    def options(qn=qn, kn=kn, pos=pos):
+        return dict(**(dict(q_norm=qn, k_norm=kn, eps=1e-6) if norm else {}),
+                    **(dict(cos=cos, sin=sin, pos=pos) if rotate else {}))
+
+    turned = lambda x: x * cos[pos][:, None] + rotate_half(x) * sin[pos][:, None] if rotate else x
+    given = lambda x, w: turned(rmsnorm(x, w, 1e-6) if norm else x)
+    want = call(given(whole[0], qn), given(whole[1], kn), whole[2])
+    got = call(*parts, max(tiles, 1), **options())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    # and that says something: every head of the longer sequences has other bits where q's norm, its weights or a position is another
+    # (of two rows one may have all the weight, whatever q is: a score 20 below the other's has 2^-29 of it)
+    other = [] if not norm else [call(*parts, max(tiles, 1), **options(qn=torch.ones_like(qn))),
+                                 call(given(whole[0], torch.ones_like(qn)), given(whole[1], kn), whole[2])]
+    if norm:
+        other.append(call(turned(whole[0] * qn), given(whole[1], kn), whole[2]))
+    if rotate:
+        other.append(call(*parts, max(tiles, 1), **options(pos=pos + 1)))
+    for out, *_ in other:
+        assert bool((out != want[0])[[0, 2]].any(-1).all())
+
+
 # -- eviction ----------------------------------------------------------------------------------------------------------
 def evict_case(dev, rows, nkv, hd, max_len, keep, recent, w, in_place, seed=0):
     g = gen(dev, seed)

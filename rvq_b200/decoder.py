@@ -229,7 +229,10 @@ class Qwen3Decoder:
         self._row = torch.zeros(1, dtype=torch.long, device=dev)              # the int4 cache's row of the step's token
         self._setup_weights()
         self.persist = None
-        self._evict_op = None
+        if kv_budget is not None:
+            from .attention import Cache4EvictOp
+            self._live = torch.zeros(d.n_layers, dtype=torch.long, device=dev)
+            self._evict_op = Cache4EvictOp(self.cache4, self.kv_weights, self._live, keep=kv_budget, recent=kv_recent)
         if native:
             self._build_step_ops()
         if step_impl == "persistent":
@@ -512,11 +515,6 @@ class Qwen3Decoder:
 
     def _evict(self, live: int) -> None:
         """Keep ``kv_budget`` of every layer's ``live`` cache rows (one launch pair for all layers)."""
-        if self._evict_op is None:
-            from .attention import Cache4EvictOp
-            self._live = torch.zeros(self.dims.n_layers, dtype=torch.long, device=self.device)
-            self._evict_op = Cache4EvictOp(self.cache4, self.kv_weights, self._live, keep=self.kv_budget,
-                                           recent=self.kv_recent)
         self._live.fill_(live)
         self._evict_op.launch()
         self._dropped += live - self.kv_budget

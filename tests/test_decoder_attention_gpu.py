@@ -141,6 +141,17 @@ def test_a_full_cache_is_evicted_before_the_slack(cuda_device):
     assert ids.numel() == 100 and dec._dropped > 0
 
 
+def test_evictions_inside_and_outside_of_inference_mode(cuda_device):
+    """The first eviction within a caller's inference mode, a later one without."""
+    art, cfg, prompt = setup(MID, 2, 2048, 13, 34, cuda_device)
+    dec = Qwen3Decoder(cfg, art, cuda_device, mode="dense", max_len=64, causal=True, kv_cache="int4", kv_budget=32, kv_slack=2,
+                       max_positions=256)
+    with torch.inference_mode():
+        ids = dec.generate(prompt, 12)
+    assert dec._dropped > 0
+    assert torch.equal(ids, dec.generate(prompt, 12))
+
+
 def test_refusals(cuda_device):
     art, cfg, prompt = setup(MID, 2, 2048, 13, 60, cuda_device)
     make = lambda **kw: Qwen3Decoder(cfg, art, cuda_device, **kw)

@@ -280,7 +280,7 @@ class PromptAttentionOp(_Op):
         if self._fresh:
             # the workspace is zero-filled in front of its first call, on that call's stream (this one may not be the one the
             # op was built on); a capture only records that, so the first call outside of one does it again
-            with torch.cuda.device(self.device):
+            with torch.cuda.device(self.device), torch.inference_mode():      # it may have been built in that mode
                 self._ws.zero_()
                 self._fresh = torch.cuda.is_current_stream_capturing()
         super().launch()

@@ -826,6 +826,25 @@ def test_prompt_workspace_on_the_stream_of_its_first_launch(cuda_device):
     assert not take_timeout()
 
 
+def test_ops_built_in_inference_mode_run_outside(cuda_device):
+    """And the other way round; 512 units, so that the prompt's workspace holds tickets."""
+    dev = cuda_device
+    g = gen(dev, 47)
+    q, k, v = randn(g, 2048, 8, 64), randn(g, 2048, 8, 64), randn(g, 2048, 8, 64)
+    out, other = torch.empty_like(q), torch.empty_like(q)
+    with torch.inference_mode():
+        op = PromptAttentionOp(q, k, v, out, scaling=0.1)
+    assert op._ws is not None
+    op.launch()
+    op = PromptAttentionOp(q, k, v, other, scaling=0.1)
+    with torch.inference_mode():
+        op.launch()
+    op.launch()
+    assert torch.equal(out, other) and not take_timeout()
+    want, _, tol, _ = ref.attend(q[-200:], k, v, 0.1, True)
+    check(out[-200:], want, tol)
+
+
 def test_two_streams_at_once(cuda_device):
     """The same kinds of op with their own buffers on two streams at the same time."""
     dev = cuda_device

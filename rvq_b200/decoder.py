@@ -115,7 +115,8 @@ class Qwen3Decoder:
     scores and softmax of a step in fp32.  ``kv_budget`` (int4): rows that stay
     in the cache: after every ``kv_slack`` steps whose live rows exceed it, the
     last ``kv_recent`` rows (None: half the budget) and those with the largest
-    attention weight summed over the steps since the prompt are kept, per layer and kv head.
+    attention weight summed over the steps since the prompt are kept, per layer and kv head
+    (equal weights: the first rows; a prompt of ``max_len`` tokens is evicted so, without weights, before the first step).
     Positions then run on past the rows: ``max_positions`` (None: max_len)
     sizes the rotary tables, ``max_len`` the cache."""
 
@@ -218,6 +219,7 @@ class Qwen3Decoder:
             self.k_cache = torch.zeros(d.n_layers, d.n_kv, max_len, d.head_dim, dtype=dt, device=dev)
             self.v_cache = torch.zeros_like(self.k_cache)
         self._dropped = self._since_evict = 0             # rows evicted since the prompt; steps since the last eviction
+        self._rows = 0                                    # cache rows in use
         self.positions = torch.arange(max_len, device=dev)
         self.causal = causal
         self.valid_bias = torch.tensor(0.0 if causal else 1.0, dtype=dt, device=dev)
@@ -518,7 +520,7 @@ class Qwen3Decoder:
         self._live.fill_(live)
         self._evict_op.launch()
         self._dropped += live - self.kv_budget
-        self._since_evict = 0
+        self._rows, self._since_evict = self.kv_budget, 0
 
     def _cb_tiles(self, cid: str) -> torch.Tensor:
         """The codebook handed to rvq_gemv_tiles: fp16 when every value is an
@@ -594,6 +596,7 @@ class Qwen3Decoder:
         if prompt.numel() > self.max_len:
             raise ValueError("prompt longer than the cache")
         self._dropped = self._since_evict = 0
+        self._rows = prompt.numel()
         if self.kv_weights is not None:
             self.kv_weights.zero_()
         with torch.inference_mode():
@@ -626,6 +629,9 @@ class Qwen3Decoder:
         if self.graph is None:
             self.capture()
         row = pos - self._dropped                         # evicted rows moved the later ones down
+        if self.kv_budget is not None and row == self._rows == self.max_len and pos < self.max_positions:
+            self._evict(row)                              # the prompt filled the cache: no step has made room yet
+            row = pos - self._dropped
         if not (0 <= row < self.max_len and pos < self.max_positions):
             raise ValueError("position outside the cache")
         self._tok.copy_(token.view(1))
@@ -633,6 +639,7 @@ class Qwen3Decoder:
         if self.cache4 is not None:
             self._row.fill_(row)
         self.graph.replay()
+        self._rows = row + 1
         if self.kv_budget is not None:
             self._since_evict += 1
             if row + 1 > self.kv_budget and (self._since_evict >= self.kv_slack or row + 1 == self.max_len):

@@ -152,6 +152,48 @@ def test_evictions_inside_and_outside_of_inference_mode(cuda_device):
     assert torch.equal(ids, dec.generate(prompt, 12))
 
 
+class HeldAfterEviction(HeldDecoder):
+    """The same for a cache whose rows were evicted: position ``pos`` is row ``pos - dropped``, its key rotated at ``pos``."""
+
+    def _attention(self, l, q, k, v, pos):
+        if pos is None:
+            return super()._attention(l, q, k, v, pos)
+        d, L = self.dims, self.layers[l]
+        q = rmsnorm(q.view(1, d.n_heads, d.head_dim), L["self_attn.q_norm.weight"], d.eps)
+        q = q * self.cos[pos][:, None] + rotate_half(q) * self.sin[pos][:, None]
+        n = int(pos) + 1 - self.dropped
+        keys, vals = (ref.values(*part).transpose(0, 1) for part in ref.unpack(self.source.data[l, :, :n], d.head_dim))
+        return ref.attend(q, keys, vals, self.scaling, False)[0].to(q.dtype).reshape(1, d.n_heads * d.head_dim)
+
+
+def test_a_prompt_that_fills_the_cache(cuda_device):
+    """A prompt of max_len tokens with a budget: evicted before the first step, without weights: the first rows and the recent
+    ones stay.  The step's logits are those over the kept rows (tolerance: test_int4_cache_logits, 2 layers)."""
+    art, cfg, prompt = setup(MID, 2, 2048, 17, 64, cuda_device)
+    kw = dict(mode="dense", max_len=64, causal=True, kv_cache="int4", kv_budget=32, kv_recent=10, max_positions=256)
+    dec = Qwen3Decoder(cfg, art, cuda_device, **kw)
+    want = HeldAfterEviction(cfg, art, cuda_device, mode="dense", max_len=256, causal=True, step_impl="torch")
+    want.source, want.dropped = dec.cache4, 32
+    dec.capture()
+    dec.prefill(prompt)
+    data = dec.cache4.data.clone()
+    with pytest.raises(ValueError):
+        dec.step(prompt[:1], 256)
+    assert dec._dropped == 0 and torch.equal(dec.cache4.data, data)
+    with torch.inference_mode():
+        for i in range(3):
+            got = dec.step(prompt[i:i + 1], 64 + i).clone()
+            assert rel(got, want._forward(prompt[i:i + 1], torch.tensor([64 + i], device=cuda_device))) < 2e-2, i
+    assert dec._dropped == 32
+    assert torch.equal(dec.cache4.data[:, :, :32], data[:, :, list(range(22)) + list(range(54, 64))])
+    ids = dec.generate(prompt, 100)
+    assert ids.numel() == 100 and torch.equal(ids, dec.generate(prompt, 100))
+    full = Qwen3Decoder(cfg, art, cuda_device, **{**kw, "max_positions": None})
+    full.prefill(prompt)
+    with pytest.raises(ValueError):                         # no position is left
+        full.step(prompt[:1], 64)
+
+
 def test_refusals(cuda_device):
     art, cfg, prompt = setup(MID, 2, 2048, 13, 60, cuda_device)
     make = lambda **kw: Qwen3Decoder(cfg, art, cuda_device, **kw)

@@ -218,7 +218,7 @@ class Qwen3Decoder:
         else:
             self.k_cache = torch.zeros(d.n_layers, d.n_kv, max_len, d.head_dim, dtype=dt, device=dev)
             self.v_cache = torch.zeros_like(self.k_cache)
-        self._dropped = self._since_evict = 0             # rows evicted since the prompt; steps since the last eviction
+        self._dropped = self._since_evict = 0             # rows evicted since the prompt; steps over the budget since the last time
         self._rows = 0                                    # cache rows in use
         self.positions = torch.arange(max_len, device=dev)
         self.causal = causal
@@ -641,9 +641,10 @@ class Qwen3Decoder:
         self.graph.replay()
         self._rows = row + 1
         if self.kv_budget is not None:
-            self._since_evict += 1
-            if row + 1 > self.kv_budget and (self._since_evict >= self.kv_slack or row + 1 == self.max_len):
-                self._evict(row + 1)
+            if row + 1 > self.kv_budget:
+                self._since_evict += 1
+                if self._since_evict >= self.kv_slack or row + 1 == self.max_len:
+                    self._evict(row + 1)
         return self._logits
 
     def check_waits(self) -> None:

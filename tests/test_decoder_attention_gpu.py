@@ -141,6 +141,17 @@ def test_a_full_cache_is_evicted_before_the_slack(cuda_device):
     assert ids.numel() == 100 and dec._dropped > 0
 
 
+def test_steps_below_the_budget_are_no_slack(cuda_device):
+    """A text that passes the budget on its way: the first eviction is due kv_slack steps after that, as every later one."""
+    art, cfg, prompt = setup(MID, 2, 2048, 19, 30, cuda_device)
+    dec = Qwen3Decoder(cfg, art, cuda_device, mode="dense", max_len=64, causal=True, kv_cache="int4", kv_budget=40, kv_slack=8,
+                       max_positions=256)
+    seen, plain = [], dec._evict
+    dec._evict = lambda live: (seen.append(live), plain(live))
+    dec.generate(prompt, 60)
+    assert seen == [48] * ((30 + 59 - 40) // 8)
+
+
 def test_evictions_inside_and_outside_of_inference_mode(cuda_device):
     """The first eviction within a caller's inference mode, a later one without."""
     art, cfg, prompt = setup(MID, 2, 2048, 13, 34, cuda_device)

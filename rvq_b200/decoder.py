@@ -219,7 +219,7 @@ class Qwen3Decoder:
             self.k_cache = torch.zeros(d.n_layers, d.n_kv, max_len, d.head_dim, dtype=dt, device=dev)
             self.v_cache = torch.zeros_like(self.k_cache)
         self._dropped = self._since_evict = 0             # rows evicted since the prompt; steps over the budget since the last time
-        self._rows = 0                                    # cache rows in use
+        self._rows = self._fixed = 0                      # cache rows in use; of them, those that eviction picked by weight
         self.positions = torch.arange(max_len, device=dev)
         self.causal = causal
         self.valid_bias = torch.tensor(0.0 if causal else 1.0, dtype=dt, device=dev)
@@ -520,7 +520,7 @@ class Qwen3Decoder:
         self._live.fill_(live)
         self._evict_op.launch()
         self._dropped += live - self.kv_budget
-        self._rows, self._since_evict = self.kv_budget, 0
+        self._rows, self._fixed, self._since_evict = self.kv_budget, self.kv_budget - self.kv_recent, 0
 
     def _cb_tiles(self, cid: str) -> torch.Tensor:
         """The codebook handed to rvq_gemv_tiles: fp16 when every value is an
@@ -596,7 +596,7 @@ class Qwen3Decoder:
         if prompt.numel() > self.max_len:
             raise ValueError("prompt longer than the cache")
         self._dropped = self._since_evict = 0
-        self._rows = prompt.numel()
+        self._rows, self._fixed = prompt.numel(), 0
         if self.kv_weights is not None:
             self.kv_weights.zero_()
         with torch.inference_mode():
@@ -625,7 +625,8 @@ class Qwen3Decoder:
         return self
 
     def step(self, token: torch.Tensor, pos: int) -> torch.Tensor:
-        """One decode step by graph replay; ``token`` a device tensor of one id."""
+        """One decode step by graph replay; ``token`` a device tensor of one id.  ``pos`` may go back to an earlier position, whose
+        token and later ones it replaces; after an eviction back to the last ``kv_recent`` ones before that at most."""
         if self.graph is None:
             self.capture()
         row = pos - self._dropped                         # evicted rows moved the later ones down
@@ -634,6 +635,8 @@ class Qwen3Decoder:
             row = pos - self._dropped
         if not (0 <= row < self.max_len and pos < self.max_positions):
             raise ValueError("position outside the cache")
+        if row < self._fixed:                             # the rows there are no longer those of the positions before pos
+            raise ValueError("position before the last kv_recent ones of the last eviction")
         self._tok.copy_(token.view(1))
         self._pos.fill_(pos)
         if self.cache4 is not None:

@@ -152,6 +152,28 @@ def test_steps_below_the_budget_are_no_slack(cuda_device):
     assert seen == [48] * ((30 + 59 - 40) // 8)
 
 
+def test_going_back_after_an_eviction(cuda_device):
+    """A step may be taken again at one of the recent positions, with the same logits; at earlier ones, whose rows are not there any
+    more, it is refused and changes nothing."""
+    art, cfg, prompt = setup(MID, 2, 2048, 23, 60, cuda_device)
+    dec = Qwen3Decoder(cfg, art, cuda_device, mode="dense", max_len=96, causal=True, kv_cache="int4", kv_budget=40, kv_recent=10,
+                       kv_slack=4, max_positions=256)
+    dec.prefill(prompt)
+    for i in range(4):
+        dec.step(prompt[i:i + 1], 60 + i)
+    assert dec._dropped == 24                               # rows 30 to 39 are positions 54 to 63
+    data, weights = dec.cache4.data.clone(), dec.kv_weights.clone()
+    for pos in (53, 30, 24):
+        with pytest.raises(ValueError):
+            dec.step(prompt[:1], pos)
+    assert torch.equal(dec.cache4.data, data) and torch.equal(dec.kv_weights, weights)
+    first = dec.step(prompt[9:10], 54).clone()
+    after = dec.step(prompt[10:11], 55).clone()
+    assert torch.equal(dec.step(prompt[9:10], 54), first) and torch.equal(dec.step(prompt[10:11], 55), after)
+    dec.prefill(prompt)
+    dec.step(prompt[:1], 10)                                # without an eviction any position will do
+
+
 def test_evictions_inside_and_outside_of_inference_mode(cuda_device):
     """The first eviction within a caller's inference mode, a later one without."""
     art, cfg, prompt = setup(MID, 2, 2048, 13, 34, cuda_device)

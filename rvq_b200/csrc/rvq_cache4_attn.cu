@@ -672,7 +672,7 @@ int check(const rvq_cache4_attn_args* a) {
     if (c.head_dim != 64 && c.head_dim != 128) return RVQ_ERR_UNSUPPORTED;
     if (a->n_heads < c.n_kv || a->n_heads % c.n_kv) return RVQ_ERR_INVALID;
     if (a->n_heads / c.n_kv > kMaxRep) return RVQ_ERR_UNSUPPORTED;
-    if (a->rows == nullptr || a->out == nullptr || ((uintptr_t)a->out & 15)) return RVQ_ERR_INVALID;
+    if (a->rows == nullptr || a->out == nullptr) return RVQ_ERR_INVALID;
     if (!vec_fits(a->q, (int64_t)c.n_seq * a->n_heads * c.head_dim)) return RVQ_ERR_INVALID;
     if ((a->k.ptr == nullptr) != (a->v.ptr == nullptr)) return RVQ_ERR_INVALID;
     if (a->k.ptr != nullptr) {

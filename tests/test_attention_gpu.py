@@ -505,6 +505,32 @@ def test_step_offsets_beyond_32_bits(cuda_device):
     assert bool((w[:2] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("max_len", [50, 4000])
+def test_step_operands_anywhere(max_len, dtype, cuda_device):
+    """q, k, v and out at addresses of single elements: the same bits, and nothing beside out is written."""
+    dev = cuda_device
+    g = gen(dev, max_len)
+    B, nh, nkv, hd = 2, 6, 2, 64
+    data = filled(dev, g, B, nkv, max_len, hd).data
+    rows = torch.tensor([max_len - 1, 17], dtype=torch.int64, device=dev)
+    whole = [randn(g, B, h, hd, dtype=dtype) for h in (nh, nkv, nkv)]
+    want = torch.zeros(B, nh, hd, dtype=dtype, device=dev)
+    Cache4AttentionOp(*whole, Cache4(B, nkv, max_len, hd, data=data.clone()), rows, want, scaling=0.1).launch()
+
+    def shifted(x, by):
+        room = torch.full((x.numel() + 16,), 7.0, dtype=dtype, device=dev)
+        room[by:by + x.numel()] = x.flatten()
+        return room, room[by:by + x.numel()].view(x.shape)
+
+    for by in (1, 3, 8):
+        room, out = shifted(torch.zeros_like(want), by)
+        Cache4AttentionOp(*(shifted(x, by)[1] for x in whole), Cache4(B, nkv, max_len, hd, data=data.clone()), rows, out,
+                          scaling=0.1).launch()
+        assert torch.equal(out, want)
+        assert bool((room[:by] == 7).all()) and bool((room[by + out.numel():] == 7).all())
+
+
 def rotated(x, w, eps, cos, sin):
     """Per-head RMSNorm and rotary embedding with the roundings of rvq_b200.decoder."""
     from rvq_b200.decoder import rmsnorm, rotate_half

@@ -175,10 +175,30 @@ def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
     return all(abs(off + i * s0 + j * s1) >= a.shape[2] for i in near(off, s0, d0) for j in near(off + i * s0, s1, d1))
 
 
+def _in_gaps(view: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether the contiguous tensor ``t`` lies in the gaps of a [tokens, heads, head_dim] view."""
+    if view.dim() != 3 or not t.is_contiguous():
+        return False
+    size = view.element_size()
+    lo, hi = t.data_ptr() - view.data_ptr(), t.data_ptr() - view.data_ptr() + t.numel() * t.element_size()
+    (s0, n0), (s1, n1) = sorted(((view.stride(d) * size, view.shape[d]) for d in (0, 1)), reverse=True)
+    # for every place along the shorter stride: the last row that starts before t's end ends before t starts
+    return all(j * s1 + min(n0 - 1, (hi - 1 - j * s1) // max(s0, 1)) * s0 + view.shape[2] * size <= lo
+               for j in range(n1) if j * s1 < hi)
+
+
 def _apart(a: torch.Tensor, b: torch.Tensor, what: str) -> None:
     (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a0 < b1 and b0 < a1 and not _interleaved(a, b):
+    if a0 < b1 and b0 < a1 and not (_interleaved(a, b) or _in_gaps(a, b) or _in_gaps(b, a)):
         raise ValueError(f"{what} must not overlap")
+
+
+def _all_apart(written, read=()) -> None:
+    """Refuses written (tensor, name) pairs that share memory with one another or with a read one; None: not there."""
+    written, read = ([(t, n) for t, n in pairs if t is not None] for pairs in (written, read))
+    for i, (a, an) in enumerate(written):
+        for b, bn in written[i + 1:] + read:
+            _apart(a, b, f"{an} and {bn}")
 
 
 class _Op:
@@ -263,11 +283,7 @@ class PromptAttentionOp(_Op):
                 _ints(cu_k, n_seq + 1, torch.int32, "cu_k")
         if lse is not None:
             _plain(lse, (nh, tokens), torch.float32, "lse")
-            _apart(lse, out, "lse and out")
-        for t, name in ((q, "q"), (k, "k"), (v, "v")):
-            _apart(t, out, f"{name} and out")
-            if lse is not None:
-                _apart(t, lse, f"{name} and lse")
+        _all_apart([(out, "out"), (lse, "lse")], [(q, "q"), (k, "k"), (v, "v"), (cu_q, "cu_q"), (cu_k, "cu_k")])
         self._on(q, k, v, out, cu_q, cu_k, lse)
         self.args = RvqPromptAttnArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cu_q), _ptr(cu_k), tokens,
                                       keys, _strides(q), _strides(k), _strides(v), _strides(out), n_seq, nh, nkv, hd,
@@ -327,12 +343,13 @@ class _Cache4RowsOp(_Op):
             _ints(cu, cache.n_seq + 1, torch.int32, "cu")
         if start is not None:
             _ints(start, cache.n_seq, torch.int64, "start")
-        _apart(k, cache.data, "k and the cache")
-        _apart(v, cache.data, "v and the cache")
+        rows, store, at = [(k, "k"), (v, "v")], [(cache.data, "the cache")], [(cu, "cu"), (start, "start")]
         if self.name == "rvq_cache4_read":
-            _apart(k, v, "k and v")
+            _all_apart(rows, store + at)
             _distinct(k, "k")
             _distinct(v, "v")
+        else:
+            _all_apart(store, rows + at)
         self._on(k, v, cache.data, cu, start)
         self.args = RvqCache4RowsArgs(cache.struct(), _ptr(k), _ptr(v), _ptr(cu), _ptr(start), k.shape[0], _strides(k),
                                       _strides(v), _native.kind_of(k), 0)
@@ -421,10 +438,9 @@ class Cache4AttentionOp(_Op):
             raise ValueError("out must be contiguous, with q's elements and type (bf16 for partials)")
         if weights is not None:
             _plain(weights, (n, nkv, cache.max_len), torch.float32, "weights")
-        written = [(out, "out"), (cache.data, "the cache")] + ([(weights, "weights")] if weights is not None else [])
-        for i, (a, an) in enumerate(written):
-            for b, bn in written[i + 1:] + [(t, tn) for t, tn in ((q, "q"), (k, "k"), (v, "v")) if t is not None]:
-                _apart(a, b, f"{an} and {bn}")
+        _all_apart([(out, "out"), (cache.data, "the cache"), (weights, "weights")],
+                   [(q, "q"), (k, "k"), (v, "v"), (rows, "rows"), (q_norm, "q_norm"), (k_norm, "k_norm"), (cos, "cos"), (sin, "sin"),
+                    (pos, "pos")])
         self._on(q, k, v, cache.data, rows, out, weights, q_norm, k_norm, cos, sin, pos)
         self.args = RvqCache4AttnArgs(qv, kv_, vv, _ptr(q_norm), _ptr(k_norm), _ptr(cos), _ptr(sin), _ptr(pos),
                                       cache.struct(), _ptr(rows), _ptr(out), _ptr(weights), n_heads, table, float(eps),
@@ -450,19 +466,19 @@ class Cache4EvictOp(_Op):
         _ints(rows, n, torch.int64, "rows")
         if (out is None) != (out_weights is None):
             raise ValueError("out and out_weights are given together")
-        if out is None:
+        apart = out is not None
+        if not apart:
             out, out_weights = cache, weights
         else:
             if (out.n_seq, out.n_kv, out.head_dim) != (n, nkv, cache.head_dim) or out.max_len < keep:
                 raise ValueError("out must hold keep rows of the same sequences and heads")
             _plain(out_weights, (n, nkv, out.max_len), torch.float32, "out_weights")
-            _apart(out.data, cache.data, "out and the cache")
-            _apart(out_weights, weights, "out_weights and weights")
         if kept is not None:
             _plain(kept, (n, nkv, keep), torch.int32, "kept")
         if new_rows is not None:
             _ints(new_rows, n, torch.int64, "new_rows")
-            _apart(new_rows, rows, "new_rows and rows")
+        _all_apart([(out.data, "out"), (out_weights, "out_weights"), (kept, "kept"), (new_rows, "new_rows")],
+                   [(rows, "rows")] + ([(cache.data, "the cache"), (weights, "weights")] if apart else []))
         self._on(cache.data, weights, rows, out.data, out_weights, kept, new_rows)
         self.kept = torch.empty(n, nkv, keep, dtype=torch.int32, device=self.device) if kept is None else kept
         self.args = RvqCache4EvictArgs(cache.struct(), out.struct(), _ptr(weights), _ptr(out_weights), _ptr(rows),

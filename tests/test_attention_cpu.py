@@ -125,6 +125,65 @@ def test_interleaved_views():
     assert said[0] > 300                                                        # it does find views that are apart
 
 
+def test_tensors_in_the_gaps_of_views():
+    """Against the bytes themselves, over many pairs."""
+    buf = torch.zeros(8192, dtype=torch.uint8)
+    g = torch.Generator().manual_seed(2)
+    r = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))
+    said = [0, 0]
+    for _ in range(3000):
+        n0, n1, hd = r(1, 5), r(1, 5), 8
+        s1 = 8 * r(1, 5)
+        s0 = s1 * n1 + 8 * r(0, 4)
+        n, st = ((n0, n1), (s0, s1)) if r(0, 1) else ((n1, n0), (s1, s0))
+        view = torch.as_strided(buf.view(BF), (*n, hd), (*st, 1), 8 * r(0, 30))
+        t = buf.view(torch.int32)[r(0, 500):][:r(1, 12)]
+        bytes_of = lambda x: {x.storage_offset() * x.element_size() + b
+                              for i in torch.cartesian_prod(*(torch.arange(m) for m in x.shape)).view(-1, x.dim())
+                              for b in range(int((i * torch.tensor(x.stride())).sum()) * x.element_size(),
+                                             int((i * torch.tensor(x.stride())).sum()) * x.element_size() + x.element_size())}
+        if said[0] + said[1] >= 600:
+            break
+        (a0, a1), (b0, b1) = attention._span(view), attention._span(t)
+        if a0 >= b1 or b0 >= a1:
+            continue
+        share = bool(bytes_of(view) & bytes_of(t))
+        assert attention._in_gaps(view, t) is not share
+        said[share] += 1
+    assert min(said) > 30
+
+
+def test_refuses_to_write_over_other_operands():
+    """One buffer for what is written and anything else of the call, of every operator."""
+    words = z(4096, dtype=torch.float32)
+    as_int = lambda n: words.view(torch.int32)[:n]
+    as_long = lambda n: words.view(torch.int64)[:n]
+    over = lambda *shape: words.view(BF)[:int(torch.tensor(shape).prod())].view(shape)
+    data = words.view(torch.uint8)[:2 * 2 * 8 * 80].view(2, 2, 8, 80)
+    stored = Cache4(2, 2, 8, 64, data=data)
+    w = words[:32].view(2, 2, 8)
+    two = dict(cu=ints(0, 3, 6, dtype=torch.int32))
+    for make in (lambda: prompt(out=over(6, 4, 64), cu_q=as_int(3)),
+                 lambda: prompt(lse=words[:24].view(4, 6), cu_q=ints(0, 3, 6, dtype=torch.int32), cu_k=as_int(3)),
+                 lambda: Cache4WriteOp(stored, z(6, 2, 64), z(6, 2, 64), cu=as_int(3)),
+                 lambda: Cache4WriteOp(stored, z(6, 2, 64), z(6, 2, 64), start=as_long(2), **two),
+                 lambda: Cache4ReadOp(cache(), over(6, 2, 64), z(6, 2, 64), cu=as_int(3)),
+                 lambda: Cache4ReadOp(cache(), z(6, 2, 64), over(6, 2, 64), start=as_long(2), **two),
+                 lambda: step(out=over(2, 4, 64), rows=as_long(2)),
+                 lambda: step(c=stored, rows=as_long(2)),
+                 lambda: step(weights=w, q_norm=over(64), k_norm=z(64)),
+                 lambda: step(out=over(2, 4, 64), cos=z(9, 64), sin=z(9, 64), pos=as_long(2)),
+                 lambda: step(out=over(2, 4, 64), cos=over(9, 64), sin=z(9, 64), pos=ints(0, 0)),
+                 lambda: evict(w=w, kept=as_int(16).view(2, 2, 4)),
+                 lambda: evict(c=stored, kept=as_int(16).view(2, 2, 4)),
+                 lambda: evict(rows=as_long(2), kept=as_int(16).view(2, 2, 4)),
+                 lambda: evict(kept=as_int(16).view(2, 2, 4), new_rows=as_long(2)),
+                 lambda: evict(out=cache(max_len=4), out_weights=words[:16].view(2, 2, 4), kept=as_int(16).view(2, 2, 4)),
+                 lambda: evict(w=w, new_rows=as_long(2))):
+        with pytest.raises(ValueError, match="overlap"):
+            make()
+
+
 def cache(n_seq=2, n_kv=2, max_len=8, hd=64):
     return Cache4(n_seq, n_kv, max_len, hd)
 

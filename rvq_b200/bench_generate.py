@@ -1,6 +1,7 @@
 """End-to-end batch-1 generation benchmark: random-init 36-layer Qwen3 model.
 
     python -m rvq_b200.bench_generate [--layers 36] [--prompt 128] [--new 128]
+        [--prompt-attention fused] [--kv-cache int4] [--causal]
 
 Model: the 2560 / 9728 / 32q / 8kv / head-128 block x 36 layers, vocab
 151936, tied bf16 embeddings, RMSNorm, RoPE theta 1e6; every projection RVQ
@@ -77,14 +78,16 @@ def margin(logits):
 
 
 def run(layers=36, prompt_len=128, new=128, vocab=151936, reps=3,
-        modes=("dense", "slot", "fused", "fused_exact", "fused_persistent"), reference=True, device="cuda:0", hbm_gbs=None):
+        modes=("dense", "slot", "fused", "fused_exact", "fused_persistent"), reference=True, device="cuda:0", hbm_gbs=None,
+        **decoder):
     """TTFT, ms/token and greedy ids per weight mode, then the same prompt
     through the drop-in engine (``_layerwise_logits`` over HF decoder layers
     on slot weights, bit-identical to the oracle engine that is pinned to the
     reference engine's own output): per mode, whether the ids are identical,
     and if not the first divergence and the engine's top-1/top-2 margin there.
     ``hbm_gbs``: HBM peak for each mode's roofline fraction (weight bytes per
-    token / ms per token)."""
+    token / ms per token).  ``decoder``: further options of ``Qwen3Decoder``
+    (prompt_attention, kv_cache, causal)."""
     device = torch.device(device)
     torch.cuda.set_device(device)
     shape = synthetic.BlockShape()
@@ -107,7 +110,7 @@ def run(layers=36, prompt_len=128, new=128, vocab=151936, reps=3,
         # "fused_persistent": fused weights, the whole step as one cooperative launch
         wmode, impl = ("fused", "persistent") if mode == "fused_persistent" else (mode, "native")
         dec = Qwen3Decoder(cfg, art, device, mode=wmode, max_len=prompt_len + new + 8, artifact_is_shard=True,
-                           step_impl=impl)
+                           step_impl=impl, **decoder)
         res, ids[mode] = time_mode(dec, prompt, new, reps)
         dec.check_waits()
         if mode in bytes_tok:
@@ -153,9 +156,12 @@ def main(argv=None):
     ap.add_argument("--vocab", type=int, default=151936)
     ap.add_argument("--modes", default="dense,slot,fused,fused_exact,fused_persistent")
     ap.add_argument("--no-reference", action="store_true")
+    ap.add_argument("--prompt-attention", default="engine", choices=("engine", "fused"))
+    ap.add_argument("--kv-cache", default="bf16", choices=("bf16", "int4"))
+    ap.add_argument("--causal", action="store_true")
     a = ap.parse_args(argv)
-    print(json.dumps(run(a.layers, a.prompt, a.new, a.vocab, modes=tuple(a.modes.split(",")),
-                         reference=not a.no_reference)))
+    print(json.dumps(run(a.layers, a.prompt, a.new, a.vocab, modes=tuple(a.modes.split(",")), reference=not a.no_reference,
+                         prompt_attention=a.prompt_attention, kv_cache=a.kv_cache, causal=a.causal)))
 
 
 if __name__ == "__main__":

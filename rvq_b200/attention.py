@@ -146,10 +146,10 @@ def _plain(t: torch.Tensor, shape, dtype: torch.dtype, name: str) -> torch.Tenso
 
 def _span(t: torch.Tensor):
     """First byte and the one behind the last of a tensor's elements."""
-    if t.numel() == 0:
-        return t.data_ptr(), t.data_ptr()
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    n, first = t.numel(), t.data_ptr()
+    if n and not t.is_contiguous():
+        n = 1 + sum((m - 1) * s for m, s in zip(t.shape, t.stride()))
+    return first, first + n * t.element_size()
 
 
 def _distinct(t: torch.Tensor, name: str) -> None:
@@ -187,18 +187,13 @@ def _in_gaps(view: torch.Tensor, t: torch.Tensor) -> bool:
                for j in range(n1) if j * s1 < hi)
 
 
-def _apart(a: torch.Tensor, b: torch.Tensor, what: str) -> None:
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a0 < b1 and b0 < a1 and not (_interleaved(a, b) or _in_gaps(a, b) or _in_gaps(b, a)):
-        raise ValueError(f"{what} must not overlap")
-
-
 def _all_apart(written, read=()) -> None:
     """Refuses written (tensor, name) pairs that share memory with one another or with a read one; None: not there."""
-    written, read = ([(t, n) for t, n in pairs if t is not None] for pairs in (written, read))
-    for i, (a, an) in enumerate(written):
-        for b, bn in written[i + 1:] + read:
-            _apart(a, b, f"{an} and {bn}")
+    written, read = ([(*_span(t), t, n) for t, n in pairs if t is not None] for pairs in (written, read))
+    for i, (a0, a1, a, an) in enumerate(written):
+        for b0, b1, b, bn in written[i + 1:] + read:
+            if a0 < b1 and b0 < a1 and not (_interleaved(a, b) or _in_gaps(a, b) or _in_gaps(b, a)):
+                raise ValueError(f"{an} and {bn} must not overlap")
 
 
 class _Op:

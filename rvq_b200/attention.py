@@ -7,7 +7,9 @@ As in ``rvq_b200.step``, each ``*Op`` resolves its pointers once and
 so launches can be captured in a CUDA graph.  The tensors an op was built
 from must outlive it and keep their storage; an op with a workspace of its own
 (``PromptAttentionOp``, ``Cache4AttentionOp``) runs one launch at
-a time and outlives its launches.
+a time and outlives its launches and graphs, or, launched on the stream it was
+built on, may be dropped with the work still queued there (what the stream
+allocates later comes after it).
 """
 
 from __future__ import annotations
@@ -243,6 +245,7 @@ class PromptAttentionOp(_Op):
     packed as the queries); without them all tokens and all keys are one sequence.  ``causal``: the last query of a
     sequence sees all its keys, each one before it one key less (with more keys than queries the first keys are
     a past that every query sees).  ``lse``: fp32 [n_heads, tokens], gets log(sum(exp(scores))).
+    Scores, softmax statistics and sums are fp32; the probabilities are rounded to q's type for the product with v.
     A query that sees no key gets zeros (lse -inf); rows outside every sequence are left as they were."""
 
     def __init__(self, q, k, v, out, *, scaling: float, causal: bool = True, cu_q: Optional[torch.Tensor] = None,
@@ -391,7 +394,8 @@ class Cache4AttentionOp(_Op):
     ``q_norm`` / ``k_norm`` (bf16 [head_dim]) and ``cos`` / ``sin`` (bf16 [positions, head_dim]) with ``pos`` (int64
     [n_seq]): per-head RMSNorm and rotary embedding of q and k first, as ``AttentionOp`` does them.
     ``weights``: fp32 [n_seq, n_kv, max_len], gets the softmax weight of every attended row, summed over the query
-    heads of its kv head, added (the new row's: set)."""
+    heads of its kv head, added (the new row's: set).
+    Scores, softmax statistics and sums are fp32; a weight times a record's step keeps 16 bits for the product with the codes."""
 
     def __init__(self, q, k, v, cache: Cache4, rows: torch.Tensor, out: torch.Tensor, *, scaling: float,
                  n_heads: Optional[int] = None, weights: Optional[torch.Tensor] = None, q_norm=None, k_norm=None,

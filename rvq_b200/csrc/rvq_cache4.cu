@@ -68,8 +68,9 @@ __device__ __forceinline__ uint8_t* record_of(const rvq_cache4_rows_args& a, int
 // HD / 4 adjacent threads per token of the block's kv head: half of them K, half V; four adjacent ones hold a group, 8
 // values (one 16-byte load or store) each, which are one code word.  A block's tokens are neighbouring records, so code
 // words and parameters fill whole sectors.  (Two or four tokens a thread: 4,096 tokens as fast, 700 at half the speed.)  Bound by
-// instructions, in write the codes' arithmetic: 4,096 tokens of 8 heads of 128 written in 10.1 us (2.2 TB/s moved), read in
-// 7.4 us (3.0 TB/s); 9 sequences of up to 700 tokens, 2 heads of 64: 3.5 and 2.6 us, a launch.
+// the issue of instructions (write: issue 87 %, ALU pipe 60 %, DRAM 32 %; read: 78, 54 and 38 %): 8 heads of 128, 65,536 tokens
+// written in 125 us (2.8 TB/s moved) and read in 92 us (3.8 TB/s), 1.9 and 1.4 us for every further 1,000 tokens; 4,096 tokens, in L2, 8.9
+// and 6.4 us; 9 sequences of up to 700 tokens, 2 heads of 64: 3.5 and 2.6 us, a launch.
 
 template <int HD, bool kWrite, int kKind>
 __global__ void __launch_bounds__(kRowsThreads) cache4_rows_kernel(rvq_cache4_rows_args a) {

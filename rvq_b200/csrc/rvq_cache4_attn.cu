@@ -27,11 +27,12 @@ using sm100::smem_addr;
 // partial results are joined in fixed order, warp by warp in the CTA and range
 // by range in a second launch, so results do not depend on scheduling.
 //
-// Bound by the issue of integer instructions (masks, shifts, conversions: of about
-// 540 instructions a tile 250 on the ALU pipe, 55 % of its peak, issue 60 %), not by
-// HBM: 64 sequences of 4,096 rows, 64/8 heads of 128, 113 us, 2.96 TB/s of records
-// (45 % of measured copy bandwidth).  One sequence of 40,000 rows with weights:
-// 27 us; of 300 rows: 7.5 us, a chain of latencies (row count, copies, three tiles,
+// No unit is full: of about 540 instructions a tile 250 are masks, shifts and conversions on
+// the ALU pipe (55 % of its peak), issue 60 %, tensor pipe 25 %; a warp that could go on waits for its turn
+// (1.3 clocks an instruction), the ALU (1.1) and results (0.9 fixed, 0.5 loads).  HBM is far away: 64 sequences of
+// 4,096 rows, 64/8 heads of 128, 113 us, 2.96 TB/s of records (45 % of measured copy
+// bandwidth).  One sequence of 40,000 rows with weights:
+// 27.6 us; of 300 rows: 7.5 us, a chain of latencies (row count, copies, three tiles,
 // the join of the warps).  Measured against this form: clusters of CTAs joining over
 // distributed shared memory left SMs idle (40,000 rows: 54 us); bulk copies with
 // mbarriers cost more instructions than cp.async (64 x 4,096: 154 against 134 us);
@@ -692,7 +693,10 @@ int check(const rvq_cache4_attn_args* a) {
 // of 4,096 rows: 45 us whole, 40 us halved; of mixed lengths 38 and 26), but none shorter than a tile for every warp of a
 // full cache.  Above that a range is a whole sequence: halves cost 64 x 8 heads of 4,096 rows 113 -> 120 us.
 // A short cache is one range, which needs no second launch: 8 heads, 300 rows 9.1 -> 7.5 us, 600 rows 9.7 -> 9.5, 750 rows
-// 9.3 -> 10.4; with weights 300 rows 9.5 -> 9.0, 500 rows 10.1 -> 10.9.
+// 9.3 -> 10.4; with weights 300 rows 9.5 -> 9.0, 500 rows 10.1 -> 10.9.  The limits go by one sequence.  Many have more to lose by a
+// second launch, and at the limits' far side one range would still pay: 8 sequences x 8 heads of 512 rows 12.3 -> 9.9 us, but of 768
+// rows (two launches) 13.0 against 11.6 in one; 32 sequences of 1,024 rows 29.7 against 20.0.  The rule goes by the cache's length, as
+// the host does not know the rows: 300 rows in a cache of 8,192 take 13.4 us.
 int plan(const rvq_cache4_attn_args& a, int* splits) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);

@@ -44,10 +44,12 @@ __device__ int g_attention_timeout;          // sticky: a bounded wait gave up
 //
 // Bound by the chain S -> softmax -> P -> PV -> S of a tile: of 3,570 clocks a step of
 // both tiles the tensor cores work 2,048 (timestamps of one CTA: softmax 1,880, of
-// which the exponentials 1,300; PV and S 1,030; waits 300).  8,192 tokens, 32/8 heads
-// of 128: causal 463 us, 1,187 TFLOP/s (71 % of the measured matrix peak, 85 % of the
-// sustained one), not causal 877 us, 1,254.  Tried: a thread a row with its 128 columns
-// (1,094 not causal, before the MMA warp became one thread); a quarter or half of the
+// which the exponentials 1,300; PV and S 1,030; waits 300); no unit is full (4,096 tokens:
+// tensor pipe 52 %, exponentials 52 %, issue 42 %).  8,192 tokens, 32/8 heads of 128,
+// short runs: causal 462 us, 1,190 TFLOP/s (71 % of the measured matrix peak), not causal
+// 877 us, 1,254; back to back until the power cap holds the clock 513 and 978 us.  Tried:
+// a thread a row with its 128 columns (1,094 not causal, before the MMA warp became one
+// thread); a quarter or half of the
 // exponentials as a polynomial on the FMA pipe (no faster: registers spill).
 // ---------------------------------------------------------------------------
 constexpr int kRows = 128;                   // operand rows of a tile (MMA M)
@@ -126,7 +128,8 @@ __device__ __forceinline__ void store16x2(void* to, const uint32_t (&y)[8]) {
 }
 
 // A whole sector by one thread.  Rows lie apart, so a warp's store is 32 lines' work whatever its width, and half a sector at
-// a time was the larger part of a unit's end: 64 tokens 11.0 -> 9.4 us, 2,048 tokens 44.9 -> 41.9, 12 packed prompts 239 -> 217.
+// a time is a good part of a unit's end: 64 tokens 10.7 us with halves, 9.4 so; 2,048 tokens 47.1 and 45.0, 12 packed prompts 237
+// and 221, 77 queries after 9,000 keys 34.8 and 32.5.
 __device__ __forceinline__ void store32(void* to, const uint32_t (&y)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
                  "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
@@ -895,7 +898,11 @@ int run(const Params& p, cudaStream_t s) {
 
 // Sizes of the launch: the pairs of tiles (each sequence has at most one that is not full) and the parts of the keys.  With
 // fewer CTAs than half the SMs and keys enough, the keys are split so that every SM has a CTA, into parts of at
-// least 4 tiles (the mean sequence's) each.
+// least 4 tiles (the mean sequence's) each.  32/8 heads of 128, whole and as split: 64 queries (8 CTAs) after 1,024 keys 23.9 and
+// 21.3 us, after 8,192 keys 126 and 28; 512 queries (64 CTAs) after 1,024 keys 31.0 and 30.1, after 8,192 keys 133 and 81.  At 8
+// tiles the two are even (512 queries after 512 keys 24.1 and 25.9), below them whole is faster (256 after 512: 18.6, halved 20.0).
+// Parts shorter than 4 tiles would pay where CTAs are very few (64 queries after 2,048 keys 21.9, with 6 parts 19.0; 16 queries
+// 18.4 and with 9 parts 13.8).
 int plan(const rvq_prompt_attn_args& a, Params* p) {
     p->rep = a.n_heads / a.n_kv;
     p->tile_tokens = kRows / p->rep;

@@ -109,10 +109,12 @@ class Qwen3Decoder:
     the budget at which it overlaps the main stream best; 0: every SM).
     ``prompt_attention``: "engine" (the engine's ops: score matrices of the
     whole prompt, bit-identical logits) or "fused" (``PromptAttentionOp``:
-    one pass, scores and softmax in fp32, memory linear in the prompt).
+    one pass, scores and softmax in fp32, probabilities rounded to the
+    runtime type for the product with V, memory linear in the prompt).
     ``kv_cache``: "bf16", or "int4": keys and values held in 4 bits
     (rvq_b200/attention.py ``Cache4``; native step, head_dim 64 or 128),
-    scores and softmax of a step in fp32.  ``kv_budget`` (int4): rows that stay
+    scores and softmax of a step in fp32 (weights keep 16 bits for the
+    product with the codes).  ``kv_budget`` (int4): rows that stay
     in the cache: after every ``kv_slack`` steps whose live rows exceed it, the
     last ``kv_recent`` rows (None: half the budget) and those with the largest
     attention weight summed over the steps since the prompt are kept, per layer and kv head

@@ -103,7 +103,7 @@ struct Smem {
     int32_t fail[8];                         // of two warps of the same rows one has given up
     uint32_t tmem;
     int32_t dead;                            // a bounded wait gave up
-    int32_t busy;                            // warps that sum rows again
+    int32_t busy;                            // warps that do what may take long
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int c0, int c1, int c2, uint32_t bar) {
@@ -151,7 +151,7 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
 }
 
 // Bounded wait of a thread; once one wait of the CTA has given up, the others end at once.  The bound does not count while a warp
-// sums rows again (repair), which waits for nothing but may take long.
+// sums rows again (repair) or walks over empty sequences (find_work), which wait for nothing but may take long.
 template <int HD>
 __device__ __forceinline__ bool wait1(Smem<HD>& S, uint32_t bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -244,12 +244,13 @@ struct Cursor {
 };
 
 // Pair number `want` and part `split` of its keys, by one warp.  Pairs are counted from the last one of the last sequence
-// down; a CTA's numbers only rise, so over all its units it goes over the sequences once.
-__device__ __forceinline__ Work find_work(const Params& p, int want, int split, Cursor& at) {
+// down; a CTA's numbers only rise, so over all its units it goes over the sequences once.  *busy counts while that goes on.
+__device__ __forceinline__ Work find_work(const Params& p, int32_t* busy, int want, int split, Cursor& at) {
     const rvq_prompt_attn_args& a = p.a;
     const int lane = threadIdx.x & 31, T = p.tile_tokens;
     const int32_t* cu_k = a.cu_k != nullptr ? a.cu_k : a.cu_q;
     Work w = {};
+    bool far = false;
     for (; at.base < a.n_seq; at.base += 32) {
         const int b = a.n_seq - 1 - at.base - lane;
         int64_t q0 = 0, q1 = 0, k0 = 0, k1 = 0;
@@ -270,9 +271,12 @@ __device__ __forceinline__ Work find_work(const Params& p, int want, int split, 
         const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
         if (want >= before + total) {
             at.before += total;
+            if (!far && lane == 0) atomicAdd(busy, 1);       // a walk over many empty sequences may take long
+            far = true;
             continue;
         }
         const int l = __ffs(__ballot_sync(0xffffffffu, want < before + upto)) - 1;
+        if (far && lane == 0) atomicSub(busy, 1);
         w.live = 1;
         w.q0 = __shfl_sync(0xffffffffu, q0, l);
         w.k0 = __shfl_sync(0xffffffffu, k0, l);
@@ -294,6 +298,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int want, int split, 
         w.clean = w.lk % kKeys != 0 && total_tiles > 0 && (w.j0 + total_tiles) * kKeys > w.lk && w.k0 + w.lk < a.keys;
         return w;
     }
+    if (far && lane == 0) atomicSub(busy, 1);
     return w;
 }
 
@@ -439,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         if (unit < p.units) {
             const int split = unit % p.splits, rest = unit / p.splits;
             // the last pairs of a causal sequence see the most keys: they start first
-            w = find_work(p, rest / a.n_kv, split, cursor);
+            w = find_work(p, &S.busy, rest / a.n_kv, split, cursor);
             w.kv = rest % a.n_kv, w.split = split;
         }
         return w;

@@ -275,6 +275,21 @@ def test_prompt_many_sequences(cuda_device):
     prompt_case(cuda_device, [0] * 100 + [70] + [0] * 100, 16, 2, 128, HF, False, seed=7)
 
 
+def test_prompt_among_millions_of_empty_sequences(cuda_device):
+    """The walk from the last sequence to the first, over three million empty ones, is longer than the waits' bound may be."""
+    dev = cuda_device
+    g = gen(dev, 53)
+    q, k, v = randn(g, 500, 2, 64), randn(g, 500, 1, 64), randn(g, 500, 1, 64)
+    cu = torch.full((3_000_003,), 300, dtype=torch.int32, device=dev)
+    cu[0], cu[-1] = 0, 500
+    out = torch.zeros_like(q)
+    PromptAttentionOp(q, k, v, out, scaling=0.1, cu_q=cu).launch()
+    assert not take_timeout()
+    for a, b in ((0, 300), (300, 500)):
+        want, _, tol, _ = ref.attend(q[a:b], k[a:b], v[a:b], 0.1, True)
+        check(out[a:b], want, tol)
+
+
 def test_prompt_bad_offsets_stay_in_bounds(cuda_device):
     """Offsets beyond the tensors are cut off at them."""
     dev = cuda_device
